@@ -113,6 +113,72 @@ TKM_ATTN_API int tkm_attn_bwd_stage(int stage, const void *qkv, const void *o, c
                                     int dtype, void *workspace, size_t workspace_bytes,
                                     void *stream);
 
+/* ---- a paged key-value cache, and attention of one new token over it ----------------------
+ *
+ * No reference counterpart (it has no decoding path).  The operators of token generation, beside
+ * the forward that reads a prompt: tkm_attn_fwd gives the prompt's outputs, tkm_attn_kv_append
+ * stores its K and V, then each new token is one append and one tkm_attn_decode per layer.
+ *
+ * A cache is a pool of pages and, per sequence, a row of a table that names its pages:
+ *   k       [num_pages][Hkv][page/32][D/32][32 tokens][32 dims]   16-bit
+ *   v       [num_pages][Hkv][page/32][D/32][32 dims][32 tokens]   16-bit
+ *   table   [B][max_pages] int32: position j of sequence b is token j % page of page
+ *           table[b][j / page]; entries behind the last position in use are not read
+ *   len     [B] int32: tokens each sequence holds
+ *   weight  [B][Hkv][max_pages * page] fp32, or NULL: the attention weight each position of each
+ *           kv head has gathered (tkm_attn_decode adds to it, tkm_attn_kv_evict goes by it)
+ * page is 32, 64, 128 or 256.  Sequences may share pages that are only read.  Every pointer is a
+ * device pointer; k and v are 16-byte aligned, the others 4-byte.
+ * table and len are read on the device, so a captured call follows them from replay to replay,
+ * and no call checks them on the host.  The kernels do: a page outside [0, num_pages) is never
+ * touched, and a length outside [0, max_pages * page] is never walked.  A sequence with one of
+ * those that it needs gets O and LSE of NaN, loses the appended rows that fall there, is left as
+ * it is by the weights and by eviction, which gives it the length -1.
+ * Calls that write a cache must not overlap others on the same cache. */
+typedef struct {
+    void *k, *v;
+    const int32_t *table;
+    int32_t *len;
+    float *weight;
+    int B, Hkv, D, page, max_pages, num_pages, dtype;
+} tkm_attn_kv;
+
+/* Stores the K and V rows of qkv [B][S][(Hq + 2*Hkv) * D]: row i < n_new[b] of sequence b goes to
+ * position start[b] + i, and len[b] becomes start[b] + n_new[b].  start NULL is len itself (rows
+ * go behind what is there); n_new NULL is S, values are clamped to [0, S].  Positions that a table
+ * does not reach are dropped, the length counts them; a negative start stores nothing and gives
+ * the length -1.  Weights of the stored positions become 0. */
+TKM_ATTN_API int tkm_attn_kv_append(const tkm_attn_kv *kv, const void *qkv, int S, int Hq, const int32_t *start,
+                                    const int32_t *n_new, void *stream);
+
+/* Bytes of device workspace tkm_attn_decode needs for this cache (0 if it refuses the arguments):
+ * the pieces of rows that several workgroups share, at most 512 * 8 * min(Hq/Hkv, 32) * (D + 2)
+ * floats, and with add_weights the scores, B * Hq * (max_pages * page + 1) floats.  It holds
+ * nothing from call to call; calls that may overlap need one each. */
+TKM_ATTN_API size_t tkm_attn_decode_workspace_bytes(const tkm_attn_kv *kv, int Hq, int add_weights);
+
+/* Attention of one query row a sequence over its len[b] cached positions: o [B][Hq * D] and (if
+ * lse != NULL) lse [B][Hq].  q: B rows of Hq * D values, q_stride elements apart (a multiple of
+ * 8; the packed row of the new token serves as it is, q_stride = (Hq + 2*Hkv) * D).  A sequence
+ * of no tokens gets O = 0, LSE = -inf.  add_weights = 1 also adds, for every position j < len[b]
+ * and kv head, the sum over its query heads of exp(score_j - LSE) to weight.  Results do not
+ * depend on timing. */
+TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv *kv, const void *q, long long q_stride, void *o, float *lse,
+                                 int Hq, float scale, int add_weights, void *workspace, size_t workspace_bytes,
+                                 void *stream);
+
+/* Cuts every sequence of more than `budget` tokens to that many, each kv head by its own weights:
+ * it keeps the first `sink` and the last `recent` positions, and of those between them the
+ * budget - sink - recent with the largest weight (equal ones: the earlier position; a NaN counts
+ * as less than any other).  What is kept keeps its order, moves to positions 0 .. budget-1 with
+ * its weights, and len[b] becomes budget; shorter sequences keep everything.  kept
+ * [B][Hkv][budget] receives the old position of each new one, -1 behind the last.
+ * dst NULL or src: in place (the pages must not be shared with another sequence).  Otherwise src
+ * stays as it is and K, V, weights (if dst has any) and lengths go to dst, which has a table, len
+ * and weight of its own, of pages that no sequence of src uses, in the same pool or another. */
+TKM_ATTN_API int tkm_attn_kv_evict(const tkm_attn_kv *src, const tkm_attn_kv *dst, int32_t *kept, int budget,
+                                   int sink, int recent, void *stream);
+
 /* Loads this library's gfx950 assembly kernels (D = 128, fp16 and bf16) on the current device.  Call
  * it once per device before capturing a graph, as the runtime does at ignite; otherwise the
  * first call on a device loads them (inside a capture, with the thread's capture mode
@@ -127,7 +193,8 @@ TKM_ATTN_API int tkm_attn_init(void);
 /* 1 if the assembly kernels are loaded on the current device (gfx950), else 0. */
 TKM_ATTN_API int tkm_attn_asm_available(void);
 
-/* Kernels launched by the calling thread's last tkm_attn_fwd / _bwd / _bwd_stage call
+/* Kernels launched by the calling thread's last tkm_attn_fwd / _bwd / _bwd_stage /
+ * _decode / _kv_append / _kv_evict call
  * (OR of the bits below; 0 after a call that failed validation).  No reference counterpart. */
 enum {
     TKM_ATTN_K_FWD_ASM = 1,     /* tkm_fa_fwd_d128_f16 (assembly) */
@@ -136,7 +203,12 @@ enum {
     TKM_ATTN_K_DQ_HIP = 8,      /* fa_bwd_dq_kernel (HIP) */
     TKM_ATTN_K_DKDV_ASM = 16,   /* tkm_fa_bwd_dkdv_d128_f16 (assembly) */
     TKM_ATTN_K_DKDV_HIP = 32,   /* fa_bwd_dkdv_kernel (HIP) */
-    TKM_ATTN_K_DELTA_HIP = 64   /* fa_bwd_delta_kernel (HIP) */
+    TKM_ATTN_K_DELTA_HIP = 64,  /* fa_bwd_delta_kernel (HIP) */
+    TKM_ATTN_K_DECODE = 128,    /* decode_kernel */
+    TKM_ATTN_K_JOIN = 256,      /* join_kernel: rows that several workgroups of it shared */
+    TKM_ATTN_K_WEIGHTS = 512,   /* weights_kernel */
+    TKM_ATTN_K_APPEND = 1024,   /* append_*_kernel */
+    TKM_ATTN_K_EVICT = 2048     /* select_kernel, move_kernel */
 };
 TKM_ATTN_API unsigned tkm_attn_last_kernels(void);
 

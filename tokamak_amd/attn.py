@@ -29,6 +29,12 @@ _i = ctypes.c_int
 _lib = None
 
 
+class _Kv(ctypes.Structure):
+    """tkm_attn_kv"""
+    _fields_ = [(n, _vp) for n in ("k", "v", "table", "len", "weight")] + [
+        (n, _i) for n in ("B", "Hkv", "D", "page", "max_pages", "num_pages", "dtype")]
+
+
 class AttnError(RuntimeError):
     """A tkm_attn_* call returned a non-zero status."""
 
@@ -71,13 +77,23 @@ def lib() -> ctypes.CDLL:
     L.tkm_attn_init.restype = _i
     L.tkm_attn_asm_available.restype = _i
     L.tkm_attn_last_kernels.restype = ctypes.c_uint
+    kv = ctypes.POINTER(_Kv)
+    L.tkm_attn_kv_append.argtypes = [kv, _vp, _i, _i, _vp, _vp, _vp]
+    L.tkm_attn_kv_append.restype = _i
+    L.tkm_attn_decode_workspace_bytes.argtypes = [kv, _i, _i]
+    L.tkm_attn_decode_workspace_bytes.restype = ctypes.c_size_t
+    L.tkm_attn_decode.argtypes = [kv, _vp, ctypes.c_longlong, _vp, _vp, _i, ctypes.c_float, _i, _vp, ctypes.c_size_t, _vp]
+    L.tkm_attn_decode.restype = _i
+    L.tkm_attn_kv_evict.argtypes = [kv, kv, _vp, _i, _i, _i, _vp]
+    L.tkm_attn_kv_evict.restype = _i
     _lib = L
     return L
 
 
 # Bits of tkm_attn_last_kernels (include/tkm_attn.h)
 KERNEL_BITS = {"fwd_asm": 1, "fwd_hip": 2, "dq_asm": 4, "dq_hip": 8, "dkdv_asm": 16,
-               "dkdv_hip": 32, "delta_hip": 64}
+               "dkdv_hip": 32, "delta_hip": 64, "decode": 128, "join": 256, "weights": 512, "append": 1024,
+               "evict": 2048}
 
 
 def init() -> None:
@@ -203,6 +219,155 @@ def gqa_bwd(qkv, o, dout, lse, B, S, Hq, Hkv, D, causal=True, kv_len=None, scale
     return dqkv
 
 
+class KvCache:
+    """A paged key-value cache over the caller's tensors (tkm_attn_kv, include/tkm_attn.h):
+
+    k       [num_pages, Hkv, page/32, D/32, 32, 32]  float16 or bfloat16, blocks of 32 tokens x 32 dims
+    v       the same shape, its blocks 32 dims x 32 tokens
+    table   [B, max_pages] int32: the pages of each sequence
+    kv_len  [B] int32: the tokens each sequence holds
+    weight  [B, Hkv, max_pages * page] float32 or None: attention weight gathered by each position
+
+    The tensors stay the caller's, and are attributes here: write into them (a new page into the table, 0 into
+    kv_len for a slot that starts anew), do not replace them.  Caches may share a pool (k, v)."""
+
+    def __init__(self, k, v, table, kv_len, weight=None):
+        dev = k.device
+        if k.dim() != 6 or tuple(k.shape[4:]) != (32, 32) or v.shape != k.shape:
+            raise ValueError("k and v must be [num_pages, Hkv, page/32, D/32, 32, 32]")
+        if table.dim() != 2:
+            raise ValueError("table must be [B, max_pages]")
+        dt = _dtype_code(k)
+        num_pages, Hkv, page, D = k.shape[0], k.shape[1], 32 * k.shape[2], 32 * k.shape[3]
+        B, max_pages = table.shape
+        _check_tensor("k", k, k.numel(), dev)
+        _check_tensor("v", v, k.numel(), dev, k.dtype)
+        _check_dtype("table", table, B * max_pages, dev, "int32")
+        _check_dtype("kv_len", kv_len, B, dev, "int32")
+        if weight is not None:
+            _check_dtype("weight", weight, B * Hkv * max_pages * page, dev, "float32")
+        self.k, self.v, self.table, self.kv_len, self.weight = k, v, table, kv_len, weight
+        self.B, self.Hkv, self.D, self.page, self.max_pages, self.num_pages = B, Hkv, D, page, max_pages, num_pages
+        self.dtype, self.device = k.dtype, dev
+        self._c = _Kv(_ptr(k), _ptr(v), _ptr(table), _ptr(kv_len), _ptr(weight), B, Hkv, D, page, max_pages, num_pages, dt)
+        self._ref = ctypes.byref(self._c)
+        self._ws = {}
+
+    @classmethod
+    def empty(cls, B, max_pages, num_pages, Hkv, D, page=64, dtype=None, device="cuda", weights=False):
+        """A cache of sequences without tokens; every table entry is -1 until the caller names a page."""
+        import torch
+        if page % 32 or D % 32:
+            raise ValueError("page and D must be multiples of 32")
+        blocks = (num_pages, Hkv, page // 32, D // 32, 32, 32)
+        k, v = (torch.empty(blocks, dtype=dtype or torch.float16, device=device) for _ in range(2))
+        return cls(k, v, torch.full((B, max_pages), -1, dtype=torch.int32, device=device),
+                   torch.zeros(B, dtype=torch.int32, device=device),
+                   torch.zeros((B, Hkv, max_pages * page), device=device) if weights else None)
+
+
+def _check_dtype(name, t, numel, device, dtype):
+    import torch
+    _check_tensor(name, t, numel, device, getattr(torch, dtype))
+
+
+def _launch(device, stream):
+    """(stream handle, context to launch and allocate in) for tensors on `device`, which need not be the
+    current one; a given stream has to be that device's."""
+    import contextlib
+    import torch
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
+        return stream.cuda_stream, torch.cuda.stream(stream)
+    same = torch._C._cuda_getDevice() == device.index
+    return torch._C._cuda_getCurrentRawStream(device.index), _SAME if same else torch.cuda.device(device)
+
+
+class _Same:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *a):
+        pass
+
+
+_SAME = _Same()
+
+
+def kv_append(qkv, cache, Hq, start=None, n_new=None, stream=None):
+    """Stores the K and V rows of packed qkv [B, S, (Hq+2Hkv)*D] (or [B, (Hq+2Hkv)*D]: one row a sequence) behind
+    what the cache holds, or from positions start [B] int32 on; kv_len becomes the start plus n_new [B] int32
+    (None: S) rows.  Page the table first: rows on positions without a page are dropped."""
+    B, W = cache.B, (Hq + 2 * cache.Hkv) * cache.D
+    S = qkv.numel() // (B * W)
+    _check_tensor("qkv", qkv, B * S * W, cache.device, cache.dtype)
+    for name, t in (("start", start), ("n_new", n_new)):
+        if t is not None:
+            _check_dtype(name, t, B, cache.device, "int32")
+    st, ctx = _launch(cache.device, stream)
+    with ctx:
+        _check("tkm_attn_kv_append", lib().tkm_attn_kv_append(cache._ref, _ptr(qkv), S, Hq, _ptr(start), _ptr(n_new), st))
+
+
+def decode_workspace_bytes(cache, Hq, add_weights=False) -> int:
+    key = (Hq, bool(add_weights))
+    if key not in cache._ws:
+        cache._ws[key] = int(lib().tkm_attn_decode_workspace_bytes(cache._ref, Hq, int(key[1])))
+    return cache._ws[key]
+
+
+def gqa_decode(q, cache, Hq, scale=None, out=None, lse=None, add_weights=False, workspace=None, stream=None):
+    """O [B, Hq*D] and LSE [B, Hq] (fp32) of one query row a sequence over the cache.  q: [B, >= Hq*D] with the Q
+    heads first, rows any multiple of 8 elements apart; the packed row of the new token does as it is.
+    add_weights: also add the softmax weights of every cached position to cache.weight."""
+    import torch
+    B, D, dev = cache.B, cache.D, cache.device
+    if q.dim() != 2 or q.shape[0] != B or q.shape[1] < Hq * D or q.stride(1) != 1:
+        raise ValueError(f"q must be [{B}, at least {Hq * D}] with contiguous rows")
+    if q.device != dev or q.dtype != cache.dtype:
+        raise ValueError(f"q must be {cache.dtype} on {dev}")
+    st, ctx = _launch(dev, stream)
+    with ctx:
+        if out is None:
+            out = torch.empty((B, Hq * D), dtype=q.dtype, device=dev)
+        else:
+            _check_tensor("out", out, B * Hq * D, dev, q.dtype)
+        if lse is None:
+            lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+        else:
+            _check_tensor("lse", lse, B * Hq, dev, torch.float32)
+        if workspace is None:
+            wbytes = decode_workspace_bytes(cache, Hq, add_weights)
+            workspace = torch.empty(wbytes, dtype=torch.uint8, device=dev)
+        else:
+            _check_tensor("workspace", workspace, workspace.numel(), dev)
+            wbytes = workspace.numel() * workspace.element_size()
+        _check("tkm_attn_decode", lib().tkm_attn_decode(
+            cache._ref, _ptr(q), q.stride(0) if B > 1 else Hq * D, _ptr(out), _ptr(lse), Hq,
+            default_scale(D) if scale is None else float(scale), int(bool(add_weights)), _ptr(workspace), wbytes, st))
+    return out, lse
+
+
+def kv_evict(cache, budget, sink=0, recent=0, dst=None, kept=None, stream=None):
+    """Cuts sequences of more than `budget` tokens to the first `sink`, the last `recent` and, of the others, those
+    with the largest cache.weight, each kv head by its own; in place, or into the cache `dst`.  Returns kept
+    [B, Hkv, budget] int32: the old position of each new one, -1 behind the last."""
+    import torch
+    shape = (cache.B, cache.Hkv, budget)
+    if dst is not None and dst.device != cache.device:
+        raise ValueError(f"dst must be on {cache.device}")
+    st, ctx = _launch(cache.device, stream)
+    with ctx:
+        if kept is None:
+            kept = torch.empty(tuple(max(0, n) for n in shape), dtype=torch.int32, device=cache.device)
+        else:
+            _check_tensor("kept", kept, math.prod(shape), cache.device, torch.int32)
+        _check("tkm_attn_kv_evict", lib().tkm_attn_kv_evict(cache._ref, None if dst is None else dst._ref, _ptr(kept),
+                                                            budget, sink, recent, st))
+    return kept
+
+
 def attention_flops(B, S, Hq, D, causal, kv_len=None, mode="fwd") -> float:
     """Algorithmic FLOPs (FlashAttention convention): 4*B*Hq*S*Skv*D, halved if causal,
     x2.5 for the backward, x3.5 for forward+backward; with kv_len, S*Skv -> S*mean(kv_len)."""
@@ -211,6 +376,6 @@ def attention_flops(B, S, Hq, D, causal, kv_len=None, mode="fwd") -> float:
     return {"fwd": f, "bwd": 2.5 * f, "fwdbwd": 3.5 * f}[mode]
 
 
-__all__ = ["gqa_fwd", "gqa_bwd", "init", "asm_available", "last_kernels", "KERNEL_BITS", "bwd_workspace_bytes", "attention_flops", "default_scale",
+__all__ = ["gqa_fwd", "gqa_bwd", "KvCache", "kv_append", "gqa_decode", "kv_evict", "decode_workspace_bytes", "init", "asm_available", "last_kernels", "KERNEL_BITS", "bwd_workspace_bytes", "attention_flops", "default_scale",
            "lib", "header_functions", "AttnError", "F16", "BF16", "BWD_DELTA", "BWD_DKDV",
            "BWD_DQ", "BWD_DQ_DELTA"]

@@ -23,7 +23,8 @@ LIB_PATH = os.path.join(PKG, LIB_NAME)
 HIP_LIB_PATH = os.path.join(PKG, "libtkm_hip.so")
 RT_SOURCES = ["tkm_gemm.hip", "tkm_gemm_mfma.hip", "tkm_rt_kernels.hip"]
 RT_C_SOURCES = ["tkm_codegen_hip.c", "tkm_hip.c"]
-SOURCES = ["attn_fwd.hip", "attn_asm.hip", "attn_bwd.hip", "tkm_attn_abi.hip"]
+SOURCES = ["attn_fwd.hip", "attn_asm.hip", "attn_bwd.hip", "tkm_attn_abi.hip", "attn_decode.hip", "attn_kv.hip",
+           "tkm_kv_abi.hip"]
 # Hand-scheduled assembly kernels: (generator module, kernel symbol).  Each is generated,
 # assembled for gfx950 and embedded in the library as a code object (a C byte array).
 ASM_KERNELS = [("tokamak_amd.asmgen.attn_fwd", "tkm_fa_fwd_d128_f16"),

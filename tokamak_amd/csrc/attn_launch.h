@@ -36,9 +36,10 @@ struct BwdArgs {
 // include/tkm_attn.h.
 enum KernelBit : unsigned {
     kFwdAsm = 1u, kFwdHip = 2u, kDqAsm = 4u, kDqHip = 8u, kDkdvAsm = 16u, kDkdvHip = 32u,
-    kDeltaHip = 64u
+    kDeltaHip = 64u, kDecode = 128u, kJoin = 256u, kWeights = 512u, kAppend = 1024u, kEvict = 2048u
 };
 void note_kernels(unsigned bits);  // ORs bits into the calling thread's record
+void reset_kernels();              // clears it, at the start of a call
 
 // Assembly code objects: load on the current device (0, or -2 with asm_load_error()),
 // and whether the assembly path exists there (gfx950, loaded).

@@ -18,6 +18,7 @@ namespace {
 thread_local unsigned t_kernels = 0;  // kernels launched by this thread's current/last call
 }  // namespace
 void note_kernels(unsigned bits) { t_kernels |= bits; }
+void reset_kernels() { t_kernels = 0; }
 }  // namespace tkm
 
 // Backward workspace of tkm_attn_bwd_noalloc: a static device array, one per GPU (each
