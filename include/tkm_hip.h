@@ -9,6 +9,7 @@
  *     (a language model's next-token loss; the reference uploads B uint8 labels,
  *     src/tkm_gpu.cu:1495), the weight-initialization seed;
  *   - a step on inputs already in device memory (benchmarks, resident data);
+ *   - the draw of the next token from logits (temperature, top-k, top-p, min-p);
  *   - accessors of device buffers for tests.
  */
 #ifndef TKM_HIP_H
@@ -102,6 +103,41 @@ TKM_API int tkm_runtime_upload(TkmRuntime *rt, const float *h_input, const void 
 
 /* Loss of the last step (synchronizes). */
 TKM_API float tkm_runtime_last_loss(TkmRuntime *rt);
+
+/* ---- the next token -----------------------------------------------------------------------
+ * No reference counterpart.  One token a row of logits, drawn from a given random number:
+ *   w_i = exp((l_i - max) / temperature); order: larger logits first, equal ones by index;
+ *   top_k keeps the first k; top_p of these the shortest head whose sum reaches top_p of theirs;
+ *   min_p of these the ones with w_i >= min_p; the token is the first i, in the vocabulary's
+ *   order, at which the running sum of the kept w exceeds u times their sum.
+ * A setting array that is NULL is off (temperature 1); so are top_k <= 0 or >= vocab, top_p >= 1
+ * and min_p <= 0.  The largest logit always stays.  temperature <= 0 takes the largest logit, of
+ * equal ones the first.  A NaN logit counts as -inf; a row of nothing but -inf gives -1.  u is in
+ * [0, 1), other values act as the nearest.  The sums are integers of 2^-45 (at 131072 words; finer
+ * for fewer), so that a draw depends neither on timing nor on the order of a sum. */
+enum { TKM_SAMPLE_F32 = 2 };             /* logits in fp32, beside TKM_ATTN_F16 and TKM_ATTN_BF16 */
+
+typedef struct {
+    const void *logits;                  /* `rows` rows of `vocab`, row_stride elements apart */
+    size_t row_stride;
+    int rows, vocab, dtype, draws;       /* vocab at most 524288 */
+    const int32_t *row_index;            /* [draws]: the row of each draw, -1 gives -1; NULL: row r for draw r */
+    const float *temperature;            /* each [draws] or NULL */
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    const float *u;                      /* [draws] */
+    int32_t *token;                      /* [draws], written */
+} tkm_sample_args;
+
+/* Device pointers; asynchronous on `stream`, allocates nothing, may be captured.  Returns
+ * TKM_ATTN_OK or a status, tkm_attn_last_error() describes it. */
+TKM_API int tkm_hip_sample(const tkm_sample_args *s, void *stream);
+
+/* tkm_runtime_forward on h_input, then `draws` draws from rows of its output on the device: only
+ * the tokens come back.  h->row_index (NULL: rows 0..draws-1), the settings, u and token are host
+ * arrays; logits, row_stride, rows, vocab and dtype of h are not read.  A row index outside the
+ * output draws -1.  Returns 0 or -1. */
+TKM_API int tkm_runtime_sample(TkmRuntime *rt, const float *h_input, const tkm_sample_args *h);
 
 /* Device buffers: the runtime's stream; a node's activation (grad = 0) or gradient (grad = 1)
  * slot of the arena; learnable tensor i (in TKM1 file order): master, 16-bit copy (or NULL),

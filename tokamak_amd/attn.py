@@ -112,9 +112,9 @@ def last_kernels() -> list:
     return [n for n, b in KERNEL_BITS.items() if bits & b]
 
 
-def _check(fn: str, rc: int) -> None:
+def _check(fn: str, rc: int, L=None) -> None:
     if rc != 0:
-        raise AttnError(fn, rc, lib().tkm_attn_last_error().decode())
+        raise AttnError(fn, rc, (L or lib()).tkm_attn_last_error().decode())
 
 
 @functools.lru_cache(maxsize=64)

@@ -145,6 +145,8 @@ struct TkmRuntime {
     hipGraph_t step_graph[2];        /* [0] clears the loss, [1] accumulates it (epochs) */
     hipGraphExec_t step_exec[2];
     float *d_out_f32;                /* tkm_runtime_forward's fp32 copy of the output node */
+    uint32_t *d_draw, *h_draw;       /* tkm_runtime_sample's settings and tokens, of draw_cap draws */
+    int draw_cap;
     float *h_stage_in;               /* pinned batch staging of the callback loops */
     uint8_t *h_stage_lbl;
     float last_lr;
@@ -1213,6 +1215,70 @@ size_t tkm_runtime_forward(TkmRuntime *rt, const float *h_input, float *h_output
     return n;
 }
 
+/* The arrays of `draws` 32-bit words each go to the device in one copy: row index, temperature, top_k,
+ * top_p, min_p, u (those given), and the tokens come back from behind them. */
+int tkm_runtime_sample(TkmRuntime *rt, const float *h_input, const tkm_sample_args *h) {
+    const char *why = NULL;
+    if (!rt || !h_input || !h || !h->u || !h->token) why = "a runtime, an input, u and token are required";
+    else if (tkm_runtime_output_elements(rt) == 0) why = "the graph ends in a loss, which has no inference output";
+    else if (h->draws < 1 || h->draws > (1 << 24)) why = "the number of draws must be positive (at most 2^24)";
+    else if (!h->row_index && (size_t)h->draws > rows_of(&rt->graph, &rt->graph.nodes[output_node(&rt->graph)]))
+        why = "more draws than rows of output need a row_index";
+    if (why) {
+        fprintf(stderr, "[TKM HIP] tkm_runtime_sample: %s\n", why);
+        return -1;
+    }
+    const size_t n = (size_t)h->draws;
+    if (h->draws > rt->draw_cap) {
+        hipFree(rt->d_draw);
+        free(rt->h_draw);
+        rt->d_draw = NULL;
+        rt->draw_cap = 0;
+        rt->h_draw = (uint32_t *)malloc(7 * n * 4);
+        if (!rt->h_draw || !HIP_OK(hipMalloc((void **)&rt->d_draw, 7 * n * 4))) return -1;
+        rt->draw_cap = h->draws;
+    }
+    const void *given[6] = {h->row_index, h->temperature, h->top_k, h->top_p, h->min_p, h->u};
+    const void *dev[6];
+    size_t at = 0;
+    for (int i = 0; i < 6; ++i) {
+        dev[i] = given[i] ? rt->d_draw + at : NULL;
+        if (!given[i]) continue;
+        memcpy(rt->h_draw + at, given[i], n * 4);
+        at += n;
+    }
+    const TkmNode *out = &rt->graph.nodes[output_node(&rt->graph)];
+    tkm_sample_args d;
+    memset(&d, 0, sizeof d);
+    d.logits = act(rt, output_node(&rt->graph));
+    d.row_stride = (size_t)out->C;
+    d.rows = (int)rows_of(&rt->graph, out);
+    d.vocab = out->C;
+    d.dtype = rt->dt;
+    d.draws = h->draws;
+    d.row_index = (const int32_t *)dev[0];
+    d.temperature = (const float *)dev[1];
+    d.top_k = (const int32_t *)dev[2];
+    d.top_p = (const float *)dev[3];
+    d.min_p = (const float *)dev[4];
+    d.u = (const float *)dev[5];
+    d.token = (int32_t *)(rt->d_draw + at);
+    if (!HIP_OK(hipMemcpyAsync(rt->d_draw, rt->h_draw, at * 4, hipMemcpyHostToDevice, rt->stream)) ||
+        tkm_runtime_upload(rt, h_input, NULL, 0))
+        return -1;
+    rt->failed = 0;
+    forward_pass(rt, 1, rt->graph.batch_size);
+    if (rt->failed) return -1;
+    if (tkm_hip_sample(&d, rt->stream)) {
+        fprintf(stderr, "[TKM HIP] tkm_runtime_sample: %s\n", tkm_attn_last_error());
+        return -1;
+    }
+    if (!HIP_OK(hipMemcpyAsync(h->token, d.token, n * 4, hipMemcpyDeviceToHost, rt->stream)) ||
+        !HIP_OK(hipStreamSynchronize(rt->stream)))
+        return -1;
+    return 0;
+}
+
 float tkm_eval_current_loss(TkmRuntime *rt) {
     if (!rt) return NAN;
     if (tkm_rt_fill_u32(rt->d_loss, 4, 0, rt->stream)) return NAN;
@@ -1718,6 +1784,8 @@ static void free_runtime(TkmRuntime *rt) {
     hipFree(rt->d_sgd);
     free(rt->clear);
     hipFree(rt->d_out_f32);
+    hipFree(rt->d_draw);
+    free(rt->h_draw);
     if (rt->h_stage_in) hipHostFree(rt->h_stage_in);
     if (rt->h_stage_lbl) hipHostFree(rt->h_stage_lbl);
     if (rt->h_pin_lr) hipHostFree(rt->h_pin_lr);

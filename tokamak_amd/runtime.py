@@ -32,6 +32,13 @@ class Opts(ctypes.Structure):
                 ("verbose", _i), ("dataset_mode", _i), ("clear_all_grads", _i)]
 
 
+class _SampleArgs(ctypes.Structure):
+    """tkm_sample_args"""
+    _fields_ = [("logits", _vp), ("row_stride", _sz), ("rows", _i), ("vocab", _i), ("dtype", _i), ("draws", _i),
+                ("row_index", _vp), ("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("u", _vp),
+                ("token", _vp)]
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is not None:
@@ -81,6 +88,8 @@ def lib() -> ctypes.CDLL:
                                 ctypes.POINTER(_sz), ctypes.POINTER(_i)], _i),
         "tkm_runtime_node_save": ([_vp, _i, _i], _vp),
         "tkm_runtime_step_kernel_count": ([_vp], _i),
+        "tkm_hip_sample": ([ctypes.POINTER(_SampleArgs), _vp], _i),
+        "tkm_runtime_sample": ([_vp, _vp, ctypes.POINTER(_SampleArgs)], _i),
         "tkm_attn_last_error": ([], ctypes.c_char_p),
     }
     for name, (args, res) in sig.items():
@@ -203,6 +212,28 @@ class Runtime:
             raise RuntimeError("tkm_runtime_forward failed")
         return out
 
+    def sample(self, x, u, rows=None, temperature=None, top_k=None, top_p=None, min_p=None) -> np.ndarray:
+        """forward(x), then one token for each of the host numbers u, drawn on the device (tkm_runtime_sample) from
+        the output's rows `rows` (None: the first ones).  A setting is None, a number for all, or one a draw."""
+        u = np.ascontiguousarray(u, np.float32).reshape(-1)
+        n, keep = u.size, []
+
+        def arg(v, dtype):
+            if v is None:
+                return None
+            v = np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype), (n,)))
+            keep.append(v)
+            return v.ctypes.data
+
+        x, token = np.ascontiguousarray(x, np.float32), np.empty(n, np.int32)
+        if x.size != self.input_elements:
+            raise ValueError(f"x has {x.size} elements, the runtime takes {self.input_elements}")
+        a = _SampleArgs(None, 0, 0, 0, 0, n, arg(rows, np.int32), arg(temperature, np.float32), arg(top_k, np.int32),
+                        arg(top_p, np.float32), arg(min_p, np.float32), u.ctypes.data, token.ctypes.data)
+        if lib().tkm_runtime_sample(self.rt, x.ctypes.data, ctypes.byref(a)):
+            raise RuntimeError("tkm_runtime_sample failed (see stderr)")
+        return token
+
     def eval(self, x, labels, count: int) -> int:
         x = np.ascontiguousarray(x, np.float32)
         lab = np.ascontiguousarray(labels, np.uint8)
@@ -243,6 +274,36 @@ class Runtime:
         return int(lib().tkm_runtime_step_kernel_count(self.rt))
 
 
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, row_index=None, out=None, stream=None):
+    """Tokens [draws] int32 drawn from device logits [rows, vocab] (float16, bfloat16 or float32; rows may be
+    apart) by the numbers u [draws] float32 in [0, 1): tkm_hip_sample, include/tkm_hip.h.  temperature, top_p, min_p
+    (float32), top_k and row_index (int32) are device tensors [draws] or None."""
+    import torch
+    dev, n = logits.device, u.numel()
+    code = {torch.float16: attn.F16, torch.bfloat16: attn.BF16, torch.float32: 2}.get(logits.dtype)
+    if code is None:
+        raise TypeError(f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
+    if not logits.is_cuda:
+        raise ValueError("logits must be on a device")
+    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError("logits must be [rows, vocab] with contiguous rows")
+    for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("row_index", row_index, torch.int32),
+                        ("out", out, torch.int32)):
+        if t is not None:
+            attn._check_tensor(name, t, n, dev, dt)
+    rows, vocab = logits.shape
+    st, ctx = attn._launch(dev, stream)
+    with ctx:
+        if out is None:
+            out = torch.empty(n, dtype=torch.int32, device=dev)
+        p = attn._ptr
+        a = _SampleArgs(p(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab, code, n, p(row_index), p(temperature),
+                        p(top_k), p(top_p), p(min_p), p(u), p(out))
+        attn._check("tkm_hip_sample", lib().tkm_hip_sample(ctypes.byref(a), st), lib())
+    return out
+
+
 def parse_weights(data: bytes) -> list:
     """The float arrays of a TKM1 weight file (magic 0x544B4D31, count, then size + values)."""
     magic, nt = np.frombuffer(data[:8], np.uint32)
@@ -267,5 +328,5 @@ def encode_weights(arrays) -> bytes:
     return b"".join(parts)
 
 
-__all__ = ["lib", "graph_buffer", "codegen", "Runtime", "parse_weights", "encode_weights", "header_functions",
+__all__ = ["lib", "graph_buffer", "codegen", "Runtime", "sample", "parse_weights", "encode_weights", "header_functions",
            "GROUP_PREP", "GROUP_PLASMA", "SIZEOF_GRAPH"]
