@@ -151,10 +151,10 @@ typedef struct {
 TKM_ATTN_API int tkm_attn_kv_append(const tkm_attn_kv *kv, const void *qkv, int S, int Hq, const int32_t *start,
                                     const int32_t *n_new, void *stream);
 
-/* Bytes of device workspace tkm_attn_decode needs for this cache (0 if it refuses the arguments):
- * the pieces of rows that several workgroups share, at most 512 * 8 * min(Hq/Hkv, 32) * (D + 2)
- * floats, and with add_weights the scores, B * Hq * (max_pages * page + 1) floats.  It holds
- * nothing from call to call; calls that may overlap need one each. */
+/* Bytes of device workspace tkm_attn_decode needs for this cache: the pieces of rows that several
+ * workgroups share, at most 512 * 8 * 16 * (D + 2) floats (none for tables of few tokens), and with
+ * add_weights the scores, B * Hq * (max_pages * page + 1) floats.  0 also if it refuses the
+ * arguments.  It holds nothing from call to call; calls that may overlap need one each. */
 TKM_ATTN_API size_t tkm_attn_decode_workspace_bytes(const tkm_attn_kv *kv, int Hq, int add_weights);
 
 /* Attention of one query row a sequence over its len[b] cached positions: o [B][Hq * D] and (if

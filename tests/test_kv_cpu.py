@@ -75,7 +75,6 @@ def test_append_refuses(kw, status, msg):
     (dict(stride=248), EINVAL, b"q_stride"), (dict(stride=260), EINVAL, b"q_stride"), (dict(q=P + 8), EALIGN, b"aligned"),
     (dict(o=P + 8), EALIGN, b"aligned"), (dict(lse=P + 2), EALIGN, b"aligned"), (dict(scale=0.0), EINVAL, b"scale"),
     (dict(scale=float("nan")), EINVAL, b"scale"), (dict(scale=float("inf")), EINVAL, b"scale"), (dict(add=2), EINVAL, b"add_weights"),
-    (dict(ws=None), EWORKSPACE, b"workspace"), (dict(wsb=16), EWORKSPACE, b"workspace"), (dict(ws=P + 4), EALIGN, b"aligned"),
     (dict(Hq=1 << 24), EUNSUPPORTED, b"too large"),
 ])
 def test_decode_refuses(kw, status, msg):
@@ -88,10 +87,18 @@ def test_decode_refuses_weights_without_room_for_them():
     assert decode(kv(max_pages=1 << 22, page=256, B=64), wsb=1 << 40) == EUNSUPPORTED
 
 
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(ws=None), EWORKSPACE, b"workspace"), (dict(wsb=16), EWORKSPACE, b"workspace"), (dict(ws=P + 4), EALIGN, b"aligned")])
+@pytest.mark.parametrize("add", [0, 1])
+def test_decode_refuses_a_workspace(kw, status, msg, add):
+    assert decode(kv(max_pages=100 if not add else 1), add=add, **kw) == status
+    assert msg in attn.lib().tkm_attn_last_error()
+
+
 def test_decode_workspace():
     L = attn.lib()
     small, large = kv(max_pages=1), kv(max_pages=1000)
-    assert 0 < L.tkm_attn_decode_workspace_bytes(ref(small), 4, 0) < L.tkm_attn_decode_workspace_bytes(ref(large), 4, 0)
+    assert 0 == L.tkm_attn_decode_workspace_bytes(ref(small), 4, 0) < L.tkm_attn_decode_workspace_bytes(ref(large), 4, 0)
     assert L.tkm_attn_decode_workspace_bytes(ref(large), 4, 0) <= 512 * 8 * 2 * 66 * 4 + 4096
     assert L.tkm_attn_decode_workspace_bytes(ref(small), 4, 1) >= 2 * 4 * 65 * 4
     assert L.tkm_attn_decode_workspace_bytes(ref(kv(D=80)), 4, 0) == 0

@@ -24,7 +24,7 @@ def q_of(case, Hq, seed=7, packed=False, mul=1.0):
 @pytest.mark.parametrize("lens", LENS)
 @pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [
     (4, 4, 64, 32, "f16"), (8, 2, 128, 64, "bf16"), (32, 2, 128, 128, "f16"), (3, 1, 64, 256, "bf16"),
-    (40, 1, 64, 64, "f16"), (34, 2, 128, 32, "bf16")])
+    (40, 1, 64, 64, "f16"), (34, 2, 128, 32, "bf16"), (100, 1, 64, 64, "f16"), (130, 2, 128, 128, "bf16")])
 def test_decode(gpu, lens, Hq, Hkv, D, page, dtype):
     from tokamak_amd import attn
     print(f"[case] {lens} Hq{Hq} Hkv{Hkv} D{D} page{page} {dtype}", flush=True)
@@ -37,7 +37,7 @@ def test_decode(gpu, lens, Hq, Hkv, D, page, dtype):
     assert torch.equal(o, o2) and torch.equal(lse, lse2)
 
 
-@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [(4, 4, 64, 32, "f16"), (8, 2, 128, 64, "bf16"), (20, 1, 128, 128, "f16")])
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [(4, 4, 64, 32, "f16"), (8, 2, 128, 64, "bf16"), (20, 1, 128, 128, "f16"), (70, 1, 64, 32, "bf16")])
 @pytest.mark.parametrize("lens", ["edges", "ragged", "long", "many"])
 def test_weights(gpu, lens, Hq, Hkv, D, page, dtype):
     from tokamak_amd import attn

@@ -271,43 +271,56 @@ def _check_dtype(name, t, numel, device, dtype):
     _check_tensor(name, t, numel, device, getattr(torch, dtype))
 
 
-def _launch(device, stream):
-    """(stream handle, context to launch and allocate in) for tensors on `device`, which need not be the
-    current one; a given stream has to be that device's."""
-    import contextlib
-    import torch
-    if stream is not None:
-        if stream.device != device:
+class _On:
+    """Where a call on tensors of one device launches and allocates: the device, which need not be the current
+    one, on its current stream or the given one, which has to be that device's."""
+    __slots__ = ("handle", "ctx")
+
+    def __init__(self, device, stream):
+        import torch
+        if stream is not None and stream.device != device:
             raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
-        return stream.cuda_stream, torch.cuda.stream(stream)
-    same = torch._C._cuda_getDevice() == device.index
-    return torch._C._cuda_getCurrentRawStream(device.index), _SAME if same else torch.cuda.device(device)
+        self.ctx = torch.cuda.device(device) if stream is None else torch.cuda.stream(stream)
+        self.handle = torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream.cuda_stream
 
-
-class _Same:
     def __enter__(self):
-        pass
+        self.ctx.__enter__()
+        return self.handle
 
     def __exit__(self, *a):
-        pass
+        return self.ctx.__exit__(*a)
 
 
-_SAME = _Same()
+def _current(device, stream):
+    """The current stream's handle, or None if the call has to change device or stream (_On) first."""
+    if stream is not None:
+        return None
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index) if torch._C._cuda_getDevice() == device.index else None
 
 
 def kv_append(qkv, cache, Hq, start=None, n_new=None, stream=None):
     """Stores the K and V rows of packed qkv [B, S, (Hq+2Hkv)*D] (or [B, (Hq+2Hkv)*D]: one row a sequence) behind
     what the cache holds, or from positions start [B] int32 on; kv_len becomes the start plus n_new [B] int32
     (None: S) rows.  Page the table first: rows on positions without a page are dropped."""
-    B, W = cache.B, (Hq + 2 * cache.Hkv) * cache.D
-    S = qkv.numel() // (B * W)
-    _check_tensor("qkv", qkv, B * S * W, cache.device, cache.dtype)
-    for name, t in (("start", start), ("n_new", n_new)):
-        if t is not None:
-            _check_dtype(name, t, B, cache.device, "int32")
-    st, ctx = _launch(cache.device, stream)
-    with ctx:
-        _check("tkm_attn_kv_append", lib().tkm_attn_kv_append(cache._ref, _ptr(qkv), S, Hq, _ptr(start), _ptr(n_new), st))
+    st = _current(cache.device, stream)
+    if st is None:
+        with _On(cache.device, stream) as st:
+            return _kv_append(qkv, cache, Hq, start, n_new, st)
+    return _kv_append(qkv, cache, Hq, start, n_new, st)
+
+
+def _kv_append(qkv, cache, Hq, start, n_new, st):
+    dev, B = cache.device, cache.B
+    row = B * (Hq + 2 * cache.Hkv) * cache.D
+    n = qkv.numel()
+    S = n // row if row > 0 else 0
+    _check_tensor("qkv", qkv, S * row if S else row, dev, cache.dtype)
+    if start is not None:
+        _check_tensor("start", start, B, dev, cache.kv_len.dtype)
+    if n_new is not None:
+        _check_tensor("n_new", n_new, B, dev, cache.kv_len.dtype)
+    _check("tkm_attn_kv_append", lib().tkm_attn_kv_append(cache._ref, qkv.data_ptr(), S, Hq, _ptr(start), _ptr(n_new), st))
 
 
 def decode_workspace_bytes(cache, Hq, add_weights=False) -> int:
@@ -321,31 +334,41 @@ def gqa_decode(q, cache, Hq, scale=None, out=None, lse=None, add_weights=False, 
     """O [B, Hq*D] and LSE [B, Hq] (fp32) of one query row a sequence over the cache.  q: [B, >= Hq*D] with the Q
     heads first, rows any multiple of 8 elements apart; the packed row of the new token does as it is.
     add_weights: also add the softmax weights of every cached position to cache.weight."""
+    st = _current(cache.device, stream)
+    if st is None:
+        with _On(cache.device, stream) as st:
+            return _gqa_decode(q, cache, Hq, scale, out, lse, add_weights, workspace, st)
+    return _gqa_decode(q, cache, Hq, scale, out, lse, add_weights, workspace, st)
+
+
+def _gqa_decode(q, cache, Hq, scale, out, lse, add_weights, workspace, st):
     import torch
     B, D, dev = cache.B, cache.D, cache.device
-    if q.dim() != 2 or q.shape[0] != B or q.shape[1] < Hq * D or q.stride(1) != 1:
+    rows, stride = q.shape, q.stride()
+    if len(rows) != 2 or rows[0] != B or rows[1] < Hq * D or stride[1] != 1:
         raise ValueError(f"q must be [{B}, at least {Hq * D}] with contiguous rows")
     if q.device != dev or q.dtype != cache.dtype:
         raise ValueError(f"q must be {cache.dtype} on {dev}")
-    st, ctx = _launch(dev, stream)
-    with ctx:
-        if out is None:
-            out = torch.empty((B, Hq * D), dtype=q.dtype, device=dev)
-        else:
-            _check_tensor("out", out, B * Hq * D, dev, q.dtype)
-        if lse is None:
-            lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
-        else:
-            _check_tensor("lse", lse, B * Hq, dev, torch.float32)
-        if workspace is None:
-            wbytes = decode_workspace_bytes(cache, Hq, add_weights)
+    if out is None:
+        out = q.new_empty((B, max(0, Hq * D)))
+    else:
+        _check_tensor("out", out, B * Hq * D, dev, q.dtype)
+    if lse is None:
+        lse = torch.empty((B, max(0, Hq)), dtype=torch.float32, device=dev)
+    else:
+        _check_tensor("lse", lse, B * Hq, dev, torch.float32)
+    if workspace is None:
+        wbytes = decode_workspace_bytes(cache, Hq, add_weights)
+        if wbytes:
             workspace = torch.empty(wbytes, dtype=torch.uint8, device=dev)
-        else:
-            _check_tensor("workspace", workspace, workspace.numel(), dev)
-            wbytes = workspace.numel() * workspace.element_size()
-        _check("tkm_attn_decode", lib().tkm_attn_decode(
-            cache._ref, _ptr(q), q.stride(0) if B > 1 else Hq * D, _ptr(out), _ptr(lse), Hq,
-            default_scale(D) if scale is None else float(scale), int(bool(add_weights)), _ptr(workspace), wbytes, st))
+    else:
+        _check_tensor("workspace", workspace, workspace.numel(), dev)
+        wbytes = workspace.numel() * workspace.element_size()
+    rc = lib().tkm_attn_decode(cache._ref, q.data_ptr(), stride[0] if B > 1 else Hq * D, out.data_ptr(), lse.data_ptr(), Hq,
+                               default_scale(D) if scale is None else scale, 1 if add_weights else 0, _ptr(workspace),
+                               wbytes, st)
+    if rc:
+        _check("tkm_attn_decode", rc)
     return out, lse
 
 
@@ -353,18 +376,22 @@ def kv_evict(cache, budget, sink=0, recent=0, dst=None, kept=None, stream=None):
     """Cuts sequences of more than `budget` tokens to the first `sink`, the last `recent` and, of the others, those
     with the largest cache.weight, each kv head by its own; in place, or into the cache `dst`.  Returns kept
     [B, Hkv, budget] int32: the old position of each new one, -1 behind the last."""
-    import torch
-    shape = (cache.B, cache.Hkv, budget)
+    st = _current(cache.device, stream)
+    if st is None:
+        with _On(cache.device, stream) as st:
+            return _kv_evict(cache, budget, sink, recent, dst, kept, st)
+    return _kv_evict(cache, budget, sink, recent, dst, kept, st)
+
+
+def _kv_evict(cache, budget, sink, recent, dst, kept, st):
     if dst is not None and dst.device != cache.device:
         raise ValueError(f"dst must be on {cache.device}")
-    st, ctx = _launch(cache.device, stream)
-    with ctx:
-        if kept is None:
-            kept = torch.empty(tuple(max(0, n) for n in shape), dtype=torch.int32, device=cache.device)
-        else:
-            _check_tensor("kept", kept, math.prod(shape), cache.device, torch.int32)
-        _check("tkm_attn_kv_evict", lib().tkm_attn_kv_evict(cache._ref, None if dst is None else dst._ref, _ptr(kept),
-                                                            budget, sink, recent, st))
+    if kept is None:
+        kept = cache.kv_len.new_empty((cache.B, cache.Hkv, max(0, budget)))
+    else:
+        _check_tensor("kept", kept, cache.B * cache.Hkv * budget, cache.device, cache.kv_len.dtype)
+    _check("tkm_attn_kv_evict", lib().tkm_attn_kv_evict(cache._ref, None if dst is None else dst._ref, kept.data_ptr(), budget,
+                                                        sink, recent, st))
     return kept
 
 

@@ -133,6 +133,30 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// Inclusive sums over the wave's lanes 0..l by DPP (6 adds; a shuffle through LDS takes about 100 clocks a step).
+// All 64 lanes take part.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T scan_step(T v) {
+    if constexpr (sizeof(T) == 8)
+        return v + (T)(((uint64_t)dpp_or_0<CTRL, ROWS>((uint32_t)((uint64_t)v >> 32)) << 32) | dpp_or_0<CTRL, ROWS>((uint32_t)v));
+    else
+        return v + (T)dpp_or_0<CTRL, ROWS>((uint32_t)v);
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v = scan_step<0x111, 0xf>(v);   // from the lane 1, 2, 4, 8 below, within rows of 16
+    v = scan_step<0x112, 0xf>(v);
+    v = scan_step<0x114, 0xf>(v);
+    v = scan_step<0x118, 0xf>(v);
+    v = scan_step<0x142, 0xa>(v);   // row 0's last lane to row 1, row 2's to row 3
+    return scan_step<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
 // ---------------------------------------------------------------------------
 // Instruction-schedule shaping (LLVM sched_group_barrier masks).  A stage that reads N LDS
 // operands and issues M MFMAs per read is ordered as: LEAD reads, then (M MFMAs, 1 read)

@@ -100,10 +100,10 @@ TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv* kv, const void* q, long long
     if (add_weights && (double)kv->B * kv->Hkv * (kv->max_pages * (double)kv->page / 1024 + 1) > kGridMost)
         return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
     const size_t need = tkm::decode_workspace(*kv, Hq, add_weights);
-    if (!workspace || workspace_bytes < need)
+    if (need && (!workspace || workspace_bytes < need))
         return fail(TKM_ATTN_EWORKSPACE, "workspace of %zu bytes required, %zu given", need,
                     workspace ? workspace_bytes : (size_t)0);
-    if (!aligned(workspace, 16)) return fail(TKM_ATTN_EALIGN, "workspace must be 16-byte aligned");
+    if (need && !aligned(workspace, 16)) return fail(TKM_ATTN_EALIGN, "workspace must be 16-byte aligned");
     const tkm::DecodeArgs a{*kv, q, q_stride, o, lse, Hq, scale, add_weights, workspace, stream};
     if (tkm::launch_decode(a)) return fail(TKM_ATTN_ELAUNCH, "decode: kernel launch failed");
     return TKM_ATTN_OK;

@@ -274,33 +274,46 @@ class Runtime:
         return int(lib().tkm_runtime_step_kernel_count(self.rt))
 
 
+_LOGITS = {}
+
+
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, row_index=None, out=None, stream=None):
     """Tokens [draws] int32 drawn from device logits [rows, vocab] (float16, bfloat16 or float32; rows may be
     apart) by the numbers u [draws] float32 in [0, 1): tkm_hip_sample, include/tkm_hip.h.  temperature, top_p, min_p
     (float32), top_k and row_index (int32) are device tensors [draws] or None."""
+    if not logits.is_cuda and logits.is_floating_point() and logits.element_size() < 8:
+        raise ValueError("logits must be on a device")
+    st = attn._current(logits.device, stream) if logits.is_cuda else 0
+    if st is None:
+        with attn._On(logits.device, stream) as st:
+            return _sample(logits, u, temperature, top_k, top_p, min_p, row_index, out, st)
+    return _sample(logits, u, temperature, top_k, top_p, min_p, row_index, out, st)
+
+
+def _sample(logits, u, temperature, top_k, top_p, min_p, row_index, out, st):
     import torch
-    dev, n = logits.device, u.numel()
-    code = {torch.float16: attn.F16, torch.bfloat16: attn.BF16, torch.float32: 2}.get(logits.dtype)
+    if not _LOGITS:
+        _LOGITS.update({torch.float16: attn.F16, torch.bfloat16: attn.BF16, torch.float32: 2})
+    dev, n, code = logits.device, u.numel(), _LOGITS.get(logits.dtype)
     if code is None:
         raise TypeError(f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
-    if not logits.is_cuda:
-        raise ValueError("logits must be on a device")
-    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or stride[1] != 1 and shape[1] > 1:
         raise ValueError("logits must be [rows, vocab] with contiguous rows")
-    for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("row_index", row_index, torch.int32),
-                        ("out", out, torch.int32)):
+    f32, i32, check = torch.float32, torch.int32, attn._check_tensor
+    check("u", u, n, dev, f32)
+    for name, t, dt in (("temperature", temperature, f32), ("top_k", top_k, i32), ("top_p", top_p, f32), ("min_p", min_p, f32),
+                        ("row_index", row_index, i32), ("out", out, i32)):
         if t is not None:
-            attn._check_tensor(name, t, n, dev, dt)
-    rows, vocab = logits.shape
-    st, ctx = attn._launch(dev, stream)
-    with ctx:
-        if out is None:
-            out = torch.empty(n, dtype=torch.int32, device=dev)
-        p = attn._ptr
-        a = _SampleArgs(p(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab, code, n, p(row_index), p(temperature),
-                        p(top_k), p(top_p), p(min_p), p(u), p(out))
-        attn._check("tkm_hip_sample", lib().tkm_hip_sample(ctypes.byref(a), st), lib())
+            check(name, t, n, dev, dt)
+    if out is None:
+        out = torch.empty(n, dtype=i32, device=dev)
+    p, vocab = attn._ptr, shape[1]
+    a = _SampleArgs(logits.data_ptr(), stride[0] if shape[0] > 1 else vocab, shape[0], vocab, code, n, p(row_index), p(temperature),
+                    p(top_k), p(top_p), p(min_p), u.data_ptr(), out.data_ptr())
+    rc = lib().tkm_hip_sample(ctypes.byref(a), st)
+    if rc:
+        attn._check("tkm_hip_sample", rc, lib())
     return out
 
 
