@@ -66,6 +66,25 @@ def test_many_words_in_one_bin(gpu):
 
 
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("kw", [{}, dict(top_k=[50] * 8), dict(top_p=[0.9] * 8), dict(min_p=[0.01] * 8), dict(top_k=[9000] * 8, top_p=[0.99] * 8, min_p=[0.001] * 8)])
+def test_first_words_unlike_the_rest(gpu, dtype, kw):
+    """Rows whose first 8192 words say nothing of the largest: none at all, far lower, many above them, +inf or NaN
+    behind; and far higher."""
+    rng = np.random.default_rng(11)
+    x = torch.from_numpy(rng.standard_normal((8, 20001)))
+    x[0, :8192] = float("-inf")
+    x[1, :8192] -= 30
+    x[2, :8192] -= 3.5
+    x[3, 12000:] += 4
+    x[4, 19000] = float("inf")
+    x[5, 8192:] = float("nan")
+    x[6, :8192] += 50
+    x[7, 20000] = 9.0
+    run(gpu, x, rng.random(8).tolist(), dtype, **kw)
+    run(gpu, x, rng.random(8).tolist(), dtype, temperature=[0.05, 2.0, 0.3, 0.3, 1.0, 0.1, 30.0, 0.7], **kw)
+
+
+@pytest.mark.parametrize("dtype", DT)
 def test_odd_logits(gpu, dtype):
     inf, nan, low = float("inf"), float("nan"), torch.finfo(DT[dtype]).min
     V = 700

@@ -132,83 +132,44 @@ __device__ __forceinline__ uint32_t key_of(float w) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSel = 1024;   // threads of a selecting workgroup
+constexpr int kSel = 1024, kSelWaves = kSel / 64;   // threads and waves of a selecting workgroup
+constexpr int kEach = 8, kChunk = kSel * kEach;      // weights a thread has at a time, and the workgroup
+constexpr int kSelBits[3] = {12, 10, 10};            // of a weight's key, from the top
 
 struct SelectLds {
-    int count[3][4];
-    int wave[2][kSel / 64][2];
+    uint32_t bins[1 << kSelBits[0]];
+    uint32_t tot[2][kSelWaves];
+    uint32_t flags[2][kEach * kSelWaves];
+    uint32_t bin, before, many;
 };
-
-// The largest key K such that at least r of the n weights have a key >= K (r >= 1), and the number above K:
-// 16 rounds of two bits, each counting three candidates at once by ballots.  E > 0: the keys stay in E
-// registers a thread; E = 0: they are read again each round.
-template <int E>
-__device__ void find_key(const float* w, int n, int r, SelectLds& lds, uint32_t& key, int& above) {
-    const int tid = threadIdx.x, lane = tid & 63;
-    uint32_t k[E > 0 ? E : 1];
-    if constexpr (E > 0) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) k[e] = e * kSel + tid < n ? key_of(w[e * kSel + tid]) : 0u;
-    }
-    if (tid < 4) lds.count[0][tid] = 0;
-    __syncthreads();
-    key = 0u;
-    above = 0;
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t step = 1u << (30 - 2 * i);
-        const uint32_t k1 = key + step, k2 = k1 + step, k3 = k2 + step;
-        int c1 = 0, c2 = 0, c3 = 0;   // of the wave
-        auto one = [&](uint32_t x) {  // candidates are above 0, the key of what is not there
-            c1 += __popcll(__ballot(x >= k1));
-            c2 += __popcll(__ballot(x >= k2));
-            c3 += __popcll(__ballot(x >= k3));
-        };
-        if constexpr (E > 0) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) one(k[e]);
-        } else {
-            for (int j = 0; j < n; j += kSel) one(j + tid < n ? key_of(w[j + tid]) : 0u);
-        }
-        if (lane == 0) {
-            atomicAdd(&lds.count[i % 3][1], c1);
-            atomicAdd(&lds.count[i % 3][2], c2);
-            atomicAdd(&lds.count[i % 3][3], c3);
-        }
-        if (tid < 4) lds.count[(i + 1) % 3][tid] = 0;   // last read two rounds ago, before the last barrier
-        __syncthreads();
-        c1 = lds.count[i % 3][1];
-        c2 = lds.count[i % 3][2];
-        c3 = lds.count[i % 3][3];
-        if (c3 >= r) {
-            key = k3;
-        } else if (c2 >= r) {
-            key = k2;
-            above = c3;
-        } else if (c1 >= r) {
-            key = k1;
-            above = c2;
-        } else {
-            above = c1;
-        }
-    }
-    __syncthreads();
-}
 
 // Chooses what one kv head of one sequence keeps: writes its old positions in ascending order to `kept`, and
 // their weights to their new places.  A sequence with a length or a page that its tables cannot have gets -1s.
+//
+// The border among the weights is found by three histograms of their keys' bits (12, 10, 10; each narrows to the
+// bin that holds the border, and the walk ends with a bin of which all are kept), of weights that stay in registers
+// where 8192 hold them all.  Then ballots number what stays: 8192 positions a barrier.  Bound by the chain of
+// barriers: as 16 rounds of counting three candidates, and 1024 positions a barrier, it took 19 us for 1180
+// tokens and 30 for 8192.
 __global__ __launch_bounds__(kSel) void select_kernel(EvictArgs a) {
     __shared__ SelectLds lds;
     const tkm_attn_kv& s = a.src;
     const tkm_attn_kv& d = a.dst;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const long long row = blockIdx.x;
     const int b = (int)(row / s.Hkv);
     const long long cap = (long long)s.max_pages * s.page, cap_d = (long long)d.max_pages * d.page;
     const int n = s.len[b];
     int32_t* kept = a.kept + row * a.budget;
+    const float* w = s.weight + row * cap;
+    float* wd = d.weight ? d.weight + row * cap_d : nullptr;
     int bad = n < 0 || n > cap;
+    float held[kEach];
+    const bool holds = n <= kChunk;
     if (!bad) {
         const int most = min(n, a.budget);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) held[e] = e * kSel + tid < n ? w[e * kSel + tid] : 0.f;
         for (int i = tid; i < (n + s.page - 1) / s.page; i += kSel) bad |= !in_pool(s, s.table[(long long)b * s.max_pages + i]);
         for (int i = tid; i < (most + d.page - 1) / d.page; i += kSel) bad |= !in_pool(d, d.table[(long long)b * d.max_pages + i]);
     }
@@ -216,8 +177,6 @@ __global__ __launch_bounds__(kSel) void select_kernel(EvictArgs a) {
         for (int i = tid; i < a.budget; i += kSel) kept[i] = -1;
         return;
     }
-    const float* w = s.weight + row * cap;
-    float* wd = d.weight ? d.weight + row * cap_d : nullptr;
     if (n <= a.budget) {
         for (int i = tid; i < a.budget; i += kSel) {
             kept[i] = i < n ? i : -1;
@@ -226,40 +185,111 @@ __global__ __launch_bounds__(kSel) void select_kernel(EvictArgs a) {
         return;
     }
     const int lo = a.sink, hi = n - a.recent, r = a.budget - a.sink - a.recent;
-    uint32_t key = 0xffffffffu;
-    int above = 0;
+    auto load = [&](int c, float (&x)[kEach]) {      // the weights of positions c + e * kSel + tid
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int i = c + e * kSel + tid;
+            x[e] = holds ? held[e] : i < n ? w[i] : 0.f;
+        }
+    };
+    // Of the positions in [lo, hi) those with a key >= sure stay, and the first `ties` of those with the key `tie`.
+    uint32_t sure = 0xffffffffu, tie = 0xffffffffu;
+    int ties = 0, flip = 0;
     if (r > 0) {
-        if (hi - lo <= 8 * kSel) find_key<8>(w + lo, hi - lo, r, lds, key, above);
-        else if (hi - lo <= 32 * kSel) find_key<32>(w + lo, hi - lo, r, lds, key, above);
-        else find_key<0>(w + lo, hi - lo, r, lds, key, above);
+        uint32_t prefix = 0, before = 0;
+        int low = 32;
+        for (int level = 0; level < 3; ++level) {
+            const int bits = kSelBits[level], bins = 1 << bits;
+            low -= bits;
+            if (tid * 4 < bins) *(uint4*)&lds.bins[tid * 4] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            for (int c = 0; c < n; c += kChunk) {
+                float x[kEach];
+                load(c, x);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int i = c + e * kSel + tid;
+                    const uint32_t k = key_of(x[e]);
+                    if (i >= lo && i < hi && (uint32_t)((uint64_t)k >> (low + bits)) == prefix)
+                        atomicAdd(&lds.bins[k >> low & (uint32_t)(bins - 1)], 1u);
+                }
+            }
+            __syncthreads();
+            // the bin, from the largest on, at which the running count reaches r
+            uint4 v = make_uint4(0, 0, 0, 0);        // bins first .. first + 3
+            const int first = bins - 4 - tid * 4;
+            if (first >= 0) v = *(const uint4*)&lds.bins[first];
+            const uint32_t sum = v.x + v.y + v.z + v.w, run = wave_scan(sum);
+            if (lane == 63) lds.tot[flip][wave] = run;
+            __syncthreads();
+            const uint32_t all = wave_scan(lane < kSelWaves ? lds.tot[flip][lane] : 0u);
+            flip ^= 1;
+            uint32_t at = before + run - sum + (wave ? (uint32_t)lane_value((int)all, wave - 1) : 0u);
+            if (at < (uint32_t)r && at + sum >= (uint32_t)r) {
+                int bin = first + 3;
+                if (at + v.w < (uint32_t)r) {
+                    at += v.w;
+                    --bin;
+                    if (at + v.z < (uint32_t)r) {
+                        at += v.z;
+                        --bin;
+                        if (at + v.y < (uint32_t)r) {
+                            at += v.y;
+                            --bin;
+                        }
+                    }
+                }
+                lds.bin = (uint32_t)bin;
+                lds.before = at;
+                lds.many = lds.bins[bin];
+            }
+            __syncthreads();
+            before = lds.before;
+            prefix = prefix << bits | lds.bin;
+            if (before + lds.many == (uint32_t)r || level == 2) {
+                sure = prefix << low;
+                if (before + lds.many != (uint32_t)r) {
+                    tie = sure++;                    // keys end below 0xffffffff
+                    ties = r - (int)before;
+                }
+                break;
+            }
+            __syncthreads();
+        }
     }
-    const int ties = r - above;      // of the weights equal to the key, the first ones
-    int sure = 0, equal = 0;         // before this chunk
-    for (int c = 0; c < n; c += kSel) {
-        const int i = c + tid, buf = (c / kSel) & 1;
-        const float x = i < n ? w[i] : 0.f;
-        const uint32_t k = key_of(x);
-        const bool mid = i >= lo && i < hi;
-        const bool g = i < n && (!mid || (r > 0 && k > key)), e = mid && r > 0 && k == key;
-        const uint64_t mg = __ballot(g), me = __ballot(e), under = (1ull << lane) - 1;
-        if (lane == 0) {
-            lds.wave[buf][wave][0] = __popcll(mg);
-            lds.wave[buf][wave][1] = __popcll(me);
+    uint32_t stay = 0, equal = 0;    // before this chunk
+    const uint64_t under = (1ull << lane) - 1;
+    for (int c = 0, buf = 0; c < n; c += kChunk, buf ^= 1) {
+        float x[kEach];
+        uint64_t g[kEach], t[kEach];
+        load(c, x);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int i = c + e * kSel + tid;
+            const uint32_t k = key_of(x[e]);
+            const bool mid = i >= lo && i < hi;
+            g[e] = __ballot(i < n && (!mid || k >= sure));
+            t[e] = __ballot(mid && ties > 0 && k == tie);
+            if (lane == 0) lds.flags[buf][e * kSelWaves + wave] = (uint32_t)(__popcll(g[e]) | __popcll(t[e]) << 16);
         }
-        __syncthreads();             // also: the chunk's weights are read before any is overwritten in place
-        int ng = sure + __popcll(mg & under), ne = equal + __popcll(me & under);
-        for (int v = 0; v < kSel / 64; ++v) {
-            const int cg = lds.wave[buf][v][0], ce = lds.wave[buf][v][1];
-            ng += v < wave ? cg : 0;
-            ne += v < wave ? ce : 0;
-            sure += cg;
-            equal += ce;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();             // also: all of the chunk's weights are read before one is overwritten in place
+        const uint32_t v0 = lds.flags[buf][lane * 2], v1 = lds.flags[buf][lane * 2 + 1], run = wave_scan(v0 + v1);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int at = e * kSelWaves + wave;
+            const uint32_t before = (uint32_t)(lane_value((int)(run - v0 - v1), at / 2) + (at % 2 ? lane_value((int)v0, at / 2) : 0));
+            const uint32_t ng = stay + (before & 0xffffu) + (uint32_t)__popcll(g[e] & under);
+            const uint32_t nt = equal + (before >> 16) + (uint32_t)__popcll(t[e] & under);
+            if ((g[e] >> lane & 1) || ((t[e] >> lane & 1) && nt < (uint32_t)ties)) {
+                const uint32_t to = ng + min(nt, (uint32_t)ties);
+                kept[to] = c + e * kSel + tid;
+                if (wd) wd[to] = x[e];
+            }
         }
-        if (g || (e && ne < ties)) {
-            const int at = ng + min(ne, ties);
-            kept[at] = i;
-            if (wd) wd[at] = x;
-        }
+        const uint32_t last = (uint32_t)lane_value((int)run, 63);
+        stay += last & 0xffffu;
+        equal += last >> 16;
     }
 }
 
