@@ -25,6 +25,8 @@
 // timing.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "attn_common.h"
 #include "attn_kv.h"
 #include "attn_launch.h"
@@ -34,7 +36,8 @@ namespace {
 
 constexpr float kSlack = 8.0f;   // m moves when a score exceeds it by more than this (log2)
 constexpr float kLift = 6.0f;    // P = 2^(s - m + kLift)
-constexpr int kWaves = 4;        // waves of a workgroup
+constexpr int kWaves = 4;        // waves of a workgroup of a split launch
+constexpr int kRowWaves = 8;     // and where a workgroup has a row
 constexpr int kGroups = 512;     // workgroups of a split launch: two on each of 256 compute units
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -66,6 +69,12 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// An element of an array that no kernel here writes, at a wave-uniform index: a scalar load also behind stores
+// (which the compiler must otherwise take for possible writes to it, and wait for all vector loads with the page's).
+__device__ __forceinline__ int fixed(const int32_t* p, long long i) {
+    return *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p + i);
+}
 
 // Tiles of a sequence; a length outside the table's capacity has none (its rows become NaN).
 __device__ __forceinline__ int tiles_of(int len, int cap) { return (unsigned)len > (unsigned)cap ? 0 : (len + 31) >> 5; }
@@ -112,18 +121,48 @@ __device__ __forceinline__ void add_piece(f32x2 ml, f32x4 x, float mm, f32x4& o,
     o += f * x;
 }
 
+// LSE from a row's maximum and sum, in log2 units and natural.
+__device__ __forceinline__ float lse2_of(float m, float l) { return l > 0.f ? m - kLift + __log2f(l) : l == 0.f ? -INFINITY : NAN; }
+__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m - kLift) * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN; }
+
+// Four positions' weights of `row` (sequence and kv head), j .. j + 3: loaded ahead of what is added to them.
+struct Weights {
+    f32x4 w;
+    float* at;
+    int left;      // of the four, those of the sequence
+    __device__ __forceinline__ void load(const P& a, long long row, int j, int len) {
+        at = a.weight + row * a.cap + j;
+        left = len - j;
+        if (left > 0) __builtin_memcpy(&w, at, 16);      // a row ends at a multiple of 32
+    }
+    // adds exp2(score - LSE), l2 the LSE; a head whose LSE is NaN, or -inf (all its scores are), adds nothing
+    __device__ __forceinline__ void add(f32x4 score, float l2) {
+        if (!(l2 > -INFINITY)) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(score[i] - l2);
+    }
+    __device__ __forceinline__ void store() const {
+        if (left >= 4) __builtin_memcpy(at, &w, 16);
+        else
+            for (int i = 0; i < left; ++i) at[i] = w[i];
+    }
+};
+
 // Where a wave stands: tile `tile` of the `nt` of row `rh` (kv head and query head group) of sequence b.
 struct At {
     int b, rh, tile, nt, len;
 };
 
-// NH waves hold 16 query heads each of the group, and TW = 4 / NH such sets walk tiles of their own.
-template <int D, int DT, int NH, bool SC>
-__global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
-    constexpr int KS = D / 32, DB = D / 16, TW = kWaves / NH;
+// NH waves hold 16 query heads each of the group, and TW = NW / NH such sets walk tiles of their own.  ROW: a
+// workgroup has a row, else its share of all tiles.  SC: the scores are kept, and with ROW and one group of query
+// heads the row's weights are added here too.
+template <int D, int DT, int NH, bool SC, bool ROW>
+__global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_kernel(P a) {
+    constexpr int NW = ROW ? kRowWaves : kWaves, KS = D / 32, DB = D / 16, TW = NW / NH;
     constexpr uint32_t TILE = D * 64;   // bytes of a tile of K or V
-    __shared__ float red_o[kWaves][16][D + 4];   // padded: 16 heads' rows start in other banks
-    __shared__ f32x2 red_ml[kWaves][16];
+    __shared__ float red_o[NW][16][D + 4];   // padded: 16 heads' rows start in other banks
+    __shared__ f32x2 red_ml[NW][16];
+    __shared__ float red_lse[16 * NH];
 
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
     const int hs = wave / TW, tw = wave % TW;
@@ -132,18 +171,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
 
     // ---- this wave's tiles
     At it;
-    int count, stride;     // tiles to do, and the step between them
+    int count;             // tiles to do
     bool shared;           // the workgroup's tiles are all of one row
     bool whole;            // ... and all of the row's
     int slot = 0;
-    if (a.groups == 0) {
+    if constexpr (ROW) {
         it.b = blockIdx.x / RH;
         it.rh = blockIdx.x % RH;
-        it.len = a.len[it.b];
+        it.len = fixed(a.len, it.b);
         it.nt = tiles_of(it.len, a.cap);
         it.tile = tw;
         count = (it.nt - tw + TW - 1) / TW;
-        stride = TW;
         shared = whole = true;
     } else {
         // the first 64 sequences' tiles, their running sum, and the call's
@@ -162,7 +200,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
                     const int w = __ffsll((unsigned long long)m) - 1;
                     it.b = uni(c + w);
                     it.nt = lane_value(n, w);
-                    it.len = a.len[it.b];
+                    it.len = fixed(a.len, it.b);
                     const int r = at - (before + lane_value(s, w) - it.nt) * RH;
                     it.rh = r / it.nt;
                     it.tile = r % it.nt;
@@ -180,32 +218,31 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
             slot = blockIdx.x * TW * 2 + (it.tile == 0 ? 1 : 0);
             it.tile += tw;
             count = max(0, (last - first - tw + TW - 1) / TW);
-            stride = TW;
-        } else {
+            } else {
             const int mine = first + tw * t;
             if (mine >= last) return;
             if (tw) find(mine);
             count = min(t, last - mine);
-            stride = 1;
         }
     }
 
     // ---- the walk
     const uint32_t koff = (uint32_t)(8 * (n16 >> 2) + (n16 & 3)) * 64 + quad * 16;   // + t * 256 + ks * 2048
     const uint32_t voff = (uint32_t)n16 * 64 + quad * 16;                            // + db * 1024
-    const int sub_mask = (1 << (a.page_shift - 5)) - 1;
-    u32x4 kf[2][2][KS], vf[2][DB], qf[KS], qn[KS];
+    const int tile_bits = a.page_shift - 5, sub_mask = (1 << tile_bits) - 1;
+    u32x4 kf[2][2][KS], vf[2][DB], qf[KS];
     f32x4 acc[DB];
     float m, l;
-    bool bad = false;
+    bool bad;
 
-    auto load = [&](int buf, const At& x) {
-        const int page = a.table[(long long)x.b * a.max_pages + (x.tile >> (a.page_shift - 5))];
+    // (of a tile behind the row's last, the table's last or whatever it says: it is not used)
+    auto page_of = [&](const At& x, int tile) { return fixed(a.table, (long long)x.b * a.max_pages + min(tile >> tile_bits, a.max_pages - 1)); };
+    auto load = [&](int buf, const At& x, int tile, int page) {
         const bool ok = (unsigned)page < (unsigned)a.num_pages;
         bad |= !ok;      // page 0 is read in its place, and the row becomes NaN
-        const long long tile = (((long long)(ok ? page : 0) * a.Hkv + x.rh / a.HG) << (a.page_shift - 5)) + (x.tile & sub_mask);
-        const char* kb = (const char*)a.k + tile * TILE;
-        const char* vb = (const char*)a.v + tile * TILE;
+        const long long at = (((long long)(ok ? page : 0) * a.Hkv + x.rh / a.HG) << tile_bits) + (tile & sub_mask);
+        const char* kb = (const char*)a.k + at * TILE;
+        const char* vb = (const char*)a.v + at * TILE;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -215,12 +252,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
     };
     // this lane's query head within the kv head, of row x
     auto head_of = [&](const At& x) { return (x.rh % a.HG * NH + hs) * 16 + n16; };
-    auto load_q = [&](const At& x) {
-        const int h = head_of(x);
-        const uint16_t* qp = a.q + (long long)x.b * a.q_stride + (x.rh / a.HG * a.G + h) * D + quad * 8;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qn[ks] = h < a.G ? ld_global16(qp + ks * 32) : u32x4{0u, 0u, 0u, 0u};
-    };
     auto reset = [&]() {
         m = -INFINITY;
         l = 0.f;
@@ -228,8 +259,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
         for (int db = 0; db < DB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
         bad = false;
     };
-    auto tile = [&](int buf, const At& x) {
-        const int left = x.len - x.tile * 32;         // visible tokens of the tile
+    auto tile = [&](int buf, const At& x, int tile, auto last) {
+        const int left = decltype(last)::value ? x.len - tile * 32 : 32;         // visible tokens of the tile
         f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -242,7 +273,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
             s[i] = s0[i] * a.sl2;
             s[4 + i] = s1[i] * a.sl2;
         }
-        if (left < 32) {
+        if (decltype(last)::value && left < 32) {
             // what lies behind the last token may be anything: its scores are replaced, and as 0 * NaN is not 0
             // its values become 0 too
 #pragma unroll
@@ -256,7 +287,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
             }
         }
         if (SC && head_of(x) < a.G) {
-            float* sp = a.scores + (((long long)x.b * a.Hkv + x.rh / a.HG) * a.G + head_of(x)) * a.cap + x.tile * 32 + quad * 8;
+            float* sp = a.scores + (((long long)x.b * a.Hkv + x.rh / a.HG) * a.G + head_of(x)) * a.cap + tile * 32 + quad * 8;
             *(f32x4*)sp = f32x4{s[0], s[1], s[2], s[3]};
             *(f32x4*)(sp + 4) = f32x4{s[4], s[5], s[6], s[7]};
         }
@@ -289,9 +320,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
     // output row of a head of the kv head of x
     auto out_row = [&](const At& x, int h) { return ((long long)x.b * a.Hkv + x.rh / a.HG) * a.G + h; };
     auto put_lse = [&](long long row, float mm, float ll) {
-        const float l2 = ll > 0.f ? mm - kLift + __log2f(ll) : ll == 0.f ? -INFINITY : NAN;
-        if (a.lse) a.lse[row] = ll > 0.f ? (mm - kLift) * kLn2 + logf(ll) : l2;
+        const float l2 = lse2_of(mm, ll);
+        if (a.lse) a.lse[row] = lse_of(mm, ll);
         if (SC) a.lse2[row] = l2;
+        return l2;
     };
     auto finish = [&](const At& x, bool all, int at) {   // private mode: this wave's sums of a row's piece
         float ll = quad_sum(l);
@@ -314,61 +346,60 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
             if (quad == 0) a.part_ml[(long long)at * a.cols + c] = f32x2{m, ll};
         }
     };
-    auto advance = [&](At& x) {
-        x.tile += stride;
-        if (!shared && x.tile == x.nt) {
-            x.tile = 0;
-            if (++x.rh == RH) {
-                x.rh = 0;
-                do {
-                    ++x.b;
-                    x.len = a.len[x.b];
-                    x.nt = tiles_of(x.len, a.cap);
-                } while (x.nt == 0);
-            }
+    // The sums of n tiles of row x from x.tile on, `stride` apart: the next tile's loads, and the page of the one
+    // after it, are under way while a tile is computed.  Straight code for all but the last two, so that the
+    // compiler can count what is in flight (a load under a condition, and it waits for all of them).
+    auto walk = [&](const At& x, int n, int stride) {
+        reset();
+        const int h = head_of(x);
+        const uint16_t* qp = a.q + (long long)x.b * a.q_stride + (x.rh / a.HG * a.G + min(h, a.G - 1)) * D + quad * 8;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const u32x4 w = ld_global16(qp + ks * 32);
+            qf[ks] = h < a.G ? w : u32x4{0u, 0u, 0u, 0u};
+        }
+        int at = x.tile, page = page_of(x, at + stride);
+        load(0, x, at, page_of(x, at));
+        auto go = [&](int buf) {          // computes tile `at`, with two more to come
+            const int next = at + stride, p = page;
+            page = page_of(x, next + stride);
+            load(buf ^ 1, x, next, p);
+            tile(buf, x, at, std::false_type());
+            at = next;
+        };
+        for (; n > 2; n -= 2) {
+            go(0);
+            go(1);
+        }
+        if (n == 2) {
+            go(0);
+            tile(1, x, at, std::true_type());
+        } else {
+            tile(0, x, at, std::true_type());
         }
     };
 
-    reset();
-    if (count > 0) {
-        At nx = it;
-        int from = it.tile;      // first tile of the row's piece (private mode)
-        load_q(it);
-        load(0, it);
-        bool bad_next = bad;
-        bad = false;
-        auto step = [&](int buf, int i) {
-            const bool more = i + 1 < count;
-            if (i == 0 || (!shared && it.tile == 0)) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) qf[ks] = qn[ks];
+    if (shared) {
+        if (count > 0) walk(it, count, TW);
+        else reset();
+    } else {
+        while (true) {
+            const int n = min(count, it.nt - it.tile);
+            walk(it, n, 1);
+            finish(it, n == it.nt, (blockIdx.x * TW + tw) * 2 + (it.tile == 0 ? 1 : 0));
+            count -= n;
+            if (count == 0) return;
+            it.tile = 0;                 // of the next row with tiles
+            if (++it.rh == RH) {
+                it.rh = 0;
+                do {
+                    ++it.b;
+                    it.len = fixed(a.len, it.b);
+                    it.nt = tiles_of(it.len, a.cap);
+                } while (it.nt == 0);
             }
-            const bool was = bad | bad_next;
-            bad = false;
-            if (more) {
-                advance(nx);
-                load(buf ^ 1, nx);
-                if (!shared && nx.tile == 0) load_q(nx);
-            }
-            bad_next = bad;
-            bad = was;
-            tile(buf, it);
-            if (!shared && (!more || nx.tile == 0)) {
-                const int n = it.tile + 1 - from;
-                const int w = blockIdx.x * TW + tw;
-                finish(it, n == it.nt, w * 2 + (from == 0 ? 1 : 0));
-                reset();
-                from = 0;
-            }
-            it = nx;
-        };
-        for (int i = 0; i < count; i += 2) {
-            step(0, i);
-            if (i + 1 < count) step(1, i + 1);
         }
-        if (shared) bad |= bad_next;
     }
-    if (!shared) return;
 
     // ---- shared mode: the waves' sums of one row
     {
@@ -378,11 +409,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) *(f32x4*)&red_o[wave][n16][db * 16 + quad * 4] = acc[db];
     }
+    it.len = fixed(a.len, it.b);
+    Weights ws = {};
+    const long long kvrow = (long long)it.b * a.Hkv + it.rh / a.HG;
+    if constexpr (SC && ROW)
+        if ((unsigned)it.len <= (unsigned)a.cap) ws.load(a, kvrow, threadIdx.x * 4, it.len);
     __syncthreads();
-    it.len = a.len[it.b];
     const bool lost = (unsigned)it.len > (unsigned)a.cap;     // no length of this table
     const int h0 = it.rh % a.HG * NH * 16, have = min(a.cols, a.G - h0);
-    for (int i = threadIdx.x; i < have * (D / 4); i += 64 * kWaves) {
+    for (int i = threadIdx.x; i < have * (D / 4); i += 64 * NW) {
         const int c = i / (D / 4), d = i % (D / 4) * 4, w0 = c / 16 * TW;
         float mm = -INFINITY;
 #pragma unroll
@@ -397,54 +432,82 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(P a) {
             o *= inv;
             const long long row = out_row(it, h0 + c);
             *(u32x2*)(a.o + row * D + d) = u32x2{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
-            if (d == 0) put_lse(row, mm, ll);
+            if (d == 0) red_lse[c] = put_lse(row, mm, ll);
         } else {
             *(f32x4*)(a.part + ((long long)slot * a.cols + c) * D + d) = o;
             if (d == 0) a.part_ml[(long long)slot * a.cols + c] = f32x2{mm, ll};
         }
     }
+    if constexpr (SC && ROW) {
+        if (lost) return;
+        __syncthreads();      // the scores of all waves too
+        for (int j = threadIdx.x * 4; j < it.len; j += 64 * NW * 4) {
+            Weights next = {};
+            next.load(a, kvrow, j + 64 * NW * 4, it.len);
+            const float* sp = a.scores + kvrow * a.G * a.cap + j;
+#pragma unroll 4
+            for (int c = 0; c < a.G; ++c) ws.add(*(const f32x4*)(sp + (long long)c * a.cap), red_lse[c]);
+            ws.store();
+            ws = next;
+        }
+    }
 }
 
-// The rows that the split launch left in pieces, and those without a tile. One workgroup a query head: D/4
-// threads have 4 dims each of a piece, and the workgroup's groups of them take pieces in turn, 8 in flight.
-template <int D, int DT, int NH>
-__global__ __launch_bounds__(256) void join_kernel(P a) {
-    constexpr int TW = kWaves / NH, DV = D / 4, PAR = 256 / DV, FLY = 8;
-    __shared__ f32x4 red_o[PAR][DV];
-    __shared__ f32x2 red_ml[PAR];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int h = blockIdx.x % (a.Hkv * a.G), b = blockIdx.x / (a.Hkv * a.G);
-    const int kvh = h / a.G, hg = h % a.G / (16 * NH), c = h % a.G % (16 * NH);
-    const int RH = a.Hkv * a.HG;
-    const long long row = blockIdx.x;
-    const int len = a.len[b], nt = tiles_of(len, a.cap);
-    if (nt == 0) {
-        const bool lost = len != 0;
-        for (int d = tid; d < D; d += 256) a.o[row * D + d] = (uint16_t)(lost ? (DT == DT_F16 ? 0x7e00 : 0x7fc0) : 0);
-        if (tid == 0 && a.lse) a.lse[row] = lost ? NAN : -INFINITY;
-        if (tid == 0 && a.lse2) a.lse2[row] = lost ? NAN : -INFINITY;
-        return;
+// The pieces in which a split launch of TW workers a workgroup left a row: `head` of single workers, those of the
+// workgroups [ga, gb) that lie in the row, and `tail` of single workers.  none: one worker or workgroup had it all.
+struct Pieces {
+    int n, head, tail, w0, ga, gb, t, r0, tw, cols;
+    __device__ __forceinline__ long long slot(int i, int c) const {
+        const int mid = gb - ga;
+        const int w = i < head ? w0 + i : i < head + mid || tail == 0 ? (ga + i - head) * tw : gb * tw + i - head - mid;
+        return ((long long)w * 2 + (w * t <= r0 ? 1 : 0)) * cols + c;
     }
+};
+template <int TW>
+__device__ __forceinline__ bool pieces_of(const P& a, int b, int rh, int nt, int lane, Pieces& p) {
     int all, before;
     count_tiles(a, b, lane, all, before);
+    const int RH = a.Hkv * a.HG;
     all *= RH;
-    const int t = tiles_each(all, a.groups * TW), T = t * TW;
-    const int r0 = before * RH + (kvh * a.HG + hg) * nt, r1 = r0 + nt;
-    const int w0 = r0 / t, w1 = (r1 - 1) / t;
-    const int ga = (r0 + T - 1) / T, gb = r1 == all ? (r1 + T - 1) / T : r1 / T;   // workgroups [ga, gb) lie in the row
-    if (w0 == w1 && ga >= gb) return;                  // one worker had all of it
-    if (gb - ga == 1 && ga * T == r0 && r1 <= gb * T) return;   // one workgroup had
-    const int head = ga < gb ? ga * TW - w0 : w1 - w0 + 1;      // pieces of single workers before those
-    const int tail = ga < gb ? max(0, w1 + 1 - gb * TW) : 0;
-    const int n = head + max(0, gb - ga) + tail;
-    auto slot = [&](int i) {
-        const int w = i < head ? w0 + i : i < head + (gb - ga) || tail == 0 ? (ga + i - head) * TW : gb * TW + i - head - (gb - ga);
-        return ((long long)w * 2 + (w * t <= r0 ? 1 : 0)) * a.cols + c;
-    };
-    const int d = tid % DV, g = tid / DV;
+    p.tw = TW;
+    p.cols = a.cols;
+    p.t = tiles_each(all, a.groups * TW);
+    const int T = p.t * TW, r1 = before * RH + rh * nt + nt;
+    p.r0 = r1 - nt;
+    p.w0 = p.r0 / p.t;
+    const int w1 = (r1 - 1) / p.t;
+    p.ga = (p.r0 + T - 1) / T;
+    p.gb = r1 == all ? (r1 + T - 1) / T : r1 / T;
+    if (p.w0 == w1 && p.ga >= p.gb) return false;
+    if (p.gb - p.ga == 1 && p.ga * T == p.r0 && r1 <= p.gb * T) return false;
+    p.head = p.ga < p.gb ? p.ga * TW - p.w0 : w1 - p.w0 + 1;
+    p.tail = p.ga < p.gb ? max(0, w1 + 1 - p.gb * TW) : 0;
+    p.n = p.head + max(0, p.gb - p.ga) + p.tail;
+    return true;
+}
+
+// A row without a tile: zeros, or NaN where the length is none of this table.
+template <int D, int DT>
+__device__ __forceinline__ void put_empty(const P& a, long long row, bool lost, int t, int threads) {
+    for (int d = t; d < D; d += threads) a.o[row * D + d] = (uint16_t)(lost ? (DT == DT_F16 ? 0x7e00 : 0x7fc0) : 0);
+    if (t == 0 && a.lse) a.lse[row] = lost ? NAN : -INFINITY;
+}
+
+// Joins the pieces of column c of a row by the TEAM threads t: D/4 of them have 4 dims each of a piece, and the
+// groups of so many take pieces in turn, 8 in flight.  A team is a wave, or a workgroup (then `red` is LDS for it).
+template <int D, int DT, int TEAM>
+__device__ __forceinline__ void join_row(const P& a, const Pieces& p, int c, long long row, int t, f32x4* red_o, f32x2* red_ml) {
+    constexpr int DV = D / 4, PAR = TEAM / DV, FLY = 8;
+    const int d = t % DV, g = t / DV;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float mm = -INFINITY, ll = 0.f;
-    for (int i0 = g; i0 < n; i0 += PAR * FLY) {
+    auto lift = [&](float top) {       // the sums so far, relative to top
+        const float f = mm == -INFINITY ? 0.f : fast_exp2(mm - top);
+        o *= f;
+        ll = mm == -INFINITY ? ll : ll * f;
+        mm = top;
+    };
+    for (int i0 = g; i0 < p.n; i0 += PAR * FLY) {
         f32x2 ml[FLY];
         f32x4 x[FLY];
         float top = mm;
@@ -452,62 +515,136 @@ __global__ __launch_bounds__(256) void join_kernel(P a) {
         for (int j = 0; j < FLY; ++j) {
             const int i = i0 + j * PAR;
             ml[j] = f32x2{-INFINITY, 0.f};
-            if (i < n) {
-                const long long s = slot(i);
+            x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (i < p.n) {
+                const long long s = p.slot(i, c);
                 ml[j] = a.part_ml[s];
                 x[j] = *(const f32x4*)(a.part + s * D + d * 4);
-            } else {
-                x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
 #pragma unroll
         for (int j = 0; j < FLY; ++j) top = fmaxf(top, ml[j][0]);
-        const float f = mm == -INFINITY ? 0.f : fast_exp2(mm - top);
-        o *= f;
-        ll = mm == -INFINITY ? ll : ll * f;
-        mm = top;
+        lift(top);
 #pragma unroll
         for (int j = 0; j < FLY; ++j) add_piece(ml[j], x[j], mm, o, ll);
     }
-    red_o[g][d] = o;
-    if (d == 0) red_ml[g] = f32x2{mm, ll};
-    __syncthreads();
-    if (tid >= DV) return;
-    mm = -INFINITY;
+    if constexpr (TEAM == 64) {
 #pragma unroll
-    for (int i = 0; i < PAR; ++i) mm = fmaxf(mm, red_ml[i][0]);
-    o = f32x4{0.f, 0.f, 0.f, 0.f};
-    ll = 0.f;
+        for (int k = DV; k < 64; k <<= 1) {
+            const f32x2 ml = {__shfl_xor(mm, k, 64), __shfl_xor(ll, k, 64)};
+            f32x4 x;
 #pragma unroll
-    for (int i = 0; i < PAR; ++i) add_piece(red_ml[i], red_o[i][tid], mm, o, ll);
-    o *= ll == 0.f ? 0.f : 1.0f / ll;
-    *(u32x2*)(a.o + row * D + tid * 4) = u32x2{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
-    if (tid == 0) {
-        const float l2 = ll > 0.f ? mm - kLift + __log2f(ll) : ll == 0.f ? -INFINITY : NAN;
-        if (a.lse) a.lse[row] = ll > 0.f ? (mm - kLift) * kLn2 + logf(ll) : l2;
-        if (a.lse2) a.lse2[row] = l2;
+            for (int i = 0; i < 4; ++i) x[i] = __shfl_xor(o[i], k, 64);
+            lift(fmaxf(mm, ml[0]));
+            add_piece(ml, x, mm, o, ll);
+        }
+    } else {
+        red_o[t] = o;
+        if (d == 0) red_ml[g] = f32x2{mm, ll};
+        __syncthreads();
+        mm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PAR; ++i) mm = fmaxf(mm, red_ml[i][0]);
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+        ll = 0.f;
+#pragma unroll
+        for (int i = 0; i < PAR; ++i) add_piece(red_ml[i], red_o[i * DV + d], mm, o, ll);
     }
+    if (g != 0) return;
+    o *= ll == 0.f ? 0.f : 1.0f / ll;
+    *(u32x2*)(a.o + row * D + d * 4) = u32x2{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
+    if (d == 0 && a.lse) a.lse[row] = lse_of(mm, ll);
 }
 
-// weight[b][kvh][j] += sum over the kv head's query heads of exp2(score - lse), 4 tokens a thread.
-__global__ __launch_bounds__(256) void weights_kernel(P a) {
+// The rows that a split launch left in pieces, and those without a tile. A team of TEAM threads a query head.
+template <int D, int DT, int NH, int TEAM>
+__global__ __launch_bounds__(256) void join_kernel(P a) {
+    __shared__ f32x4 red_o[TEAM == 64 ? 1 : 256];
+    __shared__ f32x2 red_ml[TEAM == 64 ? 1 : 1024 / D];
+    const int lane = threadIdx.x & 63, t = threadIdx.x % TEAM;
+    const long long row = (long long)blockIdx.x * (256 / TEAM) + uni(threadIdx.x / TEAM);
+    if (row >= (long long)a.B * a.Hkv * a.G) return;
+    const int h = (int)(row % (a.Hkv * a.G)), b = (int)(row / (a.Hkv * a.G)), kvh = h / a.G, hg = h % a.G / (16 * NH), c = h % a.G % (16 * NH);
+    const int len = a.len[b], nt = tiles_of(len, a.cap);
+    Pieces p;
+    if (nt == 0) put_empty<D, DT>(a, row, len != 0, t, TEAM);
+    else if (pieces_of<kWaves / NH>(a, b, kvh * a.HG + hg, nt, lane, p)) join_row<D, DT, TEAM>(a, p, c, row, t, red_o, red_ml);
+}
+
+// With weights: the same, and 1024 positions' weights of a kv head a workgroup.  Each workgroup takes the LSE of
+// the head's query heads from their pieces itself, and joins the O of every n-th of them, n the workgroups of the
+// row, so that one launch does both.
+template <int D, int DT, int NH, int TEAM>
+__global__ __launch_bounds__(256) void join_weights_kernel(P a) {
+    __shared__ f32x4 red_o[TEAM == 64 ? 1 : 256];
+    __shared__ f32x2 red_ml[TEAM == 64 ? 1 : 1024 / D];
+    __shared__ float l2[64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
     const unsigned chunks = (unsigned)(a.cap + 1023) / 1024;
-    const long long row = blockIdx.x / chunks;     // sequence and kv head
-    const int j = (int)(blockIdx.x % chunks * 1024 + threadIdx.x * 4), len = a.len[row / a.Hkv];
-    if ((unsigned)len > (unsigned)a.cap || j >= len) return;
-    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < a.G; ++g) {
-        const float l2 = a.lse2[row * a.G + g];
-        const f32x4 s = *(const f32x4*)(a.scores + (row * a.G + g) * a.cap + j);
-        if (l2 == -INFINITY) continue;    // every score is -inf: no key has a weight
-        if (l2 != l2) return;             // a page outside the pool: the weights stay
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(s[i] - l2);
+    const long long kvrow = blockIdx.x / chunks;     // sequence and kv head
+    const int chunk = (int)(blockIdx.x % chunks), b = (int)(kvrow / a.Hkv), kvh = (int)(kvrow % a.Hkv);
+    const int len = a.len[b], nt = tiles_of(len, a.cap);
+    if (nt == 0) {
+        for (int g = chunk; g < a.G; g += (int)chunks) put_empty<D, DT>(a, kvrow * a.G + g, len != 0, tid, 256);
+        return;
     }
-    float* wp = a.weight + row * a.cap + j;
+    const int mine = (len + 1023) / 1024, j = chunk * 1024 + tid * 4;
+    if (chunk >= mine) return;
+    // the weights and the first heads' scores are on their way while the LSE are joined
+    constexpr int AHEAD = 4;
+    Weights ws = {};
+    ws.load(a, kvrow, j, len);
+    const float* sp = a.scores + kvrow * a.G * a.cap + j;
+    f32x4 sc[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (j + i < len) wp[i] += w[i];
+    for (int c = 0; c < AHEAD; ++c)
+        if (c < a.G && j < len) sc[c] = *(const f32x4*)(sp + (long long)c * a.cap);
+    for (int hg = 0; hg < a.HG; ++hg) {              // up to 64 query heads at a time
+        const int g0 = hg * 16 * NH, n = min(a.cols, a.G - g0);
+        Pieces p;
+        const bool some = pieces_of<kWaves / NH>(a, b, kvh * a.HG + hg, nt, lane, p);
+        if (hg) __syncthreads();
+        if (some) {
+            for (int c = wave; c < n; c += 4) {
+                float m = -INFINITY, l = 0.f;
+                for (int i = lane; i < p.n; i += 64) {
+                    const f32x2 ml = a.part_ml[p.slot(i, c)];
+                    const float top = fmaxf(m, ml[0]);
+                    if (top == -INFINITY) {
+                        l += ml[1];
+                    } else {
+                        l = (m == -INFINITY ? l : l * fast_exp2(m - top)) + (ml[0] == -INFINITY ? ml[1] : ml[1] * fast_exp2(ml[0] - top));
+                        m = top;
+                    }
+                }
+                float top = m;
+#pragma unroll
+                for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+                if (m != -INFINITY) l *= fast_exp2(m - top);
+#pragma unroll
+                for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k, 64);
+                if (lane == 0) l2[c] = lse2_of(top, l);
+            }
+        } else if (tid < n) {
+            l2[tid] = a.lse2[kvrow * a.G + g0 + tid];
+        }
+        __syncthreads();
+        if (j < len) {
+            if (hg == 0)
+#pragma unroll
+                for (int c = 0; c < AHEAD; ++c)
+                    if (c < n) ws.add(sc[c], l2[c]);
+#pragma unroll 4
+            for (int c = hg ? 0 : AHEAD; c < n; ++c) ws.add(*(const f32x4*)(sp + (long long)(g0 + c) * a.cap), l2[c]);
+        }
+        if (!some) continue;
+        constexpr int TEAMS = 256 / TEAM;
+        for (int c = chunk * TEAMS + uni(tid / TEAM); c < n; c += mine * TEAMS) {
+            join_row<D, DT, TEAM>(a, p, c, kvrow * a.G + g0 + c, tid % TEAM, red_o, red_ml);
+            if (TEAM > 64) __syncthreads();
+        }
+    }
+    ws.store();
 }
 
 // Waves that share a kv head's query heads, 16 each, and the groups of so many heads.
@@ -516,32 +653,56 @@ int head_groups(int G) { return (G + 63) / 64; }
 int head_cols(int G) { return G < 64 ? G : 64; }
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Whether a call runs as one workgroup a row, without pieces.
-bool by_row(int cap) { return cap <= 512; }
+// Whether a call runs as one workgroup (of 8 waves) a row, in one launch without pieces: where the longest row that
+// the tables can hold is short, and longer where there are rows enough to keep HBM busy, or where the weights
+// would need the second launch anyway.  Measured, us of one workgroup a row / split and joined (B, tokens, Hkv, D;
+// ragged where B > 1):
+//   1, 200, 8, 64: 4.2 / 7.4        1, 500, 8, 128: 6.8 / 7.9         1, 1000, 8, 128: 10.7 / 8.8    1, 2000, 8, 64: 10.4 / 8.4
+//   16, 500, 8, 128: 7.6 / 12.0     16, 1000, 8, 128: 14.4 / 16.9     16, 2000, 8, 128: 25.0 / 22.3
+//   64, 1000, 8, 128: 33.1 / 37.3   64, 2000, 8, 128: 67.0 / 69.4     128, 1000, 8, 64: 31.1 / 36.9
+//   with weights  12, 1000, 4, 64: 9.5 / 16.3     4, 1000, 8, 128: 12.6 / 16.2    12, 2500, 4, 64: 16.4 / 17.7
+//                 16, 2000, 8, 128: 28.9 / 28.5   4, 8000, 4, 64: 39 / 14.9
+bool by_row(const tkm_attn_kv& kv, int Hq, int add_weights) {
+    const double kb = (double)kv.max_pages * kv.page * kv.D * 4 / 1024, rows = (double)kv.B * kv.Hkv;   // K and V of a row
+    return Hq / kv.Hkv <= 64 && kb <= (rows >= 512 ? 1280 : add_weights || rows >= 96 ? 704 : 320);
+}
 
 int groups_of(const tkm_attn_kv& kv, int Hq) {
     const double most = decode_tiles_most(kv, Hq) * head_waves(Hq / kv.Hkv) / kWaves + 1;
     return most < kGroups ? (int)most : kGroups;
 }
 
-template <int D, int DT, int NH>
-int run(const P& a, int B, hipStream_t st) {
-    const unsigned grid = a.groups ? (unsigned)a.groups : (unsigned)(B * a.Hkv * a.HG);
-    if (a.scores)
-        hipLaunchKernelGGL((decode_kernel<D, DT, NH, true>), dim3(grid), dim3(64 * kWaves), 0, st, a);
+template <int D, int DT, int NH, bool SC>
+void run(const P& a, hipStream_t st) {
+    const unsigned rows = (unsigned)(a.B * a.Hkv);
+    if (!a.groups) {
+        hipLaunchKernelGGL((decode_kernel<D, DT, NH, SC, true>), dim3(rows * a.HG), dim3(64 * kRowWaves), 0, st, a);
+        return;
+    }
+    hipLaunchKernelGGL((decode_kernel<D, DT, NH, SC, false>), dim3((unsigned)a.groups), dim3(64 * kWaves), 0, st, a);
+    const unsigned heads = rows * a.G, chunks = (unsigned)(a.cap + 1023) / 1024 * rows;
+    const bool waves = heads > 512;      // a wave a query head, or a workgroup
+    if (SC && waves)
+        hipLaunchKernelGGL((join_weights_kernel<D, DT, NH, 64>), dim3(chunks), dim3(256), 0, st, a);
+    else if (SC)
+        hipLaunchKernelGGL((join_weights_kernel<D, DT, NH, 256>), dim3(chunks), dim3(256), 0, st, a);
+    else if (waves)
+        hipLaunchKernelGGL((join_kernel<D, DT, NH, 64>), dim3((heads + 3) / 4), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((decode_kernel<D, DT, NH, false>), dim3(grid), dim3(64 * kWaves), 0, st, a);
-    if (a.groups)
-        hipLaunchKernelGGL((join_kernel<D, DT, NH>), dim3((unsigned)(B * a.Hkv * a.G)), dim3(256), 0, st, a);
-    if (a.scores)
-        hipLaunchKernelGGL(weights_kernel, dim3((unsigned)(a.cap + 1023) / 1024 * (unsigned)(B * a.Hkv)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((join_kernel<D, DT, NH, 256>), dim3(heads), dim3(256), 0, st, a);
+}
+
+template <int D, int DT, int NH>
+int run_scores(const P& a, hipStream_t st) {
+    if (a.scores) run<D, DT, NH, true>(a, st);
+    else run<D, DT, NH, false>(a, st);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
 template <int D, int DT>
-int run_heads(const P& a, int B, hipStream_t st) {
+int run_heads(const P& a, hipStream_t st) {
     const int n = head_waves(a.G);
-    return n == 1 ? run<D, DT, 1>(a, B, st) : n == 2 ? run<D, DT, 2>(a, B, st) : run<D, DT, 4>(a, B, st);
+    return n == 1 ? run_scores<D, DT, 1>(a, st) : n == 2 ? run_scores<D, DT, 2>(a, st) : run_scores<D, DT, 4>(a, st);
 }
 
 }  // namespace
@@ -554,7 +715,7 @@ size_t decode_workspace(const tkm_attn_kv& kv, int Hq, int add_weights) {
     const int G = Hq / kv.Hkv;
     const long long cap = (long long)kv.max_pages * kv.page;
     size_t n = 0;
-    if (!by_row((int)cap)) {
+    if (!by_row(kv, Hq, add_weights)) {
         const size_t slots = (size_t)groups_of(kv, Hq) * (kWaves / head_waves(G)) * 2 * head_cols(G);
         n += up256(slots * kv.D * 4) + up256(slots * 8);
     }
@@ -583,7 +744,7 @@ int launch_decode(const DecodeArgs& d) {
     a.max_pages = kv.max_pages;
     a.cap = kv.max_pages * kv.page;
     a.sl2 = d.scale * 1.4426950408889634f;
-    a.groups = by_row(a.cap) ? 0 : groups_of(kv, d.Hq);
+    a.groups = by_row(kv, d.Hq, d.add_weights) ? 0 : groups_of(kv, d.Hq);
     char* ws = (char*)d.ws;
     if (a.groups) {
         const size_t slots = (size_t)a.groups * (kWaves / head_waves(a.G)) * 2 * a.cols;
@@ -599,9 +760,9 @@ int launch_decode(const DecodeArgs& d) {
         a.scores = (float*)ws;
     }
     hipStream_t st = (hipStream_t)d.stream;
-    note_kernels(kDecode | (a.groups ? kJoin : 0u) | (a.scores ? kWeights : 0u));
-    return kv.D == 64 ? (kv.dtype == TKM_ATTN_BF16 ? run_heads<64, DT_BF16>(a, kv.B, st) : run_heads<64, DT_F16>(a, kv.B, st))
-                      : (kv.dtype == TKM_ATTN_BF16 ? run_heads<128, DT_BF16>(a, kv.B, st) : run_heads<128, DT_F16>(a, kv.B, st));
+    note_kernels(kDecode | (!a.groups ? 0u : a.scores ? kJoin | kWeights : kJoin));
+    return kv.D == 64 ? (kv.dtype == TKM_ATTN_BF16 ? run_heads<64, DT_BF16>(a, st) : run_heads<64, DT_F16>(a, st))
+                      : (kv.dtype == TKM_ATTN_BF16 ? run_heads<128, DT_BF16>(a, st) : run_heads<128, DT_F16>(a, st));
 }
 
 }  // namespace tkm
