@@ -152,7 +152,7 @@ TKM_ATTN_API int tkm_attn_kv_append(const tkm_attn_kv *kv, const void *qkv, int 
                                     const int32_t *n_new, void *stream);
 
 /* Bytes of device workspace tkm_attn_decode needs for this cache: the pieces of rows that several
- * workgroups share, at most 512 * 8 * 16 * (D + 2) floats (none for tables of few tokens), and with
+ * workgroups share, at most 256 * 8 * 16 * (D + 2) floats (none for tables of few tokens), and with
  * add_weights the scores, B * Hq * (max_pages * page + 1) floats.  0 also if it refuses the
  * arguments.  It holds nothing from call to call; calls that may overlap need one each. */
 TKM_ATTN_API size_t tkm_attn_decode_workspace_bytes(const tkm_attn_kv *kv, int Hq, int add_weights);

@@ -99,7 +99,7 @@ def test_decode_workspace():
     L = attn.lib()
     small, large = kv(max_pages=1), kv(max_pages=1000)
     assert 0 == L.tkm_attn_decode_workspace_bytes(ref(small), 4, 0) < L.tkm_attn_decode_workspace_bytes(ref(large), 4, 0)
-    assert L.tkm_attn_decode_workspace_bytes(ref(large), 4, 0) <= 512 * 8 * 2 * 66 * 4 + 4096
+    assert L.tkm_attn_decode_workspace_bytes(ref(large), 4, 0) <= 256 * 8 * 2 * 66 * 4 + 4096
     assert L.tkm_attn_decode_workspace_bytes(ref(small), 4, 1) >= 2 * 4 * 65 * 4
     assert L.tkm_attn_decode_workspace_bytes(ref(kv(D=80)), 4, 0) == 0
     assert L.tkm_attn_decode_workspace_bytes(ref(small), 5, 0) == 0

@@ -18,8 +18,10 @@
 //
 // Split over the length: all tiles of all rows (row = sequence, kv head, group of query heads) are numbered
 // row after row, and every workgroup takes the same count T of consecutive ones, whatever the lengths are:
-// the lengths are read on the device, so a captured launch fits any. T is the least that 512 (two to a CU)
-// workgroups cover. A workgroup whose tiles lie in one row deals them to its 4 waves in turn and merges
+// the lengths are read on the device, so a captured launch fits any. T is the least that 256 workgroups
+// cover, one on each compute unit (us at 131035 tokens, 8 kv heads of D 128 / 64 sequences of up to 4096 / 16 of up to
+// 8192 on one kv head, both kernels: 256 97.7 / 128.7 / 17.9, 512 99.3 / 130.0 / 20.5, 1024 99.9 / 133 / 21.8: more
+// leave more pieces). A workgroup whose tiles lie in one row deals them to its 4 waves in turn and merges
 // them through LDS; otherwise each wave takes a quarter of the range by itself. Rows that no one worker has
 // whole are merged from the pieces in a second launch, in the order of the tokens: results do not depend on
 // timing.
@@ -38,7 +40,7 @@ constexpr float kSlack = 8.0f;   // m moves when a score exceeds it by more than
 constexpr float kLift = 6.0f;    // P = 2^(s - m + kLift)
 constexpr int kWaves = 4;        // waves of a workgroup of a split launch
 constexpr int kRowWaves = 8;     // and where a workgroup has a row
-constexpr int kGroups = 512;     // workgroups of a split launch: two on each of 256 compute units
+constexpr int kGroups = 256;     // workgroups of a split launch: one on each compute unit
 constexpr float kLn2 = 0.69314718055994531f;
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
