@@ -12,7 +12,9 @@
 //
 // One workgroup of 16 waves has a row and goes over it three or four times, 8 words a thread a turn:
 //   1  the largest logit (where T <= 0, then its first index, and that is all)
-//   2  with top-k or top-p, a histogram of the logits' order-preserving bits, the upper 13: counts, sums of weights
+//   2  a histogram of the logits' order-preserving bits, the upper 13: counts for top-k.  If the bin of top-k's border
+//      and those above it have at most 2048 words, these go to a list in LDS, and the rest needs no more of the row.
+//      Otherwise, and for top-p alone, one of sums of weights
 //   3  the sums of segments of 512 words over all words in the bins above the border's, and a list in LDS of the
 //      border's bin.  The list (a histogram of 10 bits more first, if it is long) gives the border's own bits and
 //      how many of the words that equal it are in; its kept words are then added to their segments.  A bin that
@@ -324,21 +326,31 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
         least = fmaxf(least, fminf(top, f));
     }
 
-    // 2: the histogram
-    if (by_k || by_p) {
+    // 2: the histogram: of counts, which give the bin of top-k's border; if the list takes that bin and all above it,
+    // it is all that matters of the row.  Otherwise of sums, if top-p asks for them.
+    uint32_t bin_k = kNoBin;
+    uint64_t before_k = 0, none = 0;
+    bool full = false;
+    if (by_k) {
         each([&](int, const float (&x)[kPer]) {
-            if (by_p) {
-                uint64_t q[kPer];
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) q[j] = wt.of(x[j]);
+            for (int j = 0; j < kPer; ++j)
+                if (x[j] >= kLeast) atomicAdd(&lds.n0[key_of(x[j]) >> kLow0], 1u);
+        });
+        __syncthreads();
+        bin_k = find_bin<kBits0>(lds, flip, lds.n0, lds.s0, true, [&](uint64_t all) { return (uint64_t)top_k < all ? (uint64_t)top_k : 0; },
+                                 before_k, false, none);
+        by_k = bin_k != kNoBin;            // else all words are in
+        full = by_k && before_k + lds.n0[bin_k] <= kList;
+    }
+    if (by_p && !full) {
+        each([&](int, const float (&x)[kPer]) {
+            uint64_t q[kPer];
 #pragma unroll
-                for (int j = 0; j < kPer; ++j)
-                    if (q[j]) atomicAdd((unsigned long long*)&lds.s0[key_of(x[j]) >> kLow0], (unsigned long long)q[j]);
-            }
-            if (by_k)
+            for (int j = 0; j < kPer; ++j) q[j] = wt.of(x[j]);
 #pragma unroll
-                for (int j = 0; j < kPer; ++j)
-                    if (x[j] >= kLeast) atomicAdd(&lds.n0[key_of(x[j]) >> kLow0], 1u);
+            for (int j = 0; j < kPer; ++j)
+                if (q[j]) atomicAdd((unsigned long long*)&lds.s0[key_of(x[j]) >> kLow0], (unsigned long long)q[j]);
         });
         __syncthreads();
     }
@@ -346,34 +358,46 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     // 3: the border: kept are the words above `border`, and the first `in` of those equal to it.  Step 0 finds
     // top-k's, step 1 top-p's, step 2 has the sums where no list gave them.
     float border = -INFINITY;
-    uint32_t in = 0, bin0 = kNoBin, many = 0;      // many: words of bin0, which the list has unless there are too many
+    uint32_t in = 0, bin0 = kNoBin, many = 0;      // many: words that the list has, or should have if there are too many
     bool some = false;                             // only some of the words equal to the border are in
     uint64_t kept_sum = ~0ull;                     // of what top-k keeps; ~0: everything
     for (int step = 0; step < 3; ++step) {
         const bool by_count = step == 0;
-        uint64_t goal = 0, before = 0, above = 0;
+        uint64_t goal = (uint64_t)top_k, before = 0, above = 0;
         uint32_t b0 = kNoBin;
         float low = -INFINITY, cut = least;        // words of [low, cut) go to the list, those from cut on to the sums
         if (step < 2) {
             if (by_count ? !by_k : !by_p) continue;
-            b0 = find_bin<kBits0>(lds, flip, lds.n0, lds.s0, by_count, [&](uint64_t all) {
-                if (by_count) return goal = (uint64_t)top_k < all ? (uint64_t)top_k : 0;     // else all words are in
-                kept_sum = min(kept_sum, all);
-                const double x = ceil((double)top_p * (double)kept_sum);
-                return goal = x < 1.0 ? 1 : x < (double)kept_sum ? (uint64_t)x : kept_sum;
-            }, before, by_count && by_p, above);
-            if (b0 == kNoBin) {
-                by_k = false;
-                continue;
+            if (by_count) {
+                b0 = bin_k;
+                before = before_k;
+                if (by_p && !full) {
+                    uint64_t m = 0;
+                    for (int i = tid; i < 1 << kBits0; i += kThreads) m += (uint32_t)i > b0 ? lds.s0[i] : 0;
+                    before_me(lds, flip, m, above);
+                }
+            } else {
+                if (full) {
+                    for (uint32_t i = tid; i < many; i += kThreads) {
+                        const float x = logit_of(lds.list[i]);
+                        if (x >= border) atomicAdd((unsigned long long*)&lds.s0[lds.list[i] >> kLow0], (unsigned long long)wt.of(x));
+                    }
+                    __syncthreads();
+                }
+                b0 = find_bin<kBits0>(lds, flip, lds.n0, lds.s0, false, [&](uint64_t all) {
+                    kept_sum = min(kept_sum, all);
+                    const double x = ceil((double)top_p * (double)kept_sum);
+                    return goal = x < 1.0 ? 1 : x < (double)kept_sum ? (uint64_t)x : kept_sum;
+                }, before, false, none);
             }
             low = logit_of(b0 << kLow0);
             cut = logit_of((b0 + 1) << kLow0);     // behind +inf's bin a NaN: no word is from there on
         } else {
-            if ((by_k || by_p) && many <= kList) break;
+            if ((by_k || by_p) && many <= kList) break;      // (the list is not empty)
             cut = some ? logit_of(key_of(border) + 1) : border;
         }
-        const bool list_only = by_count && by_p;   // the sums are top-p's affair
-        if (b0 != bin0 || step > 0) {
+        const bool list_only = full || (by_count && by_p);   // the sums are top-p's affair, or the list's
+        if (full ? by_count : b0 != bin0 || step > 0) {
             if (tid == 0) lds.list_n = 0;
             __syncthreads();
             const float from = cut < least ? least : cut;
@@ -417,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
                 if (step < 2) {
                     uint32_t here = 0;
 #pragma unroll
-                    for (int j = 0; j < kPer; ++j) here |= x[j] >= low && !(x[j] >= cut) ? 1u << j : 0u;
+                    for (int j = 0; j < kPer; ++j) here |= x[j] >= low && (full || !(x[j] >= cut)) ? 1u << j : 0u;
                     if (__any(here)) {
                         const uint32_t c = (uint32_t)__popc(here), s = tkm::wave_scan(c);
                         uint32_t at = 0;
@@ -443,7 +467,18 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
 
         // the border's own bits: of a long list (or bin) first 10 more, and if that leaves many words the last 9
         const uint32_t* few = lds.list;
-        uint32_t n = many, equal = 0, prefix = b0;
+        uint32_t n = full ? lds.n0[b0] : many, equal = 0, prefix = b0;
+        auto pick = [&](int below) {             // the list's words with that prefix
+            for (uint32_t i = tid; i < many; i += kThreads)
+                if (lds.list[i] >> below == prefix) lds.few[atomicAdd(&lds.few_n, 1u)] = lds.list[i];
+            few = lds.few;
+        };
+        const bool want_above = by_count && by_p && !full;
+        if (full && n <= 64) {
+            pick(kLow0);
+            __syncthreads();
+            if (tid == 0) lds.few_n = 0;
+        }
         for (int level = 1; level < 3 && n > 64; ++level) {
             uint32_t* nh = level == 1 ? lds.n1 : lds.n2;
             uint64_t* sh = level == 1 ? lds.s1 : lds.s2;
@@ -465,8 +500,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
             }
             __syncthreads();
             const auto same_goal = [&](uint64_t) { return goal; };
-            const uint32_t b1 = level == 1 ? find_bin<kBits1>(lds, flip, nh, sh, by_count, same_goal, before, list_only, above)
-                                           : find_bin<kBits2>(lds, flip, nh, sh, by_count, same_goal, before, list_only, above);
+            const uint32_t b1 = level == 1 ? find_bin<kBits1>(lds, flip, nh, sh, by_count, same_goal, before, want_above, above)
+                                           : find_bin<kBits2>(lds, flip, nh, sh, by_count, same_goal, before, want_above, above);
             prefix = prefix << bits | b1;
             equal = nh[b1];
             __syncthreads();
@@ -478,9 +513,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
                 border = logit_of(prefix);
                 n = 0;
             } else if (many <= kList && equal <= 64) {
-                for (uint32_t i = tid; i < many; i += kThreads)
-                    if (lds.list[i] >> kBits2 == prefix) lds.few[atomicAdd(&lds.few_n, 1u)] = lds.list[i];
-                few = lds.few;
+                pick(kBits2);
                 n = equal;
             }
             __syncthreads();
@@ -527,6 +560,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
         }
         if (by_count) {
             in = (uint32_t)(goal - before);
+            if (full && by_p) {
+                uint64_t m = 0;
+                for (uint32_t i = tid; i < many; i += kThreads) {
+                    const float x = logit_of(lds.list[i]);
+                    m += x > border ? wt.of(x) : 0;
+                }
+                before_me(lds, flip, m, above);
+            }
             kept_sum = above + in * wt.of(border);
         } else {
             const uint64_t q = wt.of(border);
@@ -535,6 +576,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
         some = in < equal;
     }
     if ((by_k || by_p) && many <= kList) {          // the list's kept words to their segments
+        if (full) {
+            if (tid < kSegs) {
+                lds.seg[tid] = 0;
+                lds.ties[tid] = 0;
+            }
+            __syncthreads();
+        }
         for (uint32_t i = tid; i < many; i += kThreads) {
             const float x = logit_of(lds.list[i]);
             if (x == border && some) atomicAdd(&lds.ties[lds.list_seg[i]], 1u);
