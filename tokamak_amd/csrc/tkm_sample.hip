@@ -10,11 +10,11 @@
 // most. (fp32 weights, off by 2^-24 of themselves, move the borders between 131072 words so far that about one
 // draw in 10^4 meets another word.)
 //
-// One workgroup of 16 waves has a row and goes over it three or four times, 8 words a thread a turn:
-//   1  the largest logit (where T <= 0, then its first index, and that is all)
-//   2  a histogram of the logits' order-preserving bits, the upper 13: counts for top-k.  If the bin of top-k's border
-//      and those above it have at most 2048 words, these go to a list in LDS, and the rest needs no more of the row.
-//      Otherwise, and for top-p alone, one of sums of weights
+// One workgroup of 16 waves has a row and goes over it two to four times, 8 words a thread a turn:
+//   1  the largest logit (where T <= 0, then its first index, and that is all), and for top-k a histogram of the
+//      logits' order-preserving bits, the upper 13.  If the bin of top-k's border and those above it have at most
+//      2048 words, these go to a list in LDS, and the rest needs no more of the row
+//   2  otherwise, and for top-p alone, such a histogram of the weights' sums
 //   3  the sums of segments of 512 words over all words in the bins above the border's, and a list in LDS of the
 //      border's bin.  The list (a histogram of 10 bits more first, if it is long) gives the border's own bits and
 //      how many of the words that equal it are in; its kept words are then added to their segments.  A bin that
@@ -260,30 +260,39 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     const int top_k = a.top_k ? a.top_k[r] : 0;
     const float top_p = a.top_p ? a.top_p[r] : 1.0f;
     const float min_p = a.min_p ? a.min_p[r] : 0.f;
-    const bool by_p = top_p < 1.0f;
-    bool by_k = top_k > 0 && top_k < V;
+    const bool by_p = T > 0.f && top_p < 1.0f;
+    bool by_k = T > 0.f && top_k > 0 && top_k < V;
 
-    // 1: the largest
-    float top = -INFINITY;
-    each([&](int, const float (&x)[kPer]) {
+    // 1: the largest, and for top-k the histogram of counts.  If it is +inf, once more with only those words.
+    float top;
+    for (;; only_inf = true) {
+        if (by_k || by_p) {
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            for (int i = tid; i < (int)(offsetof(Lds, seg) / 16); i += kThreads) ((uint4*)&lds)[i] = zero;
+        }
+        if (tid < kTable) lds.pow2[tid] = exp2(tid * (1.0 / kTable));
+        if (tid < 64) lds.few_larger[tid] = lds.few_same[tid] = 0, lds.few_sum[tid] = 0;
+        if (tid == 0) lds.list_n = lds.few_n = 0;
+        if (by_k) __syncthreads();
+        top = -INFINITY;
+        each([&](int, const float (&x)[kPer]) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) top = fmaxf(top, x[j]);
-    });
+            for (int j = 0; j < kPer; ++j) {
+                top = fmaxf(top, x[j]);
+                if (by_k && x[j] >= kLeast) atomicAdd(&lds.n0[key_of(x[j]) >> kLow0], 1u);
+            }
+        });
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if (lane == 0) lds.tot[0][wave] = __float_as_uint(top);
-    if (tid < kTable) lds.pow2[tid] = exp2(tid * (1.0 / kTable));
-    if (tid < 64) lds.few_larger[tid] = lds.few_same[tid] = 0, lds.few_sum[tid] = 0;
-    if (tid == 0) lds.list_n = lds.few_n = 0;
-    if (by_k || by_p) {
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i < (int)(offsetof(Lds, seg) / 16); i += kThreads) ((uint4*)&lds)[i] = zero;
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        if (lane == 0) lds.tot[0][wave] = __float_as_uint(top);
+        __syncthreads();
+        top = __uint_as_float((uint32_t)lds.tot[0][lane & (kWaves - 1)]);
+#pragma unroll
+        for (int o = kWaves / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        flip = 1;
+        if (top < INFINITY) break;
+        __syncthreads();
     }
-    __syncthreads();
-    top = __uint_as_float((uint32_t)lds.tot[0][lane & (kWaves - 1)]);
-#pragma unroll
-    for (int o = kWaves / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    flip = 1;
     if (top == -INFINITY) {
         if (tid == 0) a.token[r] = -1;
         return;
@@ -305,10 +314,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
         }
         return;
     }
-    if (top == INFINITY) {
-        only_inf = true;
-        top = 0.f;
-    }
     Weight wt;
     wt.max = (double)top;
     wt.scale = fmax(kTable * 1.4426950408889634074 / (double)T, 1e-60);   // T = inf: any difference of two fp32 is nothing
@@ -326,18 +331,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
         least = fmaxf(least, fminf(top, f));
     }
 
-    // 2: the histogram: of counts, which give the bin of top-k's border; if the list takes that bin and all above it,
-    // it is all that matters of the row.  Otherwise of sums, if top-p asks for them.
+    // 2: the counts give the bin of top-k's border; if the list takes that bin and all above it, it is all that
+    // matters of the row.  Otherwise the histogram of sums, if top-p asks for it.
     uint32_t bin_k = kNoBin;
     uint64_t before_k = 0, none = 0;
     bool full = false;
     if (by_k) {
-        each([&](int, const float (&x)[kPer]) {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (x[j] >= kLeast) atomicAdd(&lds.n0[key_of(x[j]) >> kLow0], 1u);
-        });
-        __syncthreads();
         bin_k = find_bin<kBits0>(lds, flip, lds.n0, lds.s0, true, [&](uint64_t all) { return (uint64_t)top_k < all ? (uint64_t)top_k : 0; },
                                  before_k, false, none);
         by_k = bin_k != kNoBin;            // else all words are in
