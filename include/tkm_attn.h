@@ -134,7 +134,8 @@ TKM_ATTN_API int tkm_attn_bwd_stage(int stage, const void *qkv, const void *o, c
  * touched, and a length outside [0, max_pages * page] is never walked.  A sequence with one of
  * those that it needs gets O and LSE of NaN, loses the appended rows that fall there, is left as
  * it is by the weights and by eviction, which gives it the length -1.
- * Calls that write a cache must not overlap others on the same cache. */
+ * Calls that write a cache must not overlap others on the same cache, and no output may share
+ * memory with an input unless stated. */
 typedef struct {
     void *k, *v;
     const int32_t *table;

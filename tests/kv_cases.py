@@ -120,6 +120,5 @@ def evict_ref(w, n, budget, sink, recent):
     if n <= budget:
         return list(range(n))
     mid = list(range(sink, n - recent))
-    key = [-math.inf if math.isnan(w[i]) else w[i] for i in range(n)]
-    best = sorted(mid, key=lambda i: (-key[i], i))[:budget - sink - recent]
+    best = sorted(mid, key=lambda i: (1, 0.0, i) if math.isnan(w[i]) else (0, -w[i], i))[:budget - sink - recent]
     return list(range(sink)) + sorted(best) + list(range(n - recent, n))

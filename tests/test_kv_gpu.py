@@ -12,6 +12,7 @@ pytestmark = pytest.mark.gpu
 LENS = {
     "one": [1], "edges": [0, 1, 31, 32, 33, 63, 64, 65], "empty": [0, 0, 0], "ragged": [700, 0, 1, 2049, 513, 96],
     "long": [5003], "two": [4097, 40], "many": [(37 * i) % 301 for i in range(150)], "wide": [1300 + i for i in range(9)],
+    "crowd": [(13 * i) % 100 for i in range(69)] + [0, 3000, 0, 65] + [1] * 60,
 }
 
 
@@ -40,7 +41,7 @@ def test_decode(gpu, lens, Hq, Hkv, D, page, dtype):
 
 
 @pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [(4, 4, 64, 32, "f16"), (8, 2, 128, 64, "bf16"), (20, 1, 128, 128, "f16"), (70, 1, 64, 32, "bf16")])
-@pytest.mark.parametrize("lens", ["edges", "ragged", "long", "many"])
+@pytest.mark.parametrize("lens", ["edges", "ragged", "long", "many", "crowd"])
 def test_weights(gpu, lens, Hq, Hkv, D, page, dtype):
     from tokamak_amd import attn
     case = Case(gpu, LENS[lens], Hkv, D, page, dtype, weights=True)
@@ -89,7 +90,8 @@ def test_append(gpu, B, S, lens, Hq, Hkv, D, page, dtype, ragged, given):
 @pytest.mark.parametrize("lens,Hkv,D,page,dtype,budget,sink,recent", [
     ([300, 100, 0, 257], 2, 64, 32, "f16", 100, 4, 20), ([513, 512, 1], 1, 128, 64, "bf16", 512, 0, 0),
     ([90, 33], 3, 64, 32, "f16", 32, 16, 16), ([1500], 2, 128, 128, "f16", 1, 0, 1), ([1500, 1200], 1, 64, 256, "bf16", 700, 700, 0),
-    ([9500, 40000], 1, 64, 256, "f16", 5000, 3, 100), ([1400], 1, 64, 32, "bf16", 1399, 0, 300)])
+    ([9500, 40000], 1, 64, 256, "f16", 5000, 3, 100), ([1400], 1, 64, 32, "bf16", 1399, 0, 300),
+    ([2000], 2, 64, 32, "f16", 1800, 0, 0)])
 @pytest.mark.parametrize("in_place", [0, 1])
 @pytest.mark.parametrize("kind", ["random", "ties", "odd"])
 def test_evict(gpu, lens, Hkv, D, page, dtype, budget, sink, recent, in_place, kind):
@@ -187,6 +189,8 @@ def test_strides_and_given_buffers(gpu):
         attn.gqa_decode(q, case.cache, 8, add_weights=True)           # the cache has none
     with pytest.raises(ValueError):
         attn.kv_append(q, case.cache, 8)                              # not packed QKV
+    with pytest.raises(AttributeError):
+        case.cache.table = case.cache.table.clone()                   # the handle knows the first one's address
     with pytest.raises(ValueError):
         attn.kv_append(torch.zeros(3, 12 * 128, dtype=torch.bfloat16, device=gpu), case.cache, 8, start=case.cache.kv_len.long())
 

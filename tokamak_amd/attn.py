@@ -253,6 +253,11 @@ class KvCache:
         self._ref = ctypes.byref(self._c)
         self._ws = {}
 
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{name} cannot be replaced: write into the tensor")
+        super().__setattr__(name, value)
+
     @classmethod
     def empty(cls, B, max_pages, num_pages, Hkv, D, page=64, dtype=None, device="cuda", weights=False):
         """A cache of sequences without tokens; every table entry is -1 until the caller names a page."""

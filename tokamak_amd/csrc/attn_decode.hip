@@ -194,9 +194,9 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
         const int t = tiles_each(all, a.groups * TW);
         const int first = blockIdx.x * TW * t, last = min(first + TW * t, all);
         if (first >= last) return;
-        auto find = [&](int at) {     // the row that holds tile `at`
+        auto find = [&](int at) {     // the row that holds tile `at`; none, if the lengths have changed meanwhile
             int before = 0, n = n0, s = s0;
-            for (int c = 0;; c += 64) {
+            for (int c = 0; c < a.B; c += 64) {
                 const uint64_t m = __ballot((before + s) * RH > at);
                 if (m) {
                     const int w = __ffsll((unsigned long long)m) - 1;
@@ -206,14 +206,15 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
                     const int r = at - (before + lane_value(s, w) - it.nt) * RH;
                     it.rh = r / it.nt;
                     it.tile = r % it.nt;
-                    return;
+                    return true;
                 }
                 before += lane_value(s, 63);
                 n = c + 64 + lane < a.B ? tiles_of(a.len[c + 64 + lane], a.cap) : 0;
                 s = wave_scan(n);
             }
+            return false;
         };
-        find(first);
+        if (!find(first)) return;
         shared = last - first <= it.nt - it.tile;
         whole = shared && it.tile == 0 && last - first == it.nt;
         if (shared) {
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
             } else {
             const int mine = first + tw * t;
             if (mine >= last) return;
-            if (tw) find(mine);
+            if (tw && !find(mine)) return;
             count = min(t, last - mine);
         }
     }
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
             if (++it.rh == RH) {
                 it.rh = 0;
                 do {
-                    ++it.b;
+                    if (++it.b == a.B) return;
                     it.len = fixed(a.len, it.b);
                     it.nt = tiles_of(it.len, a.cap);
                 } while (it.nt == 0);
