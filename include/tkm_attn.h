@@ -161,9 +161,11 @@ TKM_ATTN_API size_t tkm_attn_decode_workspace_bytes(const tkm_attn_kv *kv, int H
 /* Attention of one query row a sequence over its len[b] cached positions: o [B][Hq * D] and (if
  * lse != NULL) lse [B][Hq].  q: B rows of Hq * D values, q_stride elements apart (a multiple of
  * 8; the packed row of the new token serves as it is, q_stride = (Hq + 2*Hkv) * D).  A sequence
- * of no tokens gets O = 0, LSE = -inf.  add_weights = 1 also adds, for every position j < len[b]
- * and kv head, the sum over its query heads of exp(score_j - LSE) to weight.  Results do not
- * depend on timing. */
+ * of no tokens gets O = 0, LSE = -inf, and so does a head whose scores are all -inf.  A NaN among
+ * a row's scores or values, a score of +inf or an infinite value makes what it reaches NaN; what
+ * lies behind len[b] may be anything.  add_weights = 1 also adds, for every position j < len[b]
+ * and kv head, the sum over its query heads of exp(score_j - LSE) to weight (nothing for a head
+ * whose LSE is -inf or NaN).  Results do not depend on timing. */
 TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv *kv, const void *q, long long q_stride, void *o, float *lse,
                                  int Hq, float scale, int add_weights, void *workspace, size_t workspace_bytes,
                                  void *stream);
@@ -207,7 +209,7 @@ enum {
     TKM_ATTN_K_DELTA_HIP = 64,  /* fa_bwd_delta_kernel (HIP) */
     TKM_ATTN_K_DECODE = 128,    /* decode_kernel */
     TKM_ATTN_K_JOIN = 256,      /* join_kernel: rows that several workgroups of it shared */
-    TKM_ATTN_K_WEIGHTS = 512,   /* weights_kernel */
+    TKM_ATTN_K_WEIGHTS = 512,   /* join_weights_kernel: the same, with the weights (JOIN is set too) */
     TKM_ATTN_K_APPEND = 1024,   /* append_*_kernel */
     TKM_ATTN_K_EVICT = 2048     /* select_kernel, move_kernel */
 };

