@@ -137,6 +137,30 @@ def test_evict(gpu, lens, Hkv, D, page, dtype, budget, sink, recent, in_place, k
     assert torch.equal(c.k.view(torch.int16), moved[0].view(torch.int16)) and torch.equal(c.v.view(torch.int16), moved[1].view(torch.int16))
 
 
+@pytest.mark.parametrize("n,extra", [(2047, 0), (2048, 0), (2048, 1), (8191, 0), (8192, 0), (8193, 0), (16383, 0), (16384, 0), (16385, 3),
+                                     (32768, 0), (49153, 0)])
+@pytest.mark.parametrize("budget,sink,recent", [(33, 0, 0), (1500, 0, 1500), (1999, 1024, 64), (2000, 4, 1000)])
+@pytest.mark.parametrize("weights", [0, 1])
+def test_evict_chooses_at_the_sizes_of_its_chunks(gpu, n, extra, budget, sink, recent, weights):
+    """Sequences as long as what a workgroup holds at a time, and one more or less; weights that are equal in crowds,
+    the border's among them; with weights in the new cache and without."""
+    from tokamak_amd import attn
+    page = 64
+    pages = (budget + page - 1) // page
+    case = Case(gpu, [n, n - 5], 1, 64, page, "f16", spare=2 * pages, extra_pages=extra, weights=True)
+    w = (case.weight * 40).floor() / 8 - 1
+    case.cache.weight.copy_(w)
+    d = attn.KvCache(case.cache.k, case.cache.v, case.free[:2 * pages].reshape(2, pages).to(torch.int32).to(gpu),
+                     torch.zeros(2, dtype=torch.int32, device=gpu), torch.zeros((2, 1, pages * page), device=gpu) if weights else None)
+    kept = attn.kv_evict(case.cache, budget, sink, recent, dst=d).cpu()
+    assert d.kv_len.tolist() == [budget] * 2
+    for b in range(2):
+        ref = evict_ref(w[b, 0].tolist(), n - 5 * b, budget, sink, recent)
+        assert kept[b, 0].tolist() == ref
+        if weights:
+            assert torch.equal(d.weight[b, 0, :budget].cpu(), w[b, 0, torch.tensor(ref)])
+
+
 @pytest.mark.parametrize("Hq,Hkv,D,dtype", [(4, 2, 64, "f16"), (8, 1, 128, "bf16")])
 @pytest.mark.parametrize("trend", [3.0, 12.0, -12.0])
 @pytest.mark.parametrize("n", [190, 4500])

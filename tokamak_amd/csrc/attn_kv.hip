@@ -14,10 +14,13 @@
 namespace tkm {
 namespace {
 
-// Elements before the 32-token tile of `tile` (within its page) of a page's kv head.
-__device__ __forceinline__ long long tile_at(const tkm_attn_kv& kv, int page, int h, int tile) {
-    return (((long long)page * kv.Hkv + h) * (kv.page / 32) + tile) * (32 * kv.D);
+// Pages are powers of two, from 32 tokens on.
+__device__ __forceinline__ int page_shift(const tkm_attn_kv& kv) { return __ffs(kv.page) - 1; }
+// Elements before the 32-token tile that holds position t in a page's kv head.
+__device__ __forceinline__ long long tile_at(const tkm_attn_kv& kv, int page, int h, int t) {
+    return ((((long long)page * kv.Hkv + h) << (page_shift(kv) - 5)) + ((t & (kv.page - 1)) >> 5)) * (32 * kv.D);
 }
+__device__ __forceinline__ int page_of(const tkm_attn_kv& kv, int b, int t) { return kv.table[(long long)b * kv.max_pages + (t >> page_shift(kv))]; }
 __device__ __forceinline__ bool in_pool(const tkm_attn_kv& kv, int page) { return (unsigned)page < (unsigned)kv.num_pages; }
 
 // Rows a sequence receives and where they start; the length it then has. A start outside the table writes
@@ -47,14 +50,13 @@ __global__ __launch_bounds__(256) void append_one_kernel(AppendArgs a) {
     const Rows r = rows_of(a, b);
     const int cap = kv.max_pages * kv.page;
     if (r.n == 1 && pos < cap) {
-        const int page = kv.table[(long long)b * kv.max_pages + pos / kv.page];
-        const int tile = pos % kv.page / 32, t = pos % 32, chunks = kv.D / 8;
+        const int page = page_of(kv, b, pos), t = pos % 32, chunks = kv.D / 8;
         if (in_pool(kv, page)) {
             const uint16_t* row = (const uint16_t*)a.qkv + ((long long)b * (a.Hq + 2 * kv.Hkv) + a.Hq) * kv.D;
             for (int i = threadIdx.x; i < 2 * kv.Hkv * chunks; i += 256) {
                 const u32x4 x = ld_global16(row + i * 8);
                 const int h = i / chunks % kv.Hkv, c = i % chunks;
-                const long long at = tile_at(kv, page, h, tile) + c / 4 * 1024;
+                const long long at = tile_at(kv, page, h, pos) + c / 4 * 1024;
                 if (i < kv.Hkv * chunks) {
                     *(u32x4*)((uint16_t*)kv.k + at + t * 32 + c % 4 * 8) = x;
                 } else {
@@ -86,9 +88,9 @@ __global__ __launch_bounds__(256) void append_rows_kernel(AppendArgs a, int tile
     const int end = (int)min((long long)r.start + r.n, (long long)cap);      // first position not written
     const int t0 = (r.start / 32 + ti) * 32;
     if (t0 >= end) return;
-    const int page = kv.table[(long long)b * kv.max_pages + t0 / kv.page];
+    const int page = page_of(kv, b, t0);
     if (!in_pool(kv, page)) return;
-    const long long at = tile_at(kv, page, h, t0 % kv.page / 32);
+    const long long at = tile_at(kv, page, h, t0);
     uint16_t* kd = (uint16_t*)kv.k + at;
     uint16_t* vd = (uint16_t*)kv.v + at;
     const int W = (a.Hq + 2 * kv.Hkv) * kv.D, chunks = kv.D / 8;
@@ -127,120 +129,133 @@ __global__ __launch_bounds__(256) void advance_kernel(AppendArgs a) {
 
 // ---- eviction -----------------------------------------------------------------------------------
 
-// A weight as an integer of the same order; NaN below all others, -0 as +0.
+// A weight as an integer of the same order, at most that of +inf; NaN below all others, -0 as +0.
 __device__ __forceinline__ uint32_t key_of(float w) {
-    if (w != w) return 0u;
     const uint32_t u = __float_as_uint(w + 0.0f);
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    const uint32_t k = u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+    return w != w ? 0u : k;
+}
+// Keys that no weight has: of a position that stays without a choice, of one behind the sequence, and none's.
+constexpr uint32_t kStays = 0xffffffffu, kGone = 0xfffffffeu, kNoKey = 0xfffffffdu;
+
+__device__ __forceinline__ uint32_t rank_in(uint64_t mask, uint32_t from) {     // from + lanes of the mask below this one
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, from));
 }
 
-constexpr int kSel = 1024, kSelWaves = kSel / 64;   // threads and waves of a selecting workgroup
-constexpr int kEach = 8, kChunk = kSel * kEach;      // weights a thread has at a time, and the workgroup
-constexpr int kSelBits[3] = {12, 10, 10};            // of a weight's key, from the top
-
-struct SelectLds {
-    uint32_t bins[1 << kSelBits[0]];
-    uint32_t tot[2][kSelWaves];
-    uint32_t flags[2][kEach * kSelWaves];
+// A selecting workgroup of T threads has EACH weights a thread at a time.
+template <int T, int EACH>
+struct Sel {
+    static constexpr int WAVES = T / 64, CHUNK = T * EACH;
+    static constexpr int BITS[3] = {T == 256 ? 11 : 12, T == 256 ? 11 : 10, 10};   // of a weight's key, from the top
+    static constexpr int PER = (1 << BITS[0]) / T;                                  // bins a thread has
+    uint32_t bins[1 << BITS[0]];
+    uint32_t tot[2][WAVES];
+    uint32_t flags[2][EACH][WAVES];
     uint32_t bin, before, many;
 };
 
-// Chooses what one kv head of one sequence keeps: writes its old positions in ascending order to `kept`, and
-// their weights to their new places.  A sequence with a length or a page that its tables cannot have gets -1s.
+// Chooses what one kv head of one sequence of n > budget tokens keeps: writes its old positions in ascending order
+// to `kept`, and their weights w to their new places wd.
 //
-// The border among the weights is found by three histograms of their keys' bits (12, 10, 10; each narrows to the
-// bin that holds the border, and the walk ends with a bin of which all are kept), of weights that stay in registers
-// where 8192 hold them all.  Then ballots number what stays: 8192 positions a barrier.  Bound by the chain of
-// barriers: as 16 rounds of counting three candidates, and 1024 positions a barrier, it took 19 us for 1180
-// tokens and 30 for 8192.
-__global__ __launch_bounds__(kSel) void select_kernel(EvictArgs a) {
-    __shared__ SelectLds lds;
-    const tkm_attn_kv& s = a.src;
-    const tkm_attn_kv& d = a.dst;
+// The border among the weights is found by three histograms of their keys' bits (12, 10, 10, or 11, 11, 10; each
+// narrows to the bin that holds the border, and the walk ends with a bin of which all are kept), of weights that
+// stay in registers where T * EACH hold them all.  Then ballots number what stays, T * EACH positions a barrier.
+// Bound by the chain of barriers and dependent loads where sequences are short (6 to 8 us for 16 heads of 1180
+// tokens, 12 for 128 of 6144), and by one workgroup's issue where they are long: 87 us for 2 heads of 110000.
+template <int T, int EACH>
+__device__ __forceinline__ void select_row(Sel<T, EACH>& lds, const EvictArgs& a, int n, const float* w, float* wd, int32_t* kept) {
+    using S = Sel<T, EACH>;
+    constexpr int PER = S::PER;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const long long row = blockIdx.x;
-    const int b = (int)(row / s.Hkv);
-    const long long cap = (long long)s.max_pages * s.page, cap_d = (long long)d.max_pages * d.page;
-    const int n = s.len[b];
-    int32_t* kept = a.kept + row * a.budget;
-    const float* w = s.weight + row * cap;
-    float* wd = d.weight ? d.weight + row * cap_d : nullptr;
-    int bad = n < 0 || n > cap;
-    float held[kEach];
-    const bool holds = n <= kChunk;
-    if (!bad) {
-        const int most = min(n, a.budget);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) held[e] = e * kSel + tid < n ? w[e * kSel + tid] : 0.f;
-        for (int i = tid; i < (n + s.page - 1) / s.page; i += kSel) bad |= !in_pool(s, s.table[(long long)b * s.max_pages + i]);
-        for (int i = tid; i < (most + d.page - 1) / d.page; i += kSel) bad |= !in_pool(d, d.table[(long long)b * d.max_pages + i]);
-    }
-    if (__syncthreads_or(bad)) {
-        for (int i = tid; i < a.budget; i += kSel) kept[i] = -1;
-        return;
-    }
-    if (n <= a.budget) {
-        for (int i = tid; i < a.budget; i += kSel) {
-            kept[i] = i < n ? i : -1;
-            if (wd && wd != w && i < n) wd[i] = w[i];
-        }
-        return;
-    }
+    const bool holds = n <= S::CHUNK;
     const int lo = a.sink, hi = n - a.recent, r = a.budget - a.sink - a.recent;
-    auto load = [&](int c, float (&x)[kEach]) {      // the weights of positions c + e * kSel + tid
+    float x[EACH], y[EACH];      // a chunk's weights, and the next one's under way
+    uint32_t key[EACH];
+    // f(e) for the positions c + e * T + tid of a chunk, e < EACH; straight code where the chunk is full, as most
+    // chunks of long sequences are
+    auto each = [&](int c, auto f) {
+        if (c + S::CHUNK <= n) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = c + e * kSel + tid;
-            x[e] = holds ? held[e] : i < n ? w[i] : 0.f;
+            for (int e = 0; e < EACH; ++e) f(e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                if (c + e * T >= n) break;
+                f(e);
+            }
         }
     };
-    // Of the positions in [lo, hi) those with a key >= sure stay, and the first `ties` of those with the key `tie`.
-    uint32_t sure = 0xffffffffu, tie = 0xffffffffu;
+    auto fetch = [&](int c) {
+        if (c + S::CHUNK <= n) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) y[e] = (w + c + e * T)[(unsigned)tid];
+        } else {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                y[e] = 0.f;
+                if (c + e * T + tid < n) y[e] = (w + c + e * T)[(unsigned)tid];
+            }
+        }
+    };
+    auto take = [&](int c) {     // the chunk that was fetched last, and its keys; fetches the next, or the first again
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) x[e] = y[e];
+        if (!holds) fetch(c + S::CHUNK < n ? c + S::CHUNK : 0);
+        if (c >= lo && c + S::CHUNK <= hi) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) key[e] = key_of(x[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int i = c + e * T + tid;
+                key[e] = i >= lo && i < hi ? key_of(x[e]) : i < n ? kStays : kGone;
+            }
+        }
+    };
+    fetch(0);
+    if (holds) take(0);
+    // Positions with a key >= sure stay, but for kGone, and the first `ties` of those with the key `tie`.
+    uint32_t sure = kStays, tie = kNoKey;
     int ties = 0, flip = 0;
     if (r > 0) {
         uint32_t prefix = 0, before = 0;
         int low = 32;
         for (int level = 0; level < 3; ++level) {
-            const int bits = kSelBits[level], bins = 1 << bits;
+            const int bits = S::BITS[level], bins = 1 << bits;
             low -= bits;
-            if (tid * 4 < bins) *(uint4*)&lds.bins[tid * 4] = make_uint4(0, 0, 0, 0);
-            __syncthreads();
-            for (int c = 0; c < n; c += kChunk) {
-                float x[kEach];
-                load(c, x);
+            if (tid * PER < bins)
 #pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int i = c + e * kSel + tid;
-                    const uint32_t k = key_of(x[e]);
-                    if (i >= lo && i < hi && (uint32_t)((uint64_t)k >> (low + bits)) == prefix)
-                        atomicAdd(&lds.bins[k >> low & (uint32_t)(bins - 1)], 1u);
-                }
+                for (int i = 0; i < PER; i += 4) *(uint4*)&lds.bins[tid * PER + i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            const uint32_t base = level ? prefix << (low + bits) : 0u, span = level ? 1u << (low + bits) : kGone;
+            for (int c = 0; c < n; c += S::CHUNK) {
+                if (!holds) take(c);
+                each(c, [&](int e) {
+                    const uint32_t k = key[e] - base;
+                    if (k < span) atomicAdd(&lds.bins[k >> low], 1u);
+                });
             }
             __syncthreads();
             // the bin, from the largest on, at which the running count reaches r
-            uint4 v = make_uint4(0, 0, 0, 0);        // bins first .. first + 3
-            const int first = bins - 4 - tid * 4;
-            if (first >= 0) v = *(const uint4*)&lds.bins[first];
-            const uint32_t sum = v.x + v.y + v.z + v.w, run = wave_scan(sum);
+            uint32_t v[PER] = {}, sum = 0;           // bins first .. first + PER - 1
+            const int first = bins - PER - tid * PER;
+            if (first >= 0) __builtin_memcpy(v, __builtin_assume_aligned(&lds.bins[first], 16), sizeof v);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) sum += v[i];
+            const uint32_t run = wave_scan(sum);
             if (lane == 63) lds.tot[flip][wave] = run;
             __syncthreads();
-            const uint32_t all = wave_scan(lane < kSelWaves ? lds.tot[flip][lane] : 0u);
+            const uint32_t all = wave_scan(lane < S::WAVES ? lds.tot[flip][lane] : 0u);
             flip ^= 1;
             uint32_t at = before + run - sum + (wave ? (uint32_t)lane_value((int)all, wave - 1) : 0u);
             if (at < (uint32_t)r && at + sum >= (uint32_t)r) {
-                int bin = first + 3;
-                if (at + v.w < (uint32_t)r) {
-                    at += v.w;
-                    --bin;
-                    if (at + v.z < (uint32_t)r) {
-                        at += v.z;
+                int bin = first + PER - 1;
+#pragma unroll
+                for (int i = PER - 1; i > 0; --i)
+                    if (bin == first + i && at + v[i] < (uint32_t)r) {
+                        at += v[i];
                         --bin;
-                        if (at + v.y < (uint32_t)r) {
-                            at += v.y;
-                            --bin;
-                        }
                     }
-                }
                 lds.bin = (uint32_t)bin;
                 lds.before = at;
                 lds.many = lds.bins[bin];
@@ -251,7 +266,7 @@ __global__ __launch_bounds__(kSel) void select_kernel(EvictArgs a) {
             if (before + lds.many == (uint32_t)r || level == 2) {
                 sure = prefix << low;
                 if (before + lds.many != (uint32_t)r) {
-                    tie = sure++;                    // keys end below 0xffffffff
+                    tie = sure++;
                     ties = r - (int)before;
                 }
                 break;
@@ -259,40 +274,85 @@ __global__ __launch_bounds__(kSel) void select_kernel(EvictArgs a) {
             __syncthreads();
         }
     }
+    uint32_t* wo = wd ? (uint32_t*)wd : (uint32_t*)kept;     // (written before kept's own value)
     uint32_t stay = 0, equal = 0;    // before this chunk
-    const uint64_t under = (1ull << lane) - 1;
-    for (int c = 0, buf = 0; c < n; c += kChunk, buf ^= 1) {
-        float x[kEach];
-        uint64_t g[kEach], t[kEach];
-        load(c, x);
+    for (int c = 0, buf = 0; c < n; c += S::CHUNK, buf ^= 1) {
+        if (!holds) take(c);
+        auto stays = [&](int e) { return __ballot(key[e] >= sure) & __ballot(key[e] != kGone); };
+        uint32_t count = 0;          // of the positions of lane e in this wave: those that stay, and << 16 those at the border
+        each(c, [&](int e) {
+            const int of = __popcll(stays(e)) | __popcll(__ballot(key[e] == tie)) << 16;
+            count = lane == e ? (uint32_t)of : count;
+        });
+        if (lane < EACH) lds.flags[buf][lane][wave] = count;
+        __syncthreads();     // also: all of the chunk's weights are here before one is overwritten in place
+        uint32_t sum = 0, mine = 0;  // of the positions of lane e: all waves', and those of the waves before this one
+        if (lane < EACH)
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = c + e * kSel + tid;
-            const uint32_t k = key_of(x[e]);
-            const bool mid = i >= lo && i < hi;
-            g[e] = __ballot(i < n && (!mid || k >= sure));
-            t[e] = __ballot(mid && ties > 0 && k == tie);
-            if (lane == 0) lds.flags[buf][e * kSelWaves + wave] = (uint32_t)(__popcll(g[e]) | __popcll(t[e]) << 16);
-        }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();             // also: all of the chunk's weights are read before one is overwritten in place
-        const uint32_t v0 = lds.flags[buf][lane * 2], v1 = lds.flags[buf][lane * 2 + 1], run = wave_scan(v0 + v1);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int at = e * kSelWaves + wave;
-            const uint32_t before = (uint32_t)(lane_value((int)(run - v0 - v1), at / 2) + (at % 2 ? lane_value((int)v0, at / 2) : 0));
-            const uint32_t ng = stay + (before & 0xffffu) + (uint32_t)__popcll(g[e] & under);
-            const uint32_t nt = equal + (before >> 16) + (uint32_t)__popcll(t[e] & under);
-            if ((g[e] >> lane & 1) || ((t[e] >> lane & 1) && nt < (uint32_t)ties)) {
-                const uint32_t to = ng + min(nt, (uint32_t)ties);
-                kept[to] = c + e * kSel + tid;
-                if (wd) wd[to] = x[e];
+            for (int v = 0; v < S::WAVES; ++v) {
+                const uint32_t f = lds.flags[buf][lane][v];
+                sum += f;
+                mine += v < wave ? f : 0;
             }
-        }
+        const uint32_t run = wave_scan(sum), before = run - sum + mine;
+        const uint32_t at_border = equal + (before >> 16), at = stay + (before & 0xffffu) + min(at_border, (uint32_t)ties);
+        each(c, [&](int e) {
+            bool in = key[e] >= sure && key[e] != kGone;
+            const uint64_t g = stays(e), t = __ballot(key[e] == tie);
+            uint32_t to = rank_in(g, (uint32_t)lane_value((int)at, e));
+            if (t) {
+                const uint32_t b0 = (uint32_t)lane_value((int)at_border, e), b = rank_in(t, b0);
+                to += min(b, (uint32_t)ties) - min(b0, (uint32_t)ties);
+                in |= key[e] == tie && b < (uint32_t)ties;
+            }
+            if (in) {
+                wo[to] = __float_as_uint(x[e]);
+                kept[to] = c + e * T + tid;
+            }
+        });
         const uint32_t last = (uint32_t)lane_value((int)run, 63);
         stay += last & 0xffffu;
         equal += last >> 16;
     }
+}
+
+// One kv head of one sequence a workgroup.  A sequence with a length or a page that its tables cannot have gets -1s.
+template <int T>
+__global__ __launch_bounds__(T) void select_kernel(EvictArgs a) {
+    constexpr int LONG = T == 256 ? 8 : 16;
+    __shared__ union {
+        Sel<T, 8> few;
+        Sel<T, LONG> many;
+    } lds;
+    const tkm_attn_kv& s = a.src;
+    const tkm_attn_kv& d = a.dst;
+    const int tid = threadIdx.x;
+    const long long row = blockIdx.x;
+    const int b = (int)(row / s.Hkv);
+    const long long cap = (long long)s.max_pages * s.page, cap_d = (long long)d.max_pages * d.page;
+    const int n = s.len[b];
+    int32_t* kept = a.kept + row * a.budget;
+    const float* w = s.weight + row * cap;
+    float* wd = d.weight ? d.weight + row * cap_d : nullptr;
+    int bad = n < 0 || n > cap;
+    if (!bad) {
+        const int most = min(n, a.budget);
+        for (int i = tid; i < (n + s.page - 1) / s.page; i += T) bad |= !in_pool(s, s.table[(long long)b * s.max_pages + i]);
+        for (int i = tid; i < (most + d.page - 1) / d.page; i += T) bad |= !in_pool(d, d.table[(long long)b * d.max_pages + i]);
+    }
+    if (__syncthreads_or(bad)) {
+        for (int i = tid; i < a.budget; i += T) kept[i] = -1;
+        return;
+    }
+    if (n <= a.budget) {
+        for (int i = tid; i < a.budget; i += T) {
+            kept[i] = i < n ? i : -1;
+            if (wd && wd != w && i < n) wd[i] = w[i];
+        }
+        return;
+    }
+    if (T == 256 || n <= T * 8) select_row<T, 8>(lds.few, a, n, w, wd, kept);
+    else select_row<T, LONG>(lds.many, a, n, w, wd, kept);
 }
 
 // Moves K and V of the kept tokens of one kv head to their new places, 256 tokens a turn and 32 dims at a time, the
@@ -311,7 +371,7 @@ __device__ __forceinline__ void move_tokens(const EvictArgs& a, int in_place, in
     const int32_t* kept = a.kept + row * a.budget;
     // element offset of a token's blocks of 32 dims, -1 for none
     auto block_of = [&](const tkm_attn_kv& kv, int t) {
-        return t < 0 ? -1ll : tile_at(kv, kv.table[(long long)b * kv.max_pages + t / kv.page], h, t % kv.page / 32);
+        return t < 0 ? -1ll : tile_at(kv, page_of(kv, b, t), h, t);
     };
     const uint16_t* vs = (const uint16_t*)s.v;
     const uint16_t* ks = (const uint16_t*)s.k;
@@ -417,12 +477,16 @@ int launch_evict(const EvictArgs& a) {
     note_kernels(kEvict);
     const int in_place = a.src.table == a.dst.table, turns = (a.budget + 255) / 256;
     const unsigned rows = (unsigned)a.src.B * a.src.Hkv;
-    hipLaunchKernelGGL(select_kernel, dim3(rows), dim3(kSel), 0, st, a);
-    // In place, and where there are few (head, turn) pairs, a workgroup has 32 dims of K or V of a head (64 pairs of
-    // D 64: 6.3 us, against 10.8 of one workgroup for all), else all of both (2048 pairs of D 128: 149 us, against
-    // 172 of one for K and one for V, and 215 of the finest).
-    const bool few = in_place || (long long)rows * turns < 1024;
-    const int parts = few ? a.src.D / 32 : 1, apart = few;
+    // Small workgroups where they hold a row: more rows at a time and cheaper barriers (1152 heads of 1226 tokens
+    // 12 us, against 41 with 1024 threads; 16 heads of 1180 8, against 11).
+    if ((long long)a.src.max_pages * a.src.page <= 2048) hipLaunchKernelGGL(select_kernel<256>, dim3(rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(select_kernel<1024>, dim3(rows), dim3(1024), 0, st, a);
+    // In place, and where there are few (head, turn) pairs, a workgroup has 32 dims of K or V of a head; where there
+    // are more, half of K's or V's dims; else all of both.  us of all / halves / 32 dims: 64 pairs of D 64 10.8 / 5.9
+    // / 5.9, 176 of D 128 8.9 / 7.0 / 9.1, 320 of D 128 26 / 22 / 25, 480 of D 128 37 / 47 / 51, 1456 of D 64 57 / 75 /
+    // 75, 2048 of D 128 149 / 172 / 215.
+    const bool few = in_place || (long long)rows * turns < 128, some = (long long)rows * turns < 400;
+    const int parts = few ? a.src.D / 32 : some ? 2 : 1, apart = few || some;
     hipLaunchKernelGGL(move_kernel, dim3(rows * parts * (apart ? 2 : 1) * (in_place ? 1 : turns)), dim3(256), 0, st, a, in_place, turns,
                        parts, apart);
     return status();
