@@ -123,7 +123,7 @@ TKM_ATTN_API int tkm_attn_bwd_stage(int stage, const void *qkv, const void *o, c
  *   k       [num_pages][Hkv][page/32][D/32][32 tokens][32 dims]   16-bit
  *   v       [num_pages][Hkv][page/32][D/32][32 dims][32 tokens]   16-bit
  *   table   [B][max_pages] int32: position j of sequence b is token j % page of page
- *           table[b][j / page]; entries behind the last position in use are not read
+ *           table[b][j / page]; entries behind the last position in use may hold anything
  *   len     [B] int32: tokens each sequence holds
  *   weight  [B][Hkv][max_pages * page] fp32, or NULL: the attention weight each position of each
  *           kv head has gathered (tkm_attn_decode adds to it, tkm_attn_kv_evict goes by it)
