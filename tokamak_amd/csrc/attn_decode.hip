@@ -9,8 +9,9 @@
 //   P^T            stays where it is: a lane holds 8 consecutive tokens of one head, which is the B operand of
 //   O^T += V^T P^T D/16 blocks of 16 dims x 16 heads, contracted over the tile's 32 tokens
 // K's rows are dealt to the two blocks so that the 8 tokens a lane ends up with are consecutive: row r of block
-// t is token 8 (r/4) + 4 t + r%4.  P goes to the second product as two 16-bit halves (hi + lo), which leaves
-// only the output's own rounding: the MFMAs have 20 times the rate that HBM can feed, so it costs no time.
+// t is token 8 (r/4) + 4 t + r%4.  P goes to the second product in 16-bit parts, two in
+// fp16 and three in bf16, which leaves what fp32 leaves (bf16's first two lose up to 2^-17 of a P): the MFMAs have 13
+// to 20 times the rate that HBM can feed, so it costs no time.
 //
 // The running maximum m moves only when a score exceeds it by more than 8 (log2 units), so that a tile needs no
 // exchange between lanes; P = exp2(s - m + 6) then stays below 2^14, and what fp16's smallest value loses of a
@@ -58,13 +59,24 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Two fp32 as 16-bit hi and lo = 16-bit(x - hi): the words {hi, lo}.
+// Two fp32 P as 16-bit parts, each what the ones before leave, rounded: the words w[0], w[1], ..  Two parts in fp16
+// hold 22 bits, three in bf16 the 24 of fp32.
 template <int DT>
-__device__ __forceinline__ u32x2 split2(float x, float y) {
-    if constexpr (DT == DT_BF16) return pack_split_bf16(x, y);
-    const uint32_t hi = pack2<DT_F16>(x, y);
-    const f16x2 h = as_f16x2(hi);
-    return u32x2{hi, pack2<DT_F16>(x - (float)h[0], y - (float)h[1])};
+constexpr int kParts = DT == DT_BF16 ? 3 : 2;
+template <int DT>
+__device__ __forceinline__ void split_p(float x, float y, uint32_t (&w)[kParts<DT>]) {
+#pragma unroll
+    for (int i = 0; i < kParts<DT>; ++i) {
+        w[i] = pack2<DT>(x, y);
+        if constexpr (DT == DT_BF16) {
+            x -= __uint_as_float(w[i] << 16);
+            y -= __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            const f16x2 h = as_f16x2(w[i]);
+            x -= (float)h[0];
+            y -= (float)h[1];
+        }
+    }
 }
 
 __device__ __forceinline__ float quad_max(float v) {   // over lanes l, l^16, l^32, l^48
@@ -313,17 +325,18 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = fast_exp2(s[i] - ref);
         l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        u32x4 hi, lo;
+        u32x4 pw[kParts<DT>];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const u32x2 w = split2<DT>(p[2 * i], p[2 * i + 1]);
-            hi[i] = w[0];
-            lo[i] = w[1];
+            uint32_t w[kParts<DT>];
+            split_p<DT>(p[2 * i], p[2 * i + 1], w);
+#pragma unroll
+            for (int j = 0; j < kParts<DT>; ++j) pw[j][i] = w[j];
         }
 #pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] = mfma16<DT>(vf[buf][db], hi, acc[db]);
+        for (int j = 0; j < kParts<DT>; ++j)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] = mfma16<DT>(vf[buf][db], lo, acc[db]);
+            for (int db = 0; db < DB; ++db) acc[db] = mfma16<DT>(vf[buf][db], pw[j], acc[db]);
     };
     // output row of a head of the kv head of x
     auto out_row = [&](const At& x, int h) { return ((long long)x.b * a.Hkv + x.rh / a.HG) * a.G + h; };
