@@ -593,6 +593,8 @@ __global__ __launch_bounds__(256) void join_kernel(P a) {
     else if (pieces_of<kWaves / NH>(a, b, kvh * a.HG + hg, nt, lane, p)) join_row<D, DT, TEAM>(a, p, c, row, t, red_o, red_ml);
 }
 
+__host__ __device__ constexpr int weight_chunks(int cap) { return (cap + 1023) / 1024; }
+
 // With weights: the same, and 1024 positions' weights of a kv head a workgroup.  Each workgroup takes the LSE of
 // the head's query heads from their pieces itself, and joins the O of every n-th of them, n the workgroups of the
 // row, so that one launch does both.
@@ -602,7 +604,7 @@ __global__ __launch_bounds__(256) void join_weights_kernel(P a) {
     __shared__ f32x2 red_ml[TEAM == 64 ? 1 : 1024 / D];
     __shared__ float l2[64];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-    const unsigned chunks = (unsigned)(a.cap + 1023) / 1024;
+    const unsigned chunks = (unsigned)weight_chunks(a.cap);
     const long long kvrow = blockIdx.x / chunks;     // sequence and kv head
     const int chunk = (int)(blockIdx.x % chunks), b = (int)(kvrow / a.Hkv), kvh = (int)(kvrow % a.Hkv);
     const int len = a.len[b], nt = tiles_of(len, a.cap);
@@ -694,15 +696,18 @@ int groups_of(const tkm_attn_kv& kv, int Hq) {
     return most < kGroups ? (int)most : kGroups;
 }
 
+int status() { return hipGetLastError() == hipSuccess ? 0 : -1; }
+
 template <int D, int DT, int NH, bool SC>
-void run(const P& a, hipStream_t st) {
+int run(const P& a, hipStream_t st) {
     const unsigned rows = (unsigned)(a.B * a.Hkv);
     if (!a.groups) {
         hipLaunchKernelGGL((decode_kernel<D, DT, NH, SC, true>), dim3(rows * a.HG), dim3(64 * kRowWaves), 0, st, a);
-        return;
+        return status();
     }
     hipLaunchKernelGGL((decode_kernel<D, DT, NH, SC, false>), dim3((unsigned)a.groups), dim3(64 * kWaves), 0, st, a);
-    const unsigned heads = rows * a.G, chunks = (unsigned)(a.cap + 1023) / 1024 * rows;
+    if (status()) return -1;      // there are no pieces to join
+    const unsigned heads = rows * a.G, chunks = (unsigned)weight_chunks(a.cap) * rows;
     const bool waves = heads > 512;      // a wave a query head, or a workgroup
     if (SC && waves)
         hipLaunchKernelGGL((join_weights_kernel<D, DT, NH, 64>), dim3(chunks), dim3(256), 0, st, a);
@@ -712,13 +717,12 @@ void run(const P& a, hipStream_t st) {
         hipLaunchKernelGGL((join_kernel<D, DT, NH, 64>), dim3((heads + 3) / 4), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((join_kernel<D, DT, NH, 256>), dim3(heads), dim3(256), 0, st, a);
+    return status();
 }
 
 template <int D, int DT, int NH>
 int run_scores(const P& a, hipStream_t st) {
-    if (a.scores) run<D, DT, NH, true>(a, st);
-    else run<D, DT, NH, false>(a, st);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return a.scores ? run<D, DT, NH, true>(a, st) : run<D, DT, NH, false>(a, st);
 }
 
 template <int D, int DT>
@@ -731,6 +735,14 @@ int run_heads(const P& a, hipStream_t st) {
 
 double decode_tiles_most(const tkm_attn_kv& kv, int Hq) {
     return (double)kv.B * kv.Hkv * head_groups(Hq / kv.Hkv) * kv.max_pages * (kv.page / 32);
+}
+
+// (The join's launch without weights has at most 64 threads a query head where these are many, and B * Hq * D at most
+// 2^30: it always fits.)
+bool decode_fits(const tkm_attn_kv& kv, int Hq, int add_weights) {
+    const double rows = (double)kv.B * kv.Hkv;
+    if (by_row(kv, Hq, add_weights)) return launch_fits(rows * head_groups(Hq / kv.Hkv), 64 * kRowWaves);
+    return !add_weights || launch_fits(rows * weight_chunks(kv.max_pages * kv.page), 256);
 }
 
 size_t decode_workspace(const tkm_attn_kv& kv, int Hq, int add_weights) {

@@ -45,7 +45,14 @@ struct EvictArgs {
     void* stream;
 };
 
-// Each launches on args.stream and returns 0, or -1 when a launch failed.
+// Whether a call's launches stay below the 2^32 threads that HIP takes (of arguments that are valid otherwise).
+inline bool launch_fits(double groups, int threads) { return groups * threads < 4294967296.0; }
+bool append_fits(const tkm_attn_kv& kv, int S);
+bool decode_fits(const tkm_attn_kv& kv, int Hq, int add_weights);
+bool evict_fits(const tkm_attn_kv& src, const tkm_attn_kv& dst, int budget);
+
+// Each launches on args.stream, of a call that fits, and returns 0, or -1 when a launch failed (what depends on it is
+// then not launched).
 int launch_append(const AppendArgs& a);
 int launch_decode(const DecodeArgs& a);
 int launch_evict(const EvictArgs& a);

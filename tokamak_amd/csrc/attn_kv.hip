@@ -459,6 +459,13 @@ int status() { return hipGetLastError() == hipSuccess ? 0 : -1; }
 
 }  // namespace
 
+// Tiles that S rows starting anywhere may touch.
+static int append_tiles(int S) { return S / 32 + (S % 32 > 1 ? 2 : 1); }
+
+bool append_fits(const tkm_attn_kv& kv, int S) {
+    return launch_fits(S == 1 ? (double)kv.B : (double)kv.B * kv.Hkv * append_tiles(S), 256);
+}
+
 int launch_append(const AppendArgs& a) {
     hipStream_t st = (hipStream_t)a.stream;
     note_kernels(kAppend);
@@ -466,29 +473,51 @@ int launch_append(const AppendArgs& a) {
         hipLaunchKernelGGL(append_one_kernel, dim3((unsigned)a.kv.B), dim3(256), 0, st, a);
         return status();
     }
-    const int tiles = (a.S + 30) / 32 + 1;     // that S rows starting anywhere may touch
+    const int tiles = append_tiles(a.S);
     hipLaunchKernelGGL(append_rows_kernel, dim3((unsigned)a.kv.B * a.kv.Hkv * tiles), dim3(256), 0, st, a, tiles);
-    if (!a.start) hipLaunchKernelGGL(advance_kernel, dim3((unsigned)(a.kv.B + 255) / 256), dim3(256), 0, st, a);
+    if (status()) return -1;
+    if (a.start) return 0;
+    hipLaunchKernelGGL(advance_kernel, dim3((unsigned)(a.kv.B + 255) / 256), dim3(256), 0, st, a);
     return status();
+}
+
+// The choosing kernel's threads: small workgroups where they hold a row, for more rows at a time and cheaper barriers
+// (1152 heads of 1226 tokens 12 us, against 41 with 1024 threads; 16 heads of 1180 8, against 11).
+static int select_threads(const tkm_attn_kv& src) { return (long long)src.max_pages * src.page <= 2048 ? 256 : 1024; }
+
+// The moving kernel's launch.  In place, and where there are few (head, turn) pairs, a workgroup has 32 dims of K or V
+// of a head; where there are more, half of K's or V's dims; else all of both.  us of all / halves / 32 dims: 64 pairs
+// of D 64 10.8 / 5.9 / 5.9, 176 of D 128 8.9 / 7.0 / 9.1, 320 of D 128 26 / 22 / 25, 480 of D 128 37 / 47 / 51, 1456 of
+// D 64 57 / 75 / 75, 2048 of D 128 149 / 172 / 215.
+struct MoveGrid {
+    int in_place, turns, parts, apart;
+    double groups;
+};
+static MoveGrid move_grid(const tkm_attn_kv& src, const tkm_attn_kv& dst, int budget) {
+    MoveGrid g;
+    g.in_place = src.table == dst.table;
+    g.turns = (budget + 255) / 256;
+    const double rows = (double)src.B * src.Hkv, pairs = rows * g.turns;
+    const bool few = g.in_place || pairs < 128, some = pairs < 400;
+    g.parts = few ? src.D / 32 : some ? 2 : 1;
+    g.apart = few || some;
+    g.groups = rows * g.parts * (g.apart ? 2 : 1) * (g.in_place ? 1 : g.turns);
+    return g;
+}
+
+bool evict_fits(const tkm_attn_kv& src, const tkm_attn_kv& dst, int budget) {
+    return launch_fits((double)src.B * src.Hkv, select_threads(src)) && launch_fits(move_grid(src, dst, budget).groups, 256);
 }
 
 int launch_evict(const EvictArgs& a) {
     hipStream_t st = (hipStream_t)a.stream;
     note_kernels(kEvict);
-    const int in_place = a.src.table == a.dst.table, turns = (a.budget + 255) / 256;
     const unsigned rows = (unsigned)a.src.B * a.src.Hkv;
-    // Small workgroups where they hold a row: more rows at a time and cheaper barriers (1152 heads of 1226 tokens
-    // 12 us, against 41 with 1024 threads; 16 heads of 1180 8, against 11).
-    if ((long long)a.src.max_pages * a.src.page <= 2048) hipLaunchKernelGGL(select_kernel<256>, dim3(rows), dim3(256), 0, st, a);
+    if (select_threads(a.src) == 256) hipLaunchKernelGGL(select_kernel<256>, dim3(rows), dim3(256), 0, st, a);
     else hipLaunchKernelGGL(select_kernel<1024>, dim3(rows), dim3(1024), 0, st, a);
-    // In place, and where there are few (head, turn) pairs, a workgroup has 32 dims of K or V of a head; where there
-    // are more, half of K's or V's dims; else all of both.  us of all / halves / 32 dims: 64 pairs of D 64 10.8 / 5.9
-    // / 5.9, 176 of D 128 8.9 / 7.0 / 9.1, 320 of D 128 26 / 22 / 25, 480 of D 128 37 / 47 / 51, 1456 of D 64 57 / 75 /
-    // 75, 2048 of D 128 149 / 172 / 215.
-    const bool few = in_place || (long long)rows * turns < 128, some = (long long)rows * turns < 400;
-    const int parts = few ? a.src.D / 32 : some ? 2 : 1, apart = few || some;
-    hipLaunchKernelGGL(move_kernel, dim3(rows * parts * (apart ? 2 : 1) * (in_place ? 1 : turns)), dim3(256), 0, st, a, in_place, turns,
-                       parts, apart);
+    if (status()) return -1;      // move_kernel goes by what the choosing kernel wrote
+    const MoveGrid g = move_grid(a.src, a.dst, a.budget);
+    hipLaunchKernelGGL(move_kernel, dim3((unsigned)g.groups), dim3(256), 0, st, a, g.in_place, g.turns, g.parts, g.apart);
     return status();
 }
 

@@ -19,7 +19,6 @@ int fail(int status, const char* fmt, ...) {
 }
 
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
-constexpr double kGridMost = 2147483647.0;
 
 int check_kv(const tkm_attn_kv* kv) {
     if (!kv) return fail(TKM_ATTN_EINVAL, "the cache must be non-null");
@@ -49,12 +48,14 @@ int check_heads(const tkm_attn_kv* kv, int Hq) {
     return TKM_ATTN_OK;
 }
 
-int check_decode(const tkm_attn_kv* kv, int Hq) {
+int check_decode(const tkm_attn_kv* kv, int Hq, int add_weights) {
     int rc = check_kv(kv);
     if (!rc) rc = check_heads(kv, Hq);
-    if (!rc && tkm::decode_tiles_most(*kv, Hq) > 1073741824.0)
+    if (rc) return rc;
+    if (tkm::decode_tiles_most(*kv, Hq) > 1073741824.0)
         return fail(TKM_ATTN_EUNSUPPORTED, "the cache's tables hold too many tiles of 32 tokens");
-    return rc;
+    if (!tkm::decode_fits(*kv, Hq, add_weights)) return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
+    return TKM_ATTN_OK;
 }
 
 }  // namespace
@@ -72,8 +73,7 @@ TKM_ATTN_API int tkm_attn_kv_append(const tkm_attn_kv* kv, const void* qkv, int 
     if (!aligned(qkv, 16) || !aligned(start, 4) || !aligned(n_new, 4))
         return fail(TKM_ATTN_EALIGN, "qkv must be 16-byte aligned, start and n_new 4-byte");
     if (n_new == kv->len) return fail(TKM_ATTN_EINVAL, "n_new must not be the cache's own len");
-    if ((double)kv->B * kv->Hkv * ((S + 30.0) / 32 + 1) > kGridMost || S > 268435456)
-        return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
+    if (!tkm::append_fits(*kv, S)) return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
     if (start == kv->len) start = nullptr;
     const tkm::AppendArgs a{*kv, qkv, S, Hq, start, n_new, stream};
     if (tkm::launch_append(a)) return fail(TKM_ATTN_ELAUNCH, "append: kernel launch failed");
@@ -81,13 +81,13 @@ TKM_ATTN_API int tkm_attn_kv_append(const tkm_attn_kv* kv, const void* qkv, int 
 }
 
 TKM_ATTN_API size_t tkm_attn_decode_workspace_bytes(const tkm_attn_kv* kv, int Hq, int add_weights) {
-    return check_decode(kv, Hq) ? 0 : tkm::decode_workspace(*kv, Hq, add_weights);
+    return check_decode(kv, Hq, add_weights != 0) ? 0 : tkm::decode_workspace(*kv, Hq, add_weights);
 }
 
 TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv* kv, const void* q, long long q_stride, void* o, float* lse, int Hq,
                                  float scale, int add_weights, void* workspace, size_t workspace_bytes, void* stream) {
     tkm::reset_kernels();
-    int rc = check_decode(kv, Hq);
+    int rc = check_decode(kv, Hq, add_weights != 0);
     if (rc) return rc;
     if (!q || !o) return fail(TKM_ATTN_EINVAL, "q and o must be non-null");
     if (add_weights != 0 && add_weights != 1) return fail(TKM_ATTN_EINVAL, "add_weights must be 0 or 1, got %d", add_weights);
@@ -97,8 +97,6 @@ TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv* kv, const void* q, long long
     if (!aligned(q, 16) || !aligned(o, 16) || !aligned(lse, 4))
         return fail(TKM_ATTN_EALIGN, "q and o must be 16-byte aligned, lse 4-byte");
     if (!(scale > 0.f) || scale == INFINITY) return fail(TKM_ATTN_EINVAL, "scale must be positive and finite");
-    if (add_weights && (double)kv->B * kv->Hkv * (kv->max_pages * (double)kv->page / 1024 + 1) > kGridMost)
-        return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
     const size_t need = tkm::decode_workspace(*kv, Hq, add_weights);
     if (need && (!workspace || workspace_bytes < need))
         return fail(TKM_ATTN_EWORKSPACE, "workspace of %zu bytes required, %zu given", need,
@@ -131,8 +129,7 @@ TKM_ATTN_API int tkm_attn_kv_evict(const tkm_attn_kv* src, const tkm_attn_kv* ds
         return fail(TKM_ATTN_EINVAL, "budget=%d must hold sink=%d and recent=%d", budget, sink, recent);
     if ((double)budget > (double)dst->max_pages * dst->page)
         return fail(TKM_ATTN_EINVAL, "budget=%d exceeds the %d pages of a table", budget, dst->max_pages);
-    if ((double)src->B * src->Hkv * (src->D / 16) * (in_place ? 1.0 : budget / 256.0 + 1) > kGridMost)
-        return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
+    if (!tkm::evict_fits(*src, *dst, budget)) return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
     const tkm::EvictArgs a{*src, *dst, kept, budget, sink, recent, stream};
     if (tkm::launch_evict(a)) return fail(TKM_ATTN_ELAUNCH, "evict: kernel launch failed");
     return TKM_ATTN_OK;
