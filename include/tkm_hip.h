@@ -120,7 +120,7 @@ enum { TKM_SAMPLE_F32 = 2 };             /* logits in fp32, beside TKM_ATTN_F16 
 typedef struct {
     const void *logits;                  /* `rows` rows of `vocab`, row_stride elements apart */
     size_t row_stride;
-    int rows, vocab, dtype, draws;       /* vocab at most 524288 */
+    int rows, vocab, dtype, draws;       /* vocab at most 524288, draws below 2^22 */
     const int32_t *row_index;            /* [draws]: the row of each draw, -1 gives -1; NULL: row r for draw r */
     const float *temperature;            /* each [draws] or NULL */
     const int32_t *top_k;

@@ -1221,7 +1221,7 @@ int tkm_runtime_sample(TkmRuntime *rt, const float *h_input, const tkm_sample_ar
     const char *why = NULL;
     if (!rt || !h_input || !h || !h->u || !h->token) why = "a runtime, an input, u and token are required";
     else if (tkm_runtime_output_elements(rt) == 0) why = "the graph ends in a loss, which has no inference output";
-    else if (h->draws < 1 || h->draws > (1 << 24)) why = "the number of draws must be positive (at most 2^24)";
+    else if (h->draws < 1 || h->draws >= (1 << 22)) why = "the number of draws must be positive and below 2^22";
     else if (!h->row_index && (size_t)h->draws > rows_of(&rt->graph, &rt->graph.nodes[output_node(&rt->graph)]))
         why = "more draws than rows of output need a row_index";
     if (why) {

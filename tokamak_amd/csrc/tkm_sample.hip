@@ -43,6 +43,7 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kPer = 8;    // words a thread a turn
 constexpr int kTurn = kThreads * kPer;
 constexpr int kMostVocab = 1 << 19;
+constexpr int kMostDraws = (1 << 22) - 1;      // HIP takes launches of fewer than 2^32 threads
 constexpr int kSeg = 64 * kPer, kSegs = kMostVocab / kSeg;           // words of a segment
 constexpr int kBits0 = 13, kBits1 = 10, kBits2 = 9, kLow0 = kBits1 + kBits2;
 constexpr int kList = 2048, kTable = 32, kQueue = 128;
@@ -658,6 +659,7 @@ extern "C" TKM_API int tkm_hip_sample(const tkm_sample_args* s, void* stream) {
         return fail(TKM_ATTN_EINVAL, "sizes must be positive (rows=%d draws=%d vocab=%d)", s->rows, s->draws, s->vocab);
     if (!s->row_index && s->draws > s->rows)
         return fail(TKM_ATTN_EINVAL, "%d draws of %d rows need a row_index", s->draws, s->rows);
+    if (s->draws > kMostDraws) return fail(TKM_ATTN_EUNSUPPORTED, "%d draws (at most %d)", s->draws, kMostDraws);
     if (s->dtype != TKM_ATTN_F16 && s->dtype != TKM_ATTN_BF16 && s->dtype != TKM_SAMPLE_F32)
         return fail(TKM_ATTN_EUNSUPPORTED, "dtype %d (supported: TKM_ATTN_F16, TKM_ATTN_BF16, TKM_SAMPLE_F32)", s->dtype);
     if (s->vocab > kMostVocab) return fail(TKM_ATTN_EUNSUPPORTED, "vocab=%d (at most %d)", s->vocab, kMostVocab);
