@@ -254,7 +254,7 @@ class KvCache:
         self._ws = {}
 
     def __setattr__(self, name, value):
-        if name in self.__dict__:
+        if name in self.__dict__ and value is not self.__dict__[name]:     # c.kv_len += 1 ends in c.kv_len = c.kv_len
             raise AttributeError(f"{name} cannot be replaced: write into the tensor")
         super().__setattr__(name, value)
 
