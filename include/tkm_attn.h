@@ -161,8 +161,10 @@ TKM_ATTN_API size_t tkm_attn_decode_workspace_bytes(const tkm_attn_kv *kv, int H
 /* Attention of one query row a sequence over its len[b] cached positions: o [B][Hq * D] and (if
  * lse != NULL) lse [B][Hq].  q: B rows of Hq * D values, q_stride elements apart (a multiple of
  * 8; the packed row of the new token serves as it is, q_stride = (Hq + 2*Hkv) * D).  A sequence
- * of no tokens gets O = 0, LSE = -inf, and so does a head whose scores are all -inf.  A NaN among
- * a row's scores or values, a score of +inf or an infinite value makes what it reaches NaN; what
+ * of no tokens gets O = 0, LSE = -inf, and so does a head whose scores are all -inf.  NaN and
+ * infinities go where the formula takes them, with exp in fp32: a NaN among a row's scores or a score
+ * of +inf makes O and LSE of the head NaN, a NaN value that dim of O; an infinite value makes the dim
+ * infinite, or NaN where its exp(score_j - LSE) is 0 or infinities of both signs meet.  What
  * lies behind len[b] may be anything.  add_weights = 1 also adds, for every position j < len[b]
  * and kv head, the sum over its query heads of exp(score_j - LSE) to weight (nothing for a head
  * whose LSE is -inf or NaN).  Results do not depend on timing. */

@@ -279,20 +279,24 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
         for (int db = 0; db < DB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
         bad = false;
     };
-    auto tile = [&](int buf, const At& x, int tile, auto last) {
-        const int left = decltype(last)::value ? x.len - tile * 32 : 32;         // visible tokens of the tile
+    // a tile's scores, log2 units: of tokens quad * 8 .. + 7
+    auto scores = [&](int buf, float (&s)[8]) {
         f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             s0 = mfma16<DT>(kf[buf][0][ks], qf[ks], s0);
             s1 = mfma16<DT>(kf[buf][1][ks], qf[ks], s1);
         }
-        float s[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             s[i] = s0[i] * a.sl2;
             s[4 + i] = s1[i] * a.sl2;
         }
+    };
+    auto tile = [&](int buf, const At& x, int tile, auto last) {
+        const int left = decltype(last)::value ? x.len - tile * 32 : 32;         // visible tokens of the tile
+        float s[8];
+        scores(buf, s);
         if (decltype(last)::value && left < 32) {
             // what lies behind the last token may be anything: its scores are replaced, and as 0 * NaN is not 0
             // its values become 0 too
@@ -338,6 +342,59 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[db] = mfma16<DT>(vf[buf][db], pw[j], acc[db]);
     };
+    // An infinite value times a part of P that is 0 or negative makes NaN of a sum, where exp(s - m) > 0 makes it
+    // infinite.  So sums that are NaN are looked at again, over the same tiles: which of their values are infinite, in
+    // which direction (a NaN counts as both), and whether a token's exp is 0, which leaves NaN.
+    auto recount = [&](const At& x, int n, int stride) {
+        constexpr uint32_t inf16 = DT == DT_F16 ? 0x7c00u : 0x7f80u, one = DT == DT_F16 ? 0x3c00u : 0x3f80u;
+        f32x4 up[DB], down[DB];
+#pragma unroll
+        for (int db = 0; db < DB; ++db) up[db] = down[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float ref = m == -INFINITY ? 0.f : m - kLift;
+        for (int at = x.tile; n > 0; --n, at += stride) {
+            load(0, x, at, page_of(x, at));
+            const int left = x.len - at * 32;
+            float s[8];
+            scores(0, s);
+            u32x4 some, none, keep;      // tokens whose exp is positive, or 0; those of the sequence
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                some[i] = none[i] = keep[i] = 0;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float p = fast_exp2(s[2 * i + j] - ref);
+                    some[i] |= p > 0.f ? one << 16 * j : 0u;
+                    none[i] |= p == 0.f ? one << 16 * j : 0u;
+                    keep[i] |= quad * 8 + 2 * i + j < left ? 0xffffu << 16 * j : 0u;
+                }
+            }
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                u32x4 pos, neg, any;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t w = vf[0][db][i] & keep[i];
+                    pos[i] = neg[i] = any[i] = 0;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t h = w >> 16 * j & 0xffffu, size = h & 0x7fffu;
+                        pos[i] |= size > inf16 || h == inf16 ? one << 16 * j : 0u;
+                        neg[i] |= size > inf16 || h == (inf16 | 0x8000u) ? one << 16 * j : 0u;
+                        any[i] |= size >= inf16 ? one << 16 * j : 0u;
+                    }
+                }
+                up[db] = mfma16<DT>(any, none, mfma16<DT>(pos, some, up[db]));
+                down[db] = mfma16<DT>(any, none, mfma16<DT>(neg, some, down[db]));
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool u = up[db][i] > 0.f, d = down[db][i] > 0.f;
+                if (acc[db][i] != acc[db][i] && u != d) acc[db][i] = u ? INFINITY : -INFINITY;
+            }
+    };
     // output row of a head of the kv head of x
     auto out_row = [&](const At& x, int h) { return ((long long)x.b * a.Hkv + x.rh / a.HG) * a.G + h; };
     auto put_lse = [&](long long row, float mm, float ll) {
@@ -371,6 +428,7 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
     // after it, are under way while a tile is computed.  Straight code for all but the last two, so that the
     // compiler can count what is in flight (a load under a condition, and it waits for all of them).
     auto walk = [&](const At& x, int n, int stride) {
+        const int all = n;
         reset();
         const int h = head_of(x);
         const uint16_t* qp = a.q + (long long)x.b * a.q_stride + (x.rh / a.HG * a.G + min(h, a.G - 1)) * D + quad * 8;
@@ -398,6 +456,12 @@ __global__ __launch_bounds__(64 * (ROW ? kRowWaves : kWaves), 2) void decode_ker
         } else {
             tile(0, x, at, std::true_type());
         }
+        bool nan = false;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan |= acc[db][i] != acc[db][i];
+        if (__builtin_expect(__any(nan), 0)) recount(x, all, stride);
     };
 
     if (shared) {
