@@ -113,8 +113,8 @@ TKM_API float tkm_runtime_last_loss(TkmRuntime *rt);
  * A setting array that is NULL is off (temperature 1); so are top_k <= 0 or >= vocab, top_p >= 1
  * and min_p <= 0.  The largest logit always stays.  temperature <= 0 takes the largest logit, of
  * equal ones the first.  A NaN logit counts as -inf; a row of nothing but -inf gives -1.  u is in
- * [0, 1), other values act as the nearest.  The sums are integers of 2^-45 (at 131072 words; finer
- * for fewer), so that a draw depends neither on timing nor on the order of a sum. */
+ * [0, 1), other values act as the nearest.  The sums are integers of 2^-45 at 131072 words
+ * (2^-50 for few, 2^-43 for the most), so that a draw depends neither on timing nor on the order of a sum. */
 enum { TKM_SAMPLE_F32 = 2 };             /* logits in fp32, beside TKM_ATTN_F16 and TKM_ATTN_BF16 */
 
 typedef struct {

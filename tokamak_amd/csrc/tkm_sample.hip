@@ -5,10 +5,10 @@
 //   top-k: the first k; top-p: of these the shortest head whose sum reaches p of theirs; min-p: of these w >= min_p
 //   token: the first i, in the vocabulary's order, at which the running sum of the kept w exceeds u * their sum
 //
-// Weights are summed as integers, w * 2^shift rounded to nearest (shift 44 at 131072 words and up to 50): integer
-// sums are the same in any order, so a draw does not depend on timing, and a border is off by 2^-45 a word at
-// most. (fp32 weights, off by 2^-24 of themselves, move the borders between 131072 words so far that about one
-// draw in 10^4 meets another word.)
+// Weights are summed as integers, w * 2^shift rounded to nearest (shift 45 at 131072 words, 43 at the most words, 50 at
+// few): integer sums are the same in any order, so a draw does not depend on timing, and a border is off by half of
+// 2^-shift a word at most, 2^-46 at 131072 words.  (fp32 weights, off by 2^-24 of themselves, move the borders between
+// 131072 words so far that about one draw in 10^4 meets another word.)
 //
 // One workgroup of 16 waves has a row and goes over it two to four times, 8 words a thread a turn:
 //   1  the largest logit (where T <= 0, then its first index, and that is all), and for top-k a histogram of the
@@ -19,7 +19,7 @@
 //      border's bin.  The list (a histogram of 10 bits more first, if it is long) gives the border's own bits and
 //      how many of the words that equal it are in; its kept words are then added to their segments.  A bin that
 //      does not fit the list is gone through in memory instead, and the segments after that.  (Once for each of
-//      top-k and top-p, unless their borders share a bin; a row without either has all words in 3.)
+//      top-k and top-p; a row without either has all words in 3.)
 //   4  the running sum of the segments finds the one that holds the token, and one wave finds the word in it.
 // Few words are kept of most rows, so 3 packs those a wave meets and takes 64 exponentials at a time.
 // Bound by the passes over the row (from L2 or the Infinity Cache after the first), by the fp64 operations of 2,
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     // 3: the border: kept are the words above `border`, and the first `in` of those equal to it.  Step 0 finds
     // top-k's, step 1 top-p's, step 2 has the sums where no list gave them.
     float border = -INFINITY;
-    uint32_t in = 0, bin0 = kNoBin, many = 0;      // many: words that the list has, or should have if there are too many
+    uint32_t in = 0, many = 0;      // many: words that the list has, or should have if there are too many
     bool some = false;                             // only some of the words equal to the border are in
     uint64_t kept_sum = ~0ull;                     // of what top-k keeps; ~0: everything
     for (int step = 0; step < 3; ++step) {
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
             cut = some ? logit_of(key_of(border) + 1) : border;
         }
         const bool list_only = full || (by_count && by_p);   // the sums are top-p's affair, or the list's
-        if (full ? by_count : b0 != bin0 || step > 0) {
+        if (!full || by_count) {
             if (tid == 0) lds.list_n = 0;
             __syncthreads();
             const float from = cut < least ? least : cut;
@@ -462,7 +462,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
                 }
             });
             __syncthreads();
-            bin0 = b0;
             many = lds.list_n;
         }
         if (step == 2) break;
