@@ -96,7 +96,8 @@ TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv* kv, const void* q, long long
         return fail(TKM_ATTN_EINVAL, "q_stride=%lld must be a multiple of 8 and at least Hq * D", q_stride);
     if (!aligned(q, 16) || !aligned(o, 16) || !aligned(lse, 4))
         return fail(TKM_ATTN_EALIGN, "q and o must be 16-byte aligned, lse 4-byte");
-    if (!(scale > 0.f) || scale == INFINITY) return fail(TKM_ATTN_EINVAL, "scale must be positive and finite");
+    if (!(scale > 0.f) || scale * 1.4426950408889634f == INFINITY)     // scores are in log2 units
+        return fail(TKM_ATTN_EINVAL, "scale must be positive and finite, also times log2(e)");
     const size_t need = tkm::decode_workspace(*kv, Hq, add_weights);
     if (need && (!workspace || workspace_bytes < need))
         return fail(TKM_ATTN_EWORKSPACE, "workspace of %zu bytes required, %zu given", need,
