@@ -165,7 +165,8 @@ TKM_ATTN_API size_t tkm_attn_decode_workspace_bytes(const tkm_attn_kv *kv, int H
  * infinities go where the formula takes them, with exp in fp32: a NaN among a row's scores or a score
  * of +inf makes O and LSE of the head NaN, a NaN value that dim of O; an infinite value makes the dim
  * infinite, or NaN where its exp(score_j - LSE) is 0 or infinities of both signs meet.  What
- * lies behind len[b] may be anything.  add_weights = 1 also adds, for every position j < len[b]
+ * lies behind len[b] may be anything.  Sums are fp32 with weights of up to 2^14: bf16 values beyond
+ * 2^114 over the number of tokens may overflow them.  add_weights = 1 also adds, for every position j < len[b]
  * and kv head, the sum over its query heads of exp(score_j - LSE) to weight (nothing for a head
  * whose LSE is -inf or NaN).  Results do not depend on timing. */
 TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv *kv, const void *q, long long q_stride, void *o, float *lse,
@@ -178,7 +179,8 @@ TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv *kv, const void *q, long long
  * as less than any other).  What is kept keeps its order, moves to positions 0 .. budget-1 with
  * its weights, and len[b] becomes budget; shorter sequences keep everything.  kept
  * [B][Hkv][budget] receives the old position of each new one, -1 behind the last.
- * dst NULL or src: in place (the pages must not be shared with another sequence).  Otherwise src
+ * dst NULL or src: in place (the pages must not be shared with another sequence; slower by some
+ * times for large caches, whose tokens then move in turn).  Otherwise src
  * stays as it is and K, V, weights (if dst has any) and lengths go to dst, which has a table, len
  * and weight of its own, of pages that no sequence of src uses, in the same pool or another. */
 TKM_ATTN_API int tkm_attn_kv_evict(const tkm_attn_kv *src, const tkm_attn_kv *dst, int32_t *kept, int budget,

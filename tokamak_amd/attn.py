@@ -338,7 +338,9 @@ def decode_workspace_bytes(cache, Hq, add_weights=False) -> int:
 def gqa_decode(q, cache, Hq, scale=None, out=None, lse=None, add_weights=False, workspace=None, stream=None):
     """O [B, Hq*D] and LSE [B, Hq] (fp32) of one query row a sequence over the cache.  q: [B, >= Hq*D] with the Q
     heads first, rows any multiple of 8 elements apart; the packed row of the new token does as it is.
-    add_weights: also add the softmax weights of every cached position to cache.weight."""
+    add_weights: also add the softmax weights of every cached position to cache.weight.
+    workspace: decode_workspace_bytes(cache, Hq, add_weights) bytes, allocated for the call if not given; with
+    add_weights these are over B * Hq * 4 bytes for every position that the table can hold."""
     st = _current(cache.device, stream)
     if st is None:
         with _On(cache.device, stream) as st:
@@ -379,7 +381,7 @@ def _gqa_decode(q, cache, Hq, scale, out, lse, add_weights, workspace, st):
 
 def kv_evict(cache, budget, sink=0, recent=0, dst=None, kept=None, stream=None):
     """Cuts sequences of more than `budget` tokens to the first `sink`, the last `recent` and, of the others, those
-    with the largest cache.weight, each kv head by its own; in place, or into the cache `dst`.  Returns kept
+    with the largest cache.weight, each kv head by its own; in place, or into the cache `dst` (faster).  Returns kept
     [B, Hkv, budget] int32: the old position of each new one, -1 behind the last."""
     st = _current(cache.device, stream)
     if st is None:

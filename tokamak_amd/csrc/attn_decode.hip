@@ -20,17 +20,19 @@
 // Split over the length: all tiles of all rows (row = sequence, kv head, group of query heads) are numbered
 // row after row, and every workgroup takes the same count T of consecutive ones, whatever the lengths are:
 // the lengths are read on the device, so a captured launch fits any. T is the least that 256 workgroups
-// cover, one on each compute unit (us at 131035 tokens, 8 kv heads of D 128 / 64 sequences of up to 4096 / 16 of up to
-// 8192 on one kv head, both kernels: 256 97.7 / 128.7 / 17.9, 512 99.3 / 130.0 / 20.5, 1024 99.9 / 133 / 21.8: more
+// cover, one on each compute unit (us a call at 131035 tokens, 8 kv heads of D 128 / 64 sequences of up to 4096 / 16 of up
+// to 8192 on one kv head: 256 97.8 / 125.8 / 15.5, 512 99.6 / 127.1 / 18.4, 1024 99.9 / 130.3 / 19.8: more
 // leave more pieces). A workgroup whose tiles lie in one row deals them to its 4 waves in turn and merges
 // them through LDS; otherwise each wave takes a quarter of the range by itself. Rows that no one worker has
 // whole are merged from the pieces in a second launch, in the order of the tokens: results do not depend on
 // timing.
 //
-// us on one card: 131035 tokens, 8 kv heads of D 128 (537 MB of K and V): 94, and 5 for the join: 5.4 TB/s (a loop
-// that only reads takes 84 to 88 for as much; the XCDs read at different rates, 72 to 88 us for equal shares); 64
-// sequences of up to 4096 (671 MB): 117 + 5, 5.5 TB/s; 16 of up to 8192 on one kv head of 32 query heads (42 MB):
-// 12.2 + 4.4; 200 tokens in one launch: 4.8.
+// us of the kernels: 131035 tokens, 8 kv heads of D 128 (537 MB of K and V): 93, and 5 for the join: 5.5 TB/s (a loop that
+// only reads takes 84 to 88 for as much; the XCDs read at different rates, 72 to 88 us for equal shares); 64 sequences
+// of up to 4096 (671 MB on average): 117 + 5, 5.5 TB/s; 16 of up to 8192 on one kv head of 32 query heads (42 MB):
+// 12.6 + 4.4; 200 tokens in one launch: 4.8.  With weights the second launch has a workgroup for each 1024 positions
+// that the tables can hold: 16 sequences of 500 on 8 kv heads, 8.2 + 36 in tables of 32768 (10.6 in one launch where
+// the tables hold 512).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
