@@ -146,9 +146,10 @@ __device__ __forceinline__ void add_piece(f32x2 ml, f32x4 x, float mm, f32x4& o,
 __device__ __forceinline__ float lse2_of(float m, float l) { return l > 0.f ? m - kLift + __log2f(l) : l == 0.f ? -INFINITY : NAN; }
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m - kLift) * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN; }
 
-// Four positions' weights of `row` (sequence and kv head), j .. j + 3: loaded ahead of what is added to them.
+// Four positions' weights of `row` (sequence and kv head), j .. j + 3: loaded ahead of what is added to them.  The query
+// heads' are summed first and added once: alone they may be below half a step of what a position has gathered.
 struct Weights {
-    f32x4 w;
+    f32x4 w, sum;
     float* at;
     int left;      // of the four, those of the sequence
     __device__ __forceinline__ void load(const P& a, long long row, int j, int len) {
@@ -160,12 +161,13 @@ struct Weights {
     __device__ __forceinline__ void add(f32x4 score, float l2) {
         if (!(l2 > -INFINITY)) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] += fast_exp2(score[i] - l2);
+        for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(score[i] - l2);
     }
     __device__ __forceinline__ void store() const {
-        if (left >= 4) __builtin_memcpy(at, &w, 16);
+        const f32x4 x = w + sum;
+        if (left >= 4) __builtin_memcpy(at, &x, 16);
         else
-            for (int i = 0; i < left; ++i) at[i] = w[i];
+            for (int i = 0; i < left; ++i) at[i] = x[i];
     }
 };
 
