@@ -186,6 +186,115 @@ TKM_ATTN_API int tkm_attn_decode(const tkm_attn_kv *kv, const void *q, long long
 TKM_ATTN_API int tkm_attn_kv_evict(const tkm_attn_kv *src, const tkm_attn_kv *dst, int32_t *kept, int budget,
                                    int sink, int recent, void *stream);
 
+/* ---- a serving step: packed rows of several sequences over the paged cache -----------------
+ *
+ * No reference counterpart.  A step's rows are packed: sequence b has n_new[b] of them, from row
+ * row_start[b] on, and what lies behind the last sequence's rows is never written.  In the order of
+ * use: tkm_attn_kv_plan once a step (pages, lengths, and for each row its sequence, position and
+ * slot), then for each layer tkm_attn_kv_append_rows (rotation, and K and V into that layer's pages)
+ * and tkm_attn_chunk.  Layers may share table and len, and so the plan; each has its k and v.
+ * As above, all arrays are read on the device, nothing is allocated, and every call may be captured. */
+
+/* Rotary positions: pair i of the first `rot` dims of a head turns by pos * turns[i] * 2^-64 of a
+ * circle, (x0, x1) -> factor * (x0 cos - x1 sin, x0 sin + x1 cos); the other dims pass as they are.
+ * The product with a position is exact modulo whole turns, so angles hold up to position 2^31 - 1.
+ * A plain host struct: fill it with one of the calls below, pass it by address, no device memory. */
+enum { TKM_ROPE_HALVES = 0,    /* pair i: dims i and i + rot/2 */
+       TKM_ROPE_PAIRS = 1 };   /* pair i: dims 2i and 2i + 1 */
+typedef struct {
+    int rot, layout;
+    float factor;
+    uint64_t turns[64];
+} tkm_attn_rope;
+
+/* Frequencies f_i = theta^(-2i/rot), in radians a position, and how they are scaled for contexts
+ * `scale` >= 1 times longer than the `original` ones of training:
+ *   NONE    f_i
+ *   LINEAR  f_i / scale
+ *   NTK     theta * scale^(rot / (rot - 2)) in theta's place
+ *   BANDS   t = (original f_i / 2 pi - low) / (high - low) clamped to [0, 1]: (1 - t) f_i / scale + t f_i
+ *   YARN    d(x) = rot ln(original / (2 pi x)) / (2 ln theta), a = max(floor(d(high)), 0),
+ *           b = min(ceil(d(low)), rot - 1), t = (i - a) / (b - a, or 0.001 if b <= a) clamped to
+ *           [0, 1]: t f_i / scale + (1 - t) f_i; factor 0.1 ln(scale) + 1
+ * low and high: BANDS turns over the original context (1, 4), YARN likewise (1, 32).  factor 0:
+ * the kind's own (1, but for YARN). */
+enum { TKM_ROPE_NONE = 0, TKM_ROPE_LINEAR = 1, TKM_ROPE_NTK = 2, TKM_ROPE_BANDS = 3, TKM_ROPE_YARN = 4 };
+typedef struct {
+    int rot, layout, scaling;
+    double theta, scale, original, low, high, factor;
+} tkm_attn_rope_params;
+
+TKM_ATTN_API int tkm_attn_rope_init(const tkm_attn_rope_params *p, tkm_attn_rope *rope);
+/* The same from rot/2 frequencies, radians a position, each below 2 pi * 2^31 in size. */
+TKM_ATTN_API int tkm_attn_rope_from_freqs(const double *freqs, int rot, int layout, double factor, tkm_attn_rope *rope);
+
+/* Rotates the Q and K heads of `rows` rows of (Hq + 2*Hkv) * D values, strides in elements (multiples
+ * of 8); Hkv 0: rows of Q heads.  V is copied.  out == in (and the strides equal): in place, V is left
+ * alone.  Row r is at position pos[r], or r % S where pos is NULL; a row of a negative position is
+ * left as it is in out.  inverse = 1 turns the other way, which is the gradient: din from dout.
+ * 0 rows launch nothing. */
+TKM_ATTN_API int tkm_attn_rope_rows(const tkm_attn_rope *rope, const void *in, long long in_stride, void *out,
+                                    long long out_stride, const int32_t *pos, int S, int rows, int Hq, int Hkv, int D,
+                                    int dtype, int inverse, void *stream);
+
+/* The pages that no sequence has, as a stack, and how many each sequence has; all device arrays. */
+typedef struct {
+    int32_t *free;      /* [num_pages]; the first *n_free are free, the last of them is taken first */
+    int32_t *n_free;    /* [1] */
+    int32_t *held;      /* [B]: the pages that each table row names, from its beginning on */
+} tkm_attn_pages;
+
+/* What a step does, written by tkm_attn_kv_plan; all device arrays. */
+typedef struct {
+    int32_t *n_new;       /* [B]: rows of each sequence: what it wanted, or 0 */
+    int32_t *row_start;   /* [B + 1]: its first row, and behind the last sequence the number of rows */
+    int32_t *seq, *pos;   /* [rows]: each row's sequence and position; -1 behind the last row */
+    int64_t *slot;        /* [rows]: page * the page's tokens + token; -1 behind the last row, and where
+                             the table has no page of the pool */
+} tkm_attn_plan;
+
+/* Makes room for want[b] more tokens of each sequence behind start[b] (NULL: len itself), and lays the
+ * step's rows out.  A sequence that holds more pages than start[b] + want[b] tokens need gives the rest
+ * back, in the order of sequences and positions, and their table entries become -1: want 0 and start 0
+ * end a sequence, want 0 after an eviction frees what it left.  Then, in the order of sequences, each
+ * takes the pages that it lacks, if the free ones suffice for it and all that lacked pages before it,
+ * and its rows if they fit into `rows` behind those of the sequences before it that got theirs; else it
+ * gets no page and no row (and from the first whose pages are missing on, only those that lack none go
+ * on).  So does one that would outgrow its table, wants less than 1, or whose start lies outside the
+ * table.  len[b] becomes start[b] + n_new[b].
+ * The tables' pages must be theirs alone.  With start given, a second call of the same step changes
+ * nothing.  kv's table and len are written; its k and v are not touched and may be any layer's. */
+TKM_ATTN_API int tkm_attn_kv_plan(const tkm_attn_kv *kv, const tkm_attn_pages *pages, const int32_t *want,
+                                  const int32_t *start, const tkm_attn_plan *plan, int rows, void *stream);
+
+/* Stores the K and V heads of the plan's rows of qkv (rows `stride` elements apart, a multiple of 8) in
+ * their slots, and the Q heads in q (rows q_stride apart; NULL: nowhere; qkv itself with its stride: in
+ * place), Q and K rotated to the rows' positions if rope is not NULL.  Rows of a negative position are
+ * left alone; a slot outside the pool is not written.  Weights of the stored positions become 0 (rows of
+ * a sequence or position outside the tables are passed over there).  len is not touched.  Of plan, seq, pos and slot are
+ * read; slots of two rows must differ. */
+TKM_ATTN_API int tkm_attn_kv_append_rows(const tkm_attn_kv *kv, const tkm_attn_rope *rope, const void *qkv,
+                                         long long stride, void *q, long long q_stride, const tkm_attn_plan *plan,
+                                         int rows, int Hq, void *stream);
+
+/* Bytes of device workspace tkm_attn_chunk needs; 0 also if it refuses the arguments.  It holds nothing
+ * from call to call; calls that may overlap need one each. */
+TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int rows, int Hq);
+
+/* Attention of each sequence's new rows over its len[b] cached positions, their own among them: row i
+ * of n_new[b] stands at position p = len[b] - n_new[b] + i and sees the positions j < len[b], with
+ * causal = 1 those of j <= p, and with window > 0 (causal only) of these j > p - window.
+ * q: `rows` rows of Hq * D values, q_stride elements apart (a multiple of 8); o [rows][Hq * D]; lse
+ * [rows][Hq] or NULL.  Sequence b has the rows row_start[b] .. row_start[b] + n_new[b] - 1; row_start
+ * NULL: from b * (rows / B) on, n_new NULL (only then): rows / B.  Rows outside [0, rows) are passed
+ * over, other sequences' rows must not be among them; rows of no sequence stay as they are in o and lse.
+ * A row that sees nothing gets O = 0, LSE = -inf; NaN, infinities, lengths and pages outside their
+ * bounds act as in tkm_attn_decode, and what a row does not see has no part in it, whatever it holds.
+ * Scores, softmax and sums are fp32.  Results do not depend on timing. */
+TKM_ATTN_API int tkm_attn_chunk(const tkm_attn_kv *kv, const void *q, long long q_stride, const int32_t *row_start,
+                                const int32_t *n_new, int rows, void *o, float *lse, int Hq, float scale, int causal,
+                                int window, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Loads this library's gfx950 assembly kernels (D = 128, fp16 and bf16) on the current device.  Call
  * it once per device before capturing a graph, as the runtime does at ignite; otherwise the
  * first call on a device loads them (inside a capture, with the thread's capture mode
@@ -201,7 +310,7 @@ TKM_ATTN_API int tkm_attn_init(void);
 TKM_ATTN_API int tkm_attn_asm_available(void);
 
 /* Kernels launched by the calling thread's last tkm_attn_fwd / _bwd / _bwd_stage /
- * _decode / _kv_append / _kv_evict call
+ * _decode / _kv_append / _kv_evict / _rope_rows / _kv_plan / _kv_append_rows / _chunk call
  * (OR of the bits below; 0 after a call that failed validation).  No reference counterpart. */
 enum {
     TKM_ATTN_K_FWD_ASM = 1,     /* tkm_fa_fwd_d128_f16 (assembly) */
@@ -215,7 +324,10 @@ enum {
     TKM_ATTN_K_JOIN = 256,      /* join_kernel: rows that several workgroups of it shared */
     TKM_ATTN_K_WEIGHTS = 512,   /* join_weights_kernel: the same, with the weights (JOIN is set too) */
     TKM_ATTN_K_APPEND = 1024,   /* append_*_kernel */
-    TKM_ATTN_K_EVICT = 2048     /* select_kernel, move_kernel */
+    TKM_ATTN_K_EVICT = 2048,    /* select_kernel, move_kernel */
+    TKM_ATTN_K_ROPE = 4096,     /* rope_kernel */
+    TKM_ATTN_K_PLAN = 8192,     /* plan_kernel, slots_kernel */
+    TKM_ATTN_K_CHUNK = 16384    /* chunk_kernel (JOIN is set too where rows may be shared) */
 };
 TKM_ATTN_API unsigned tkm_attn_last_kernels(void);
 

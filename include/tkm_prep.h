@@ -107,6 +107,11 @@ TKM_ATTN_API int tkm_prep_bwd(const tkm_prep *p, const void *dout, void *din,
                               float *dgamma, float *dbias, int rows, int accumulate,
                               void *workspace, size_t workspace_bytes, void *stream);
 
+/* The rotary positions of d's RoPE as include/tkm_attn.h has them (pairs, over the whole head, its
+ * exponents and rescaling): tkm_attn_rope_rows then turns a row of position p as the kernels here turn
+ * row p of a sequence, up to the rounding of their fp32 angles.  Needs has_rope = 1. */
+TKM_ATTN_API int tkm_prep_rope(const tkm_prep_desc *d, tkm_attn_rope *rope);
+
 /* The prelude every generated source starts with (static storage, do not free).
  * Counterpart of NVRTC_STANDALONE_PRELUDE, reference src/tkm_gpu.cu:722-827. */
 TKM_ATTN_API const char *tkm_hip_prelude(void);

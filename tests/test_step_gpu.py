@@ -1,0 +1,328 @@
+"""A serving step's calls on the GPU: rotary positions, the plan, the append of packed rows and the attention of new
+rows, against the operators in 64 bits (step_cases.py has the bounds).  Moves and whole numbers are compared exactly."""
+import math
+
+import pytest
+import torch
+
+from kv_cases import DT, HALF, TINY, Case, dense
+from step_cases import check_chunk, check_rounded, freqs_ref, plan_ref, rope_ref
+
+pytestmark = pytest.mark.gpu
+
+ROPES = [(128, 128, "halves", None), (128, 64, "pairs", "yarn"), (64, 40, "halves", "bands"), (64, 62, "pairs", "ntk"),
+         (64, 20, "pairs", "linear"), (128, 36, "halves", None), (64, 2, "halves", None), (128, 126, "halves", "linear"), (64, 2, "pairs", "ntk")]
+SCALED = {None: {}, "linear": {"scale": 4.0}, "ntk": {"scale": 4.0}, "bands": {"scale": 8.0}, "yarn": {"scale": 4.0}}
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def randn(shape, dtype, seed=0, mul=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * mul).to(DT[dtype])
+
+
+def rope_of(rot, layout, scaling, theta=10000.0):
+    from tokamak_amd import attn
+    return attn.Rope(rot, theta=theta, layout=layout, scaling=scaling, **SCALED[scaling]), freqs_ref(rot, theta, scaling, **SCALED[scaling])
+
+
+# ---- rotary positions ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D,rot,layout,scaling", ROPES)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,Hq,Hkv", [(1, 1, 1), (37, 8, 2), (9, 5, 0), (1500, 6, 3), (4100, 1, 1)])
+def test_rope(gpu, D, rot, layout, scaling, dtype, rows, Hq, Hkv):
+    from tokamak_amd import attn
+    print(f"[case] rows {rows} Hq{Hq} Hkv{Hkv} D{D} rot {rot} {layout} {scaling} {dtype}", flush=True)
+    r, (freqs, factor) = rope_of(rot, layout, scaling)
+    C = (Hq + 2 * Hkv) * D
+    g = torch.Generator().manual_seed(rows)
+    pos = torch.randint(0, 1 << 20, (rows,), generator=g)
+    pos[rows // 2], pos[-1] = 0, (1 << 31) - 1
+    if rows > 5:
+        pos[3], pos[4] = -1, -(1 << 31)
+    x = randn((rows, C), dtype, 1)
+    wide = torch.full((rows, C + 24), 7.0, dtype=DT[dtype], device=gpu)
+    for inverse, call in ((False, attn.rope_fwd), (True, attn.rope_bwd)):
+        e = x.double().reshape(rows, Hq + 2 * Hkv, D)
+        y, err = e.clone(), torch.zeros_like(e)
+        y[:, :Hq + Hkv], err[:, :Hq + Hkv] = rope_ref(e[:, :Hq + Hkv], pos.tolist(), freqs, factor, layout, inverse)
+        gone = pos < 0
+        wide.fill_(7.0)
+        wide[:, 8:8 + C] = -3.0
+        out = call(x.to(gpu), r, Hq, Hkv, D, i32(pos.tolist(), gpu), None, wide[:, 8:8 + C])      # rows apart, another stride
+        assert attn.last_kernels() == ["rope"]
+        got = out.cpu().double().reshape(e.shape)
+        assert (got[gone] == -3.0).all() and (wide[:, :8] == 7.0).all() and (wide[:, 8 + C:] == 7.0).all()
+        check_rounded(got[~gone], y[~gone], err[~gone], dtype, "inverse" if inverse else "forward")
+        assert torch.equal(got[~gone][..., rot:], e[~gone][..., rot:]) and torch.equal(got[~gone][:, Hq + Hkv:], e[~gone][:, Hq + Hkv:])
+        inp = x.to(gpu)
+        assert call(inp, r, Hq, Hkv, D, i32(pos.tolist(), gpu), None, inp) is inp               # in place
+        assert torch.equal(inp.cpu()[~gone], out.cpu()[~gone]) and torch.equal(inp.cpu()[gone], x[gone])
+
+
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+def test_rope_is_a_training_step(gpu, layout):
+    """Rows of sequences of S, by their place; the gradient is that of the rotation: <dy, R x> = <R^T dy, x>, and
+    differences of the rotation along dx give the same (64 bits on the CPU for both)."""
+    from tokamak_amd import attn
+    B, S, Hq, Hkv, D = 3, 50, 4, 2, 64
+    r, (freqs, factor) = rope_of(48, layout, "yarn")
+    x, dy = randn((B, S, (Hq + 2 * Hkv) * D), "f16", 1), randn((B, S, (Hq + 2 * Hkv) * D), "f16", 2)
+    y = attn.rope_fwd(x.to(gpu), r, Hq, Hkv, D, S=S)
+    dx = attn.rope_bwd(dy.to(gpu), r, Hq, Hkv, D, S=S)
+    pos = [i % S for i in range(B * S)]
+
+    def turned(v, inverse=False):
+        v = v.double().reshape(B * S, Hq + 2 * Hkv, D)
+        out, e = v.clone(), torch.zeros_like(v)
+        out[:, :Hq + Hkv], e[:, :Hq + Hkv] = rope_ref(v[:, :Hq + Hkv], pos, freqs, factor, layout, inverse)
+        return out, e
+    for got, (want, e), what in ((y, turned(x), "y"), (dx, turned(dy, True), "dx")):
+        check_rounded(got.cpu().double().reshape(want.shape), want, e, "f16", what)
+    # the gradient against differences: a linear map's are exact up to the rounding of dx, half a step a value
+    step = randn(x.shape, "f16", 3).double()
+    along = ((turned(x.double() + step)[0] - turned(x.double() - step)[0]) / 2 * dy.double().reshape(B * S, -1, D)).sum()
+    d = dx.cpu().double()
+    bound = ((HALF["f16"] * d.abs() + 2.0 ** -19 * dy.double().abs().amax() * factor + TINY["f16"]) * step.abs()).sum()
+    assert abs((d * step).sum() - along) <= bound
+
+
+def test_rope_agrees_with_prep(gpu):
+    """The rows that the qkv-prep kernels turn by their place, up to their fp32 angles: S of 300 at 1 radian a row is
+    off by 2^-24 * 300, and its sine and cosine by no more."""
+    from tokamak_amd import attn, prep
+    Hq, Hkv, D, S = 4, 2, 64, 300
+    p = prep.Prep(Hq, Hkv, D, S, rope=True, dtype="f16", scale=4.0)
+    x = randn((2 * S, p.C), "f16", 5).to(gpu)
+    want = p.fwd(x, torch.zeros(p.C, device=gpu))[0].double()
+    got = attn.rope_fwd(x, attn.Rope.of_prep(p.desc), Hq, Hkv, D, S=S).double()
+    size = x.double().abs().reshape(-1, D // 2, 2).sum(2).repeat_interleave(2, 1).reshape(got.shape)
+    assert ((got - want).abs() <= 2 * HALF["f16"] * want.abs() + (2 * 300 * 2.0 ** -24 + 2.0 ** -20) * size + 2 * TINY["f16"]).all()
+
+
+# ---- the plan -------------------------------------------------------------------------------------------
+
+
+class Pool:
+    """A cache without data to speak of, its pages and a few requests."""
+
+    def __init__(self, dev, B, page, max_pages, num_pages, held, seed=0):
+        from tokamak_amd import attn
+        g = torch.Generator().manual_seed(seed)
+        ids = torch.randperm(num_pages, generator=g).tolist()
+        self.B, self.page, self.max_pages, self.num_pages, self.dev = B, page, max_pages, num_pages, dev
+        self.table, used = [], 0
+        for n in held:
+            self.table.append(ids[used:used + n] + [-1] * (max_pages - n))
+            used += n
+        self.held, self.n_free = list(held), num_pages - used
+        self.free = ids[used:] + [-5] * used
+        pool = torch.zeros((num_pages, 1, page // 32, 2, 32, 32), dtype=torch.float16, device=dev)
+        self.cache = attn.KvCache(pool, pool.clone(), i32(self.table, dev), torch.zeros(B, dtype=torch.int32, device=dev))
+        self.pages = attn.KvPages(i32(self.free, dev), i32([self.n_free], dev), i32(self.held, dev))
+
+    def step(self, want, start, rows, given=True, plan=None):
+        from tokamak_amd import attn
+        ref = plan_ref(self.table, self.free, self.n_free, self.held, want, start, self.page, self.num_pages, rows)
+        if not given:
+            self.cache.kv_len.copy_(i32(start, self.dev))
+        p = attn.kv_plan(self.cache, self.pages, i32(want, self.dev), rows=rows, start=i32(start, self.dev) if given else None, plan=plan)
+        assert attn.last_kernels() == ["plan"]
+        self.compare(p, ref)
+        self.table, self.free, self.n_free, self.held = ref["table"], ref["free"], ref["n_free"][0], ref["held"]
+        return p, ref
+
+    def compare(self, p, ref):
+        got = {"table": self.cache.table, "free": self.pages.free, "n_free": self.pages.n_free, "held": self.pages.held,
+               "kv_len": self.cache.kv_len, "n_new": p.n_new, "row_start": p.row_start, "seq": p.seq, "pos": p.pos, "slot": p.slot}
+        for k, v in got.items():
+            assert v.tolist() == ref[k], k
+
+
+@pytest.mark.parametrize("B,page,rows,num", [(1, 32, 1, 3), (7, 64, 900, 40), (64, 32, 64, 400), (300, 32, 5000, 900), (1024, 256, 700, 3000),
+                                             (1025, 32, 9000, 2500), (2600, 64, 6000, 9000), (5000, 32, 5001, 9000)])
+@pytest.mark.parametrize("given", [0, 1])
+def test_plan(gpu, B, page, rows, num, given):
+    """Several steps in a row, with sequences that grow, end, shrink, ask for too much and lie outside their tables."""
+    g = torch.Generator().manual_seed(B)
+    most = 9
+    held = torch.randint(0, max(1, min(most, num // B) + 1), (B,), generator=g).tolist()
+    pool = Pool(gpu, B, page, most, num, held)
+    start = [max(0, h * page - int(x)) for h, x in zip(held, torch.randint(0, page, (B,), generator=g))]
+    for step in range(4):
+        print(f"[case] B{B} page{page} rows{rows} step {step}", flush=True)
+        kind = torch.randint(0, 12, (B,), generator=g).tolist()
+        size = torch.randint(1, 3 * rows // B + 3, (B,), generator=g).tolist()
+        want = [1 if k < 5 else n if k < 8 else 0 if k < 10 else -3 if k == 10 else (1 << 31) - 1 for k, n in zip(kind, size)]
+        for b in range(1, B, 5):
+            if kind[b] == 9:
+                start[b] = 0
+        if B > 6:
+            start[5], start[6] = -1, most * page + 1
+        _, ref = pool.step(want, start, rows, bool(given))
+        _, again = pool.step(want, start, rows, True) if given else (None, None)
+        if given:          # whoever got its rows gets the same again
+            assert all(a == n for a, n in zip(again["n_new"], ref["n_new"]) if n)
+        start = [max(0, n) if b not in (5, 6) else 0 for b, n in enumerate(ref["kv_len"])]
+
+
+def test_plan_edges(gpu):
+    from tokamak_amd import attn
+    pool = Pool(gpu, 3, 32, 4, 12, [4, 0, 1])
+    pool.step([0, 128, 31], [128, 0, 1], 200)                 # exactly full tables and pages
+    pool.step([1, 1, 1], [128, 128, 32], 200)                 # over them
+    pool.step([0, 0, 0], [0, 0, 0], 200)                      # all end
+    assert pool.n_free == 12
+    pool.step([128, 128, 128], [0, 0, 0], 384)                # the whole pool
+    assert pool.n_free == 0
+    pool.step([0, 5, 0], [0, 128, 128], 0)                    # no rows at all; the first one's pages come back
+    # a stack that says more than there is, and table entries and pages outside the pool, reach nothing
+    pool.pages.n_free.fill_(1 << 30)
+    pool.pages.held.copy_(i32([1 << 30, -7, 4], gpu))
+    pool.pages.free.fill_(99)
+    p = attn.kv_plan(pool.cache, pool.pages, i32([5, 70, 1], gpu), rows=100, start=i32([0, 0, 127], gpu))
+    assert p.n_new.tolist() == [5, 70, 1] and (p.slot[5:75] == -1).all() and pool.cache.table[1, :3].tolist() == [99, 99, 99]   # 70 tokens: 3 pages of none held
+    with pytest.raises(ValueError):
+        attn.kv_plan(pool.cache, pool.pages, i32([5, 70, 1], gpu))
+    with pytest.raises(ValueError):
+        attn.kv_plan(pool.cache, pool.pages, i32([5, 70], gpu), rows=4)
+
+
+# ---- packed rows into the cache ----------------------------------------------------------------------------
+
+
+def packed(starts, n_new, case, behind=3):
+    """(seq, pos, slot, row_start) lists of packed rows at the given positions of a case's pages, some rows behind."""
+    table, page = case.cache.table.tolist(), case.page
+    seq = [b for b, n in enumerate(n_new) for _ in range(n)]
+    pos = [starts[b] + i for b, n in enumerate(n_new) for i in range(n)]
+    slot = [table[b][p // page] * page + p % page for b, p in zip(seq, pos)]
+    row_start = [sum(n_new[:b]) for b in range(len(n_new) + 1)]
+    pad = [-1] * behind
+    return seq + pad, pos + pad, slot + pad, row_start
+
+
+@pytest.mark.parametrize("D,rot,layout,scaling", ROPES[:6] + [(64, 0, "halves", None), (128, 0, "halves", None)])
+@pytest.mark.parametrize("starts,n_new,Hq,Hkv,page,dtype", [
+    ([0], [1], 1, 1, 32, "f16"), ([0, 31, 200, 5], [1, 1, 1, 0], 4, 2, 32, "bf16"), ([5, 64, 0, 33], [77, 1, 0, 140], 2, 2, 64, "f16"),
+    ([3, 500], [700, 611], 6, 3, 128, "bf16"), ([0] + [7] * 40, [40] * 41, 8, 1, 256, "f16")])
+def test_append_rows(gpu, D, rot, layout, scaling, starts, n_new, Hq, Hkv, page, dtype):
+    from tokamak_amd import attn
+    print(f"[case] {len(starts)} sequences Hq{Hq} Hkv{Hkv} D{D} page{page} rot {rot} {layout} {dtype}", flush=True)
+    pages = max((s + n + page - 1) // page for s, n in zip(starts, n_new))
+    case = Case(gpu, [pages * page] * len(starts), Hkv, D, page, dtype, extra_pages=0, weights=True)
+    c = case.cache
+    seq, pos, slot, row_start = packed(starts, n_new, case)
+    rows, total = len(seq), len(seq) - 3
+    if total > 2:
+        slot[2] = case.cache.num_pages * page        # not a slot of the pool: the row's K and V go nowhere, Q is turned
+    plan = attn.KvPlan(i32(n_new, gpu), i32(row_start, gpu), i32(seq, gpu), i32(pos, gpu), torch.tensor(slot, device=gpu))
+    r, (freqs, factor) = rope_of(rot, layout, scaling) if rot else (None, (None, None))
+    W = (Hq + 2 * Hkv) * D
+    x = randn((rows, W), dtype, 3)
+    before = [t.clone() for t in (c.k, c.v, c.weight, c.kv_len)]
+    ref = x.double().reshape(rows, Hq + 2 * Hkv, D)
+    err = torch.zeros_like(ref)
+    if rot:
+        ref[:, :Hq + Hkv], err[:, :Hq + Hkv] = rope_ref(ref[:, :Hq + Hkv], [max(0, p) for p in pos], freqs, factor, layout)
+    for mode in ("new", "given", "in place"):
+        for t, old in zip((c.k, c.v, c.weight), before):
+            t.copy_(old)
+        inp = torch.full((rows, W + 16), 9.0, dtype=DT[dtype], device=gpu)[:, :W]      # rows further apart
+        inp.copy_(x)
+        given = torch.full((rows, Hq * D + 8), 5.0, dtype=DT[dtype], device=gpu)
+        q = attn.kv_append_rows(inp, c, Hq, plan, rope=r, q={"new": None, "given": given, "in place": inp}[mode])
+        assert attn.last_kernels() == ["append"]
+        if mode == "given":
+            assert q is given and (given[:, Hq * D:] == 5.0).all() and (given[total:] == 5.0).all()
+        elif mode == "in place" or rot == 0:
+            assert q is inp and torch.equal(inp[:, Hq * D:].cpu(), x[:, Hq * D:]) and torch.equal(inp[total:].cpu(), x[total:])
+        got = q[:total, :Hq * D].cpu().double().reshape(total, Hq, D)
+        check_rounded(got, ref[:total, :Hq], err[:total, :Hq], dtype, f"q {mode}")
+        assert torch.equal(got[..., rot:], ref[:total, :Hq, rot:])
+    k, v, w = (t.clone().cpu() for t in before[:3])
+    ek = torch.zeros(k.shape, dtype=torch.float64)
+    k, v = k.double(), v.double()
+    for i in range(total):
+        if 0 <= slot[i] < c.num_pages * page:
+            at, tile, tok = slot[i] // page, slot[i] % page // 32, slot[i] % 32
+            k[at, :, tile, :, tok] = ref[i, Hq:Hq + Hkv].reshape(Hkv, D // 32, 32)
+            ek[at, :, tile, :, tok] = err[i, Hq:Hq + Hkv].reshape(Hkv, D // 32, 32)
+            v[at, :, tile, :, :, tok] = ref[i, Hq + Hkv:].reshape(Hkv, D // 32, 32)
+            w[seq[i], :, pos[i]] = 0
+    assert torch.equal(c.v.cpu().double().nan_to_num(77.0), v.nan_to_num(77.0))
+    assert torch.equal(c.weight.cpu(), w) and torch.equal(c.kv_len, before[3])
+    gk = c.k.cpu().double()
+    there = torch.isfinite(k)
+    assert torch.equal(gk[~there].nan_to_num(77.0), k[~there].nan_to_num(77.0))
+    check_rounded(gk[there], k[there], ek[there] + (0 if rot else -TINY[dtype] / 2), dtype, "k")
+
+
+# ---- attention of new rows -----------------------------------------------------------------------------------
+
+SETS = {
+    "one": ([1], [1]), "edges": ([1, 31, 32, 33, 64, 65, 0, 96], [1, 5, 32, 1, 64, 2, 0, 33]), "few": ([3, 10], [7, 12]),
+    "nothing": ([0, 0], [3, 0]), "ragged": ([700, 0, 2049, 513, 96, 40], [1, 0, 300, 513, 17, 40]), "long": ([5003], [3]), "prompt": ([1500], [1500]),
+    "many": ([(37 * i) % 301 + 4 for i in range(150)], [1 + i % 3 for i in range(150)]), "two": ([4097, 40], [150, 1]),
+}
+HEADS = [(4, 4, 64, 32, "f16"), (8, 2, 128, 64, "bf16"), (16, 1, 128, 128, "f16"), (3, 1, 64, 256, "bf16"), (10, 2, 64, 64, "f16"),
+         (34, 2, 128, 32, "bf16"), (150, 1, 64, 64, "f16")]
+
+
+def queries(total, Hq, Hkv, D, dtype, dev, seed=7, mul=1.0, wide=True):
+    return randn((total, (Hq + (2 * Hkv if wide else 0)) * D), dtype, seed, mul).to(dev)
+
+
+@pytest.mark.parametrize("name", SETS)
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", HEADS)
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 1), (True, 70), (True, 1000)])
+def test_chunk(gpu, name, Hq, Hkv, D, page, dtype, causal, window):
+    from tokamak_amd import attn
+    lens, n_new = SETS[name]
+    if sum(n_new) * Hq * max(lens) > 3e7:
+        n_new = [min(n, 130) for n in n_new]
+    print(f"[case] {name} Hq{Hq} Hkv{Hkv} D{D} page{page} {dtype} causal {causal} window {window}", flush=True)
+    case = Case(gpu, lens, Hkv, D, page, dtype)
+    total = sum(n_new)
+    q = queries(total + 3, Hq, Hkv, D, dtype, gpu)
+    row_start = [sum(n_new[:b]) for b in range(len(n_new) + 1)]
+    out = torch.full((total + 3, Hq * D), 4.0, dtype=DT[dtype], device=gpu)
+    lse = torch.full((total + 3, Hq), 4.0, device=gpu)
+    attn.gqa_chunk(q, case.cache, Hq, i32(row_start, gpu), i32(n_new, gpu), causal=causal, window=window, out=out, lse=lse)
+    assert attn.last_kernels()[-1] == "chunk"
+    assert (out[total:] == 4.0).all() and (lse[total:] == 4.0).all()
+    check_chunk(case, lens, n_new, q, out, lse, Hq, causal=causal, window=window)
+    again = attn.gqa_chunk(q[:total, :Hq * D].contiguous(), case.cache, Hq, i32(row_start, gpu)[:len(lens)], i32(n_new, gpu), causal=causal, window=window)
+    check_chunk(case, lens, n_new, q, *again, Hq, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", HEADS[:3])
+def test_chunk_of_padded_rows(gpu, Hq, Hkv, D, page, dtype):
+    """A batch of S rows a sequence, all of them or the first n_new."""
+    from tokamak_amd import attn
+    lens, S = [100, 33, 900], 33
+    case = Case(gpu, lens, Hkv, D, page, dtype)
+    q = queries(3 * S, Hq, Hkv, D, dtype, gpu)
+    o, lse = attn.gqa_chunk(q, case.cache, Hq)
+    check_chunk(case, lens, [S] * 3, q, o, lse, Hq)
+    out = torch.full((3 * S, Hq * D), 4.0, dtype=DT[dtype], device=gpu)
+    o, lse = attn.gqa_chunk(q, case.cache, Hq, n_new=i32([5, 0, 32], gpu), out=out)
+    check_chunk(case, lens, [5, 0, 32], q, o, lse, Hq, row_start=[0, S, 2 * S])
+    for rows in ([5, 2 * S], [2 * S + 32, 3 * S]):
+        assert (out[rows[0]:rows[1]] == 4.0).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", HEADS[:2])
+@pytest.mark.parametrize("mul,trend,scale", [(8.0, 0.0, None), (1.0, 30.0, None), (1.0, -30.0, None), (0.01, 0.0, 1.0), (1.0, 0.0, 1e-6), (4.0, 300.0, 1.0)])
+def test_chunk_of_steep_scores(gpu, Hq, Hkv, D, page, dtype, mul, trend, scale):
+    """Scores that grow or fall along the keys by far more than fp16 holds, and flat ones."""
+    from tokamak_amd import attn
+    lens, n_new = [1400, 70], [70, 70]
+    case = Case(gpu, lens, Hkv, D, page, dtype, mul=mul, trend=trend)
+    q = queries(140, Hq, Hkv, D, dtype, gpu, mul=mul)
+    o, lse = attn.gqa_chunk(q, case.cache, Hq, scale=scale)
+    check_chunk(case, lens, n_new, q, o, lse, Hq, scale=scale)

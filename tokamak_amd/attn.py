@@ -35,6 +35,27 @@ class _Kv(ctypes.Structure):
         (n, _i) for n in ("B", "Hkv", "D", "page", "max_pages", "num_pages", "dtype")]
 
 
+class _RopeParams(ctypes.Structure):
+    """tkm_attn_rope_params"""
+    _fields_ = [("rot", _i), ("layout", _i), ("scaling", _i)] + [
+        (n, ctypes.c_double) for n in ("theta", "scale", "original", "low", "high", "factor")]
+
+
+class _Rope(ctypes.Structure):
+    """tkm_attn_rope"""
+    _fields_ = [("rot", _i), ("layout", _i), ("factor", ctypes.c_float), ("turns", ctypes.c_uint64 * 64)]
+
+
+class _Pages(ctypes.Structure):
+    """tkm_attn_pages"""
+    _fields_ = [(n, _vp) for n in ("free", "n_free", "held")]
+
+
+class _Plan(ctypes.Structure):
+    """tkm_attn_plan"""
+    _fields_ = [(n, _vp) for n in ("n_new", "row_start", "seq", "pos", "slot")]
+
+
 class AttnError(RuntimeError):
     """A tkm_attn_* call returned a non-zero status."""
 
@@ -86,6 +107,21 @@ def lib() -> ctypes.CDLL:
     L.tkm_attn_decode.restype = _i
     L.tkm_attn_kv_evict.argtypes = [kv, kv, _vp, _i, _i, _i, _vp]
     L.tkm_attn_kv_evict.restype = _i
+    ll, rope, plan = ctypes.c_longlong, ctypes.POINTER(_Rope), ctypes.POINTER(_Plan)
+    L.tkm_attn_rope_init.argtypes = [ctypes.POINTER(_RopeParams), rope]
+    L.tkm_attn_rope_init.restype = _i
+    L.tkm_attn_rope_from_freqs.argtypes = [ctypes.POINTER(ctypes.c_double), _i, _i, ctypes.c_double, rope]
+    L.tkm_attn_rope_from_freqs.restype = _i
+    L.tkm_attn_rope_rows.argtypes = [rope, _vp, ll, _vp, ll, _vp] + [_i] * 7 + [_vp]
+    L.tkm_attn_rope_rows.restype = _i
+    L.tkm_attn_kv_plan.argtypes = [kv, ctypes.POINTER(_Pages), _vp, _vp, plan, _i, _vp]
+    L.tkm_attn_kv_plan.restype = _i
+    L.tkm_attn_kv_append_rows.argtypes = [kv, rope, _vp, ll, _vp, ll, plan, _i, _i, _vp]
+    L.tkm_attn_kv_append_rows.restype = _i
+    L.tkm_attn_chunk_workspace_bytes.argtypes = [kv, _i, _i]
+    L.tkm_attn_chunk_workspace_bytes.restype = ctypes.c_size_t
+    L.tkm_attn_chunk.argtypes = [kv, _vp, ll, _vp, _vp, _i, _vp, _vp, _i, ctypes.c_float, _i, _i, _vp, ctypes.c_size_t, _vp]
+    L.tkm_attn_chunk.restype = _i
     _lib = L
     return L
 
@@ -93,7 +129,7 @@ def lib() -> ctypes.CDLL:
 # Bits of tkm_attn_last_kernels (include/tkm_attn.h)
 KERNEL_BITS = {"fwd_asm": 1, "fwd_hip": 2, "dq_asm": 4, "dq_hip": 8, "dkdv_asm": 16,
                "dkdv_hip": 32, "delta_hip": 64, "decode": 128, "join": 256, "weights": 512, "append": 1024,
-               "evict": 2048}
+               "evict": 2048, "rope": 4096, "plan": 8192, "chunk": 16384}
 
 
 def init() -> None:
@@ -402,6 +438,276 @@ def _kv_evict(cache, budget, sink, recent, dst, kept, st):
     return kept
 
 
+class Rope:
+    """Rotary positions (tkm_attn_rope, include/tkm_attn.h): the first `rot` dims of a head turn, pair i by freqs[i]
+    radians a position.
+
+    layout   "halves" (dims i and i + rot/2) or "pairs" (2i and 2i + 1)
+    scaling  None, or "linear", "ntk", "bands", "yarn": for contexts `scale` times longer than the `original` ones of
+             training; low and high: turns over the original context (bands 1 and 4, yarn 1 and 32 if not given)
+    factor   of the rotated dims; None: the scaling's own
+    freqs    rot/2 frequencies in place of theta and scaling"""
+
+    LAYOUTS = {"halves": 0, "pairs": 1}
+    SCALINGS = {None: 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
+
+    def __init__(self, rot, theta=10000.0, layout="halves", scaling=None, scale=1.0, original=8192.0, low=None, high=None,
+                 factor=None, freqs=None):
+        if layout not in self.LAYOUTS:
+            raise ValueError(f"layout must be one of {list(self.LAYOUTS)}, got {layout!r}")
+        if scaling not in self.SCALINGS:
+            raise ValueError(f"scaling must be one of {list(self.SCALINGS)}, got {scaling!r}")
+        self._c = _Rope()
+        self._ref = ctypes.byref(self._c)
+        if freqs is not None:
+            if scaling is not None:
+                raise ValueError("freqs are taken as they are: scale them, and leave scaling out")
+            freqs = [float(f) for f in freqs]
+            if 2 * len(freqs) != rot:
+                raise ValueError(f"{len(freqs)} frequencies for {rot} rotated dims")
+            _check("tkm_attn_rope_from_freqs", lib().tkm_attn_rope_from_freqs(
+                (ctypes.c_double * len(freqs))(*freqs), rot, self.LAYOUTS[layout], factor or 0.0, self._ref))
+        else:
+            p = _RopeParams(rot, self.LAYOUTS[layout], self.SCALINGS[scaling], theta, scale, original, 1.0 if low is None else low,
+                            (32.0 if scaling == "yarn" else 4.0) if high is None else high, factor or 0.0)
+            _check("tkm_attn_rope_init", lib().tkm_attn_rope_init(ctypes.byref(p), self._ref))
+
+    @classmethod
+    def of_prep(cls, desc):
+        """The rotation of a qkv-prep descriptor (prep.Desc with RoPE): its frequencies, pairs over the whole head."""
+        from . import prep
+        r = cls.__new__(cls)
+        r._c = _Rope()
+        r._ref = ctypes.byref(r._c)
+        _check("tkm_prep_rope", prep.lib().tkm_prep_rope(ctypes.byref(desc), r._ref))
+        return r
+
+    rot = property(lambda self: self._c.rot)
+    factor = property(lambda self: self._c.factor)
+
+    def freqs(self):
+        """The frequencies as they are held, modulo a whole turn a position: floats in [0, 2 pi)."""
+        return [t * (2.0 * math.pi / 2.0 ** 64) for t in self._c.turns[:self._c.rot // 2]]
+
+
+def rope_fwd(x, rope, Hq, Hkv, D, pos=None, S=None, out=None, stream=None):
+    """Rotates the Q and K heads of packed rows x [..., (Hq+2Hkv)*D] (rows any multiple of 8 elements apart in a 2-D
+    x) to the positions pos [rows] int32, or, if these are None, to r % S of the row r; V is copied.  A row of a
+    negative position stays as it is in out.  out: a new tensor, or a given one; x itself: in place."""
+    return _rope_on(x, rope, Hq, Hkv, D, pos, S, out, 0, stream)
+
+
+def rope_bwd(dout, rope, Hq, Hkv, D, pos=None, S=None, dx=None, stream=None):
+    """The gradient of rope_fwd's x from that of its output: the rotation the other way."""
+    return _rope_on(dout, rope, Hq, Hkv, D, pos, S, dx, 1, stream)
+
+
+def _rope_on(x, rope, Hq, Hkv, D, pos, S, out, inverse, stream):
+    st = _current(x.device, stream) if x.is_cuda else None
+    if st is None:
+        if not x.is_cuda:
+            raise ValueError("the rows must be on a GPU")
+        with _On(x.device, stream) as st:
+            return _rope(x, rope, Hq, Hkv, D, pos, S, out, inverse, st)
+    return _rope(x, rope, Hq, Hkv, D, pos, S, out, inverse, st)
+
+
+def _rows_of(name, t, width, device, dtype, least=False):
+    """(rows, stride in elements) of a tensor of rows: 2-D with contiguous rows, or contiguous."""
+    if t.device != device or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} on {device}")
+    shape = t.shape
+    if len(shape) == 0 or (shape[-1] < width if least else shape[-1] != width):
+        raise ValueError(f"{name} must have rows of {'at least ' if least else ''}{width} elements")
+    n = t.numel() // shape[-1] if shape[-1] else 0
+    if len(shape) == 2:
+        if t.stride(1) != 1 and shape[1] > 1:
+            raise ValueError(f"{name} must have contiguous rows")
+        return n, t.stride(0) if n > 1 else (shape[1] + 7) // 8 * 8
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, or of two dimensions")
+    return n, shape[-1]
+
+
+def _rope(x, rope, Hq, Hkv, D, pos, S, out, inverse, st):
+    dt, dev, width = _dtype_code(x), x.device, (Hq + 2 * Hkv) * D
+    rows, stride = _rows_of("x", x, width, dev, x.dtype)
+    if pos is None:
+        if S is None:
+            raise ValueError("rows need positions, or the S rows of a sequence")
+    else:
+        _check_dtype("pos", pos, rows, dev, "int32")
+    if out is None:
+        out = x.new_empty(x.shape)
+    n, ostride = _rows_of("out", out, width, dev, x.dtype)
+    if n != rows:
+        raise ValueError(f"out has {n} rows, expected {rows}")
+    _check("tkm_attn_rope_rows", lib().tkm_attn_rope_rows(rope._ref, x.data_ptr(), stride, out.data_ptr(), ostride, _ptr(pos),
+                                                          1 if S is None else S, rows, Hq, Hkv, D, dt, inverse, st))
+    return out
+
+
+class KvPages:
+    """The pages of a pool that no sequence has, and how many each sequence has (tkm_attn_pages): free [num_pages]
+    int32, of which the first n_free [1] int32 are free, and held [B] int32.  The tensors stay the caller's."""
+
+    def __init__(self, free, n_free, held):
+        dev = held.device
+        _check_dtype("free", free, free.numel(), dev, "int32")
+        _check_dtype("n_free", n_free, 1, dev, "int32")
+        _check_dtype("held", held, held.numel(), dev, "int32")
+        self.free, self.n_free, self.held, self.device = free, n_free, held, dev
+        self._c = _Pages(_ptr(free), _ptr(n_free), _ptr(held))
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def all_free(cls, cache):
+        """Of a cache whose sequences have no pages yet: page 0 is taken first."""
+        import torch
+        dev, n = cache.device, cache.num_pages
+        return cls(torch.arange(n - 1, -1, -1, dtype=torch.int32, device=dev), torch.full((1,), n, dtype=torch.int32, device=dev),
+                   torch.zeros(cache.B, dtype=torch.int32, device=dev))
+
+
+class KvPlan:
+    """What a step does (tkm_attn_plan), written by kv_plan: n_new [B], row_start [B + 1], and per packed row seq, pos
+    [rows], all int32, and slot [rows] int64."""
+
+    def __init__(self, n_new, row_start, seq, pos, slot):
+        dev, B, rows = n_new.device, n_new.numel(), slot.numel()
+        _check_dtype("n_new", n_new, B, dev, "int32")
+        _check_dtype("row_start", row_start, B + 1, dev, "int32")
+        _check_dtype("seq", seq, rows, dev, "int32")
+        _check_dtype("pos", pos, rows, dev, "int32")
+        _check_dtype("slot", slot, rows, dev, "int64")
+        self.n_new, self.row_start, self.seq, self.pos, self.slot = n_new, row_start, seq, pos, slot
+        self.B, self.rows, self.device = B, rows, dev
+        self._c = _Plan(_ptr(n_new), _ptr(row_start), _ptr(seq), _ptr(pos), _ptr(slot))
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, B, rows, device="cuda"):
+        import torch
+        i32 = [torch.empty(n, dtype=torch.int32, device=device) for n in (B, B + 1, rows, rows)]
+        return cls(*i32, torch.empty(rows, dtype=torch.int64, device=device))
+
+
+def kv_plan(cache, pages, want, rows=None, start=None, plan=None, stream=None):
+    """Makes room for want [B] int32 more tokens of each sequence behind start [B] int32 (None: kv_len itself), takes
+    pages from the pool and gives back what sequences no longer need, advances kv_len, and lays out the step's packed
+    rows, at most `rows` of them (or as many as the given plan has).  A sequence whose pages or rows are not there gets
+    none: its plan.n_new is 0.  include/tkm_attn.h has the rules.  Returns the plan."""
+    st = _current(cache.device, stream)
+    if st is None:
+        with _On(cache.device, stream) as st:
+            return _kv_plan(cache, pages, want, rows, start, plan, st)
+    return _kv_plan(cache, pages, want, rows, start, plan, st)
+
+
+def _kv_plan(cache, pages, want, rows, start, plan, st):
+    dev, B = cache.device, cache.B
+    if plan is None:
+        if rows is None or rows < 0:
+            raise ValueError("a plan of how many rows?")
+        plan = KvPlan.empty(B, rows, dev)
+    elif rows is not None and rows != plan.rows:
+        raise ValueError(f"the plan has {plan.rows} rows, not {rows}")
+    if pages.device != dev or plan.device != dev:
+        raise ValueError(f"pages and plan must be on {dev}")
+    if pages.held.numel() != B or plan.B != B or pages.free.numel() != cache.num_pages:
+        raise ValueError(f"pages and plan must be of {B} sequences and {cache.num_pages} pages")
+    _check_tensor("want", want, B, dev, cache.kv_len.dtype)
+    if start is not None:
+        _check_tensor("start", start, B, dev, cache.kv_len.dtype)
+    _check("tkm_attn_kv_plan", lib().tkm_attn_kv_plan(cache._ref, pages._ref, want.data_ptr(), _ptr(start), plan._ref, plan.rows, st))
+    return plan
+
+
+def kv_append_rows(qkv, cache, Hq, plan, rope=None, q=None, stream=None):
+    """Stores the K and V heads of a plan's packed rows qkv [rows, (Hq+2Hkv)*D] in their slots of the cache, K rotated
+    to its position if there is a rope, and returns the Q heads [rows, >= Hq*D], rotated too: a new tensor, or the
+    given q (qkv itself: in place; without a rope and q they stay where they are).  kv_len is the plan's business."""
+    st = _current(cache.device, stream)
+    if st is None:
+        with _On(cache.device, stream) as st:
+            return _kv_append_rows(qkv, cache, Hq, plan, rope, q, st)
+    return _kv_append_rows(qkv, cache, Hq, plan, rope, q, st)
+
+
+def _kv_append_rows(qkv, cache, Hq, plan, rope, q, st):
+    dev, D = cache.device, cache.D
+    rows, stride = _rows_of("qkv", qkv, (Hq + 2 * cache.Hkv) * D, dev, cache.dtype)
+    if plan.device != dev or plan.rows != rows:
+        raise ValueError(f"the plan must be of {rows} rows, on {dev}")
+    if q is None:
+        q = qkv if rope is None else qkv.new_empty((rows, max(0, Hq * D)))
+    n, q_stride = _rows_of("q", q, Hq * D, dev, cache.dtype, least=True)
+    if n != rows:
+        raise ValueError(f"q has {n} rows, expected {rows}")
+    _check("tkm_attn_kv_append_rows", lib().tkm_attn_kv_append_rows(
+        cache._ref, None if rope is None else rope._ref, qkv.data_ptr(), stride, q.data_ptr(), q_stride, plan._ref, rows, Hq, st))
+    return q
+
+
+def chunk_workspace_bytes(cache, rows, Hq) -> int:
+    key = ("chunk", rows, Hq)
+    if key not in cache._ws:
+        if len(cache._ws) > 256:
+            cache._ws.clear()
+        cache._ws[key] = int(lib().tkm_attn_chunk_workspace_bytes(cache._ref, rows, Hq))
+    return cache._ws[key]
+
+
+def gqa_chunk(q, cache, Hq, row_start=None, n_new=None, scale=None, causal=True, window=0, out=None, lse=None, workspace=None,
+              stream=None):
+    """O [rows, Hq*D] and LSE [rows, Hq] (fp32) of each sequence's new rows over its cached positions, their own
+    among them (append first).  q: [rows, >= Hq*D] with the Q heads first.  Sequence b has n_new[b] int32 rows from
+    row_start[b] int32 on (a plan's; row_start None: from b * (rows / B), n_new None: rows / B), and the last of them
+    stands at its last position.  causal: a row sees the positions up to its own, with a window only the last `window`
+    of these.  Rows of no sequence stay as they are in out and lse.
+    workspace: chunk_workspace_bytes(cache, rows, Hq) bytes, allocated for the call if not given."""
+    st = _current(cache.device, stream)
+    if st is None:
+        with _On(cache.device, stream) as st:
+            return _gqa_chunk(q, cache, Hq, row_start, n_new, scale, causal, window, out, lse, workspace, st)
+    return _gqa_chunk(q, cache, Hq, row_start, n_new, scale, causal, window, out, lse, workspace, st)
+
+
+def _gqa_chunk(q, cache, Hq, row_start, n_new, scale, causal, window, out, lse, workspace, st):
+    import torch
+    D, dev, B = cache.D, cache.device, cache.B
+    if len(q.shape) != 2:
+        raise ValueError(f"q must be [rows, at least {Hq * D}]")
+    rows, stride = _rows_of("q", q, Hq * D, dev, cache.dtype, least=True)
+    i32 = cache.kv_len.dtype
+    if row_start is not None and not B <= row_start.numel() <= B + 1:
+        raise ValueError(f"row_start must have {B} entries, or {B + 1}")
+    if row_start is not None:
+        _check_tensor("row_start", row_start, row_start.numel(), dev, i32)
+    if n_new is not None:
+        _check_tensor("n_new", n_new, B, dev, i32)
+    if out is None:
+        out = q.new_empty((rows, max(0, Hq * D)))
+    else:
+        _check_tensor("out", out, rows * Hq * D, dev, q.dtype)
+    if lse is None:
+        lse = torch.empty((rows, max(0, Hq)), dtype=torch.float32, device=dev)
+    else:
+        _check_tensor("lse", lse, rows * Hq, dev, torch.float32)
+    if workspace is None:
+        wbytes = chunk_workspace_bytes(cache, rows, Hq)
+        if wbytes:
+            workspace = torch.empty(wbytes, dtype=torch.uint8, device=dev)
+    else:
+        _check_tensor("workspace", workspace, workspace.numel(), dev)
+        wbytes = workspace.numel() * workspace.element_size()
+    rc = lib().tkm_attn_chunk(cache._ref, q.data_ptr(), stride, _ptr(row_start), _ptr(n_new), rows, out.data_ptr(), lse.data_ptr(), Hq,
+                              default_scale(D) if scale is None else scale, 1 if causal else 0, window, _ptr(workspace), wbytes, st)
+    if rc:
+        _check("tkm_attn_chunk", rc)
+    return out, lse
+
+
 def attention_flops(B, S, Hq, D, causal, kv_len=None, mode="fwd") -> float:
     """Algorithmic FLOPs (FlashAttention convention): 4*B*Hq*S*Skv*D, halved if causal,
     x2.5 for the backward, x3.5 for forward+backward; with kv_len, S*Skv -> S*mean(kv_len)."""
@@ -410,6 +716,7 @@ def attention_flops(B, S, Hq, D, causal, kv_len=None, mode="fwd") -> float:
     return {"fwd": f, "bwd": 2.5 * f, "fwdbwd": 3.5 * f}[mode]
 
 
-__all__ = ["gqa_fwd", "gqa_bwd", "KvCache", "kv_append", "gqa_decode", "kv_evict", "decode_workspace_bytes", "init", "asm_available", "last_kernels", "KERNEL_BITS", "bwd_workspace_bytes", "attention_flops", "default_scale",
+__all__ = ["gqa_fwd", "gqa_bwd", "KvCache", "kv_append", "gqa_decode", "kv_evict", "decode_workspace_bytes", "Rope", "rope_fwd", "rope_bwd", "KvPages", "KvPlan", "kv_plan", "kv_append_rows",
+           "gqa_chunk", "chunk_workspace_bytes", "init", "asm_available", "last_kernels", "KERNEL_BITS", "bwd_workspace_bytes", "attention_flops", "default_scale",
            "lib", "header_functions", "AttnError", "F16", "BF16", "BWD_DELTA", "BWD_DKDV",
            "BWD_DQ", "BWD_DQ_DELTA"]

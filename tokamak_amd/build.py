@@ -24,7 +24,7 @@ HIP_LIB_PATH = os.path.join(PKG, "libtkm_hip.so")
 RT_SOURCES = ["tkm_gemm.hip", "tkm_gemm_mfma.hip", "tkm_rt_kernels.hip", "tkm_sample.hip"]
 RT_C_SOURCES = ["tkm_codegen_hip.c", "tkm_hip.c"]
 SOURCES = ["attn_fwd.hip", "attn_asm.hip", "attn_bwd.hip", "tkm_attn_abi.hip", "attn_decode.hip", "attn_kv.hip",
-           "tkm_kv_abi.hip"]
+           "attn_plan.hip", "attn_rope.hip", "attn_chunk.hip", "tkm_kv_abi.hip"]
 # Hand-scheduled assembly kernels: (generator module, kernel symbol).  Each is generated,
 # assembled for gfx950 and embedded in the library as a code object (a C byte array).
 ASM_KERNELS = [("tokamak_amd.asmgen.attn_fwd", "tkm_fa_fwd_d128_f16"),
@@ -34,7 +34,7 @@ ASM_KERNELS = [("tokamak_amd.asmgen.attn_fwd", "tkm_fa_fwd_d128_f16"),
                ("tokamak_amd.asmgen.attn_dq", "tkm_fa_bwd_dq_d128_f16"),
                ("tokamak_amd.asmgen.attn_dq", "tkm_fa_bwd_dq_d128_bf16")]
 C_SOURCES = ["tkm_error.c", "tkm_prelude.c", "tkm_codegen_util.c", "tkm_prep_codegen.c", "tkm_rtc.c",
-             "tkm_plasma_codegen.c", "tkm_plasma_rt.c"]
+             "tkm_plasma_codegen.c", "tkm_plasma_rt.c", "tkm_rope.c"]
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = "gfx950"
 

@@ -1,0 +1,529 @@
+// attn_chunk.hip -- attention of several new tokens a sequence over a paged key-value cache (gfx950).
+//
+//   row i of sequence b stands at p = len[b] - n[b] + i and sees lo <= j < hi:  s_j = scale <q, k_j>
+//   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m);  lse = m + ln sum_j exp(s_j - m)
+//
+// A kv head's query heads share its keys, so that the rows of a tile are (token, query head of the kv head) pairs:
+// row r is token r / G, head r % G.  An item is (kv head, sequence, tile of 128 such rows), 32 rows a wave; it walks
+// the tiles of 64 tokens that any of its rows sees.  Keys and values move HBM -> LDS by DMA, double-buffered, in the
+// cache's own 32 x 32 blocks (attn_kv.h), 64-byte rows whose 16-byte chunks are stored at c ^ (row / 4 % 4): operand
+// reads of 16 rows then meet all banks once.  Per tile and wave:
+//   S^T = K Q^T        32 tokens x 32 rows an MFMA block; lane = row.  K's tokens are dealt to the block's rows with
+//                      bits 2 and 3 swapped, so that the 8 registers of a k-step are 8 consecutive tokens:
+//   P^T                stays in its registers, as the B operand of
+//   O^T += V^T P^T     whose A operand is 8 consecutive tokens of a dim, one 16-byte read of a V block.
+//
+// P = 2^(s - m + 8): m moves only when a lane's sum of a tile reaches fp16's largest value, and the 8 keep weights of
+// down to 2^-22 of the row's largest in fp16's normal range.  In fp16 P goes to the second product as one number (11
+// bits, as in the kernels of whole sequences), in bf16 as two (16 bits).
+//
+// Splitting: all items' tiles are numbered in one line, kv head after kv head, and every workgroup takes an equal
+// share, whatever the lengths are, which are read on the device: a first launch of one workgroup lists the items of a
+// kv head and their sums of tiles.  Items that no one workgroup has whole leave pieces in the workspace, which a third
+// launch joins in the order of the tokens: results do not depend on timing.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.h"
+#include "attn_kv.h"
+#include "attn_launch.h"
+#include "attn_scan.h"
+
+namespace tkm {
+namespace {
+
+constexpr int BM = 128;           // rows of an item
+constexpr int BN = 64;            // tokens of a tile
+constexpr int kWaves = 4;
+constexpr int kWorkers = 512;     // workgroups: two on each compute unit
+constexpr float kLift = 8.0f;
+constexpr float kSumMax = 65504.0f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+// An item of a kv head: tile t of sequence b's rows, and the tiles of tokens before it in the head's line.
+struct Item {
+    int b, t;
+    int64_t at;
+};
+struct Line {
+    int64_t total;     // tiles of tokens of a kv head
+    int64_t items;
+};
+
+struct C {   // kernel arguments
+    const uint16_t *k, *v;
+    const int32_t *table, *len;
+    const uint16_t* q;
+    const int32_t *row_start, *n_new;
+    uint16_t* o;
+    float* lse;
+    Line* line;
+    Item* items;       // and one behind the last
+    float* part;       // pieces: [slot][BM][D] unnormalised O, then [slot][BM] (m, l)
+    float2* part_ml;
+    long long q_stride;
+    int B, Hkv, G, num_pages, page_shift, max_pages, cap, rows, causal, window, workers;
+    float sl2;         // scale * log2(e)
+};
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// An element of an array that no kernel of the launch writes, at a wave-uniform index: a scalar load.
+__device__ __forceinline__ int fixed(const int32_t* p, long long i) {
+    return *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p + i);
+}
+__device__ __forceinline__ int64_t fixed64(const int64_t* p) {
+    return *(const __attribute__((address_space(4))) int64_t*)(uintptr_t)p;
+}
+__device__ __forceinline__ Item fixed_item(const Item* p) {
+    Item e;
+    const auto* q = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+    e.b = q[0];
+    e.t = q[1];
+    e.at = fixed64(&p->at);
+    return e;
+}
+
+// A sequence's rows: `n` of them from row `row0` on, the first at position `pos`; len -1 if it lies outside the table.
+struct Seq {
+    int n, row0, pos, len;
+};
+__device__ __forceinline__ Seq seq_of(const C& a, int b) {
+    Seq s;
+    const int each = a.rows / a.B;
+    s.row0 = a.row_start ? a.row_start[b] : b * each;
+    const int n = a.n_new ? a.n_new[b] : each;
+    s.len = a.len[b];
+    if ((unsigned)s.len > (unsigned)a.cap) s.len = -1;
+    s.n = s.row0 < 0 || s.row0 >= a.rows ? 0 : max(0, min(n, a.rows - s.row0));
+    s.pos = s.len - max(n, 0);       // above -2^31: neither is below -1, nor n above 2^31 - 1
+    return s;
+}
+// The positions that the row of token i sees: [lo, hi).
+__device__ __forceinline__ int2 seen_by(const C& a, const Seq& s, int i) {
+    if (!a.causal) return int2{0, max(s.len, 0)};
+    const int p = s.pos + i;
+    return int2{a.window ? max(0, p - a.window + 1) : 0, max(0, min(p + 1, s.len))};
+}
+// The tiles [x, y) of tokens that rows [first, last] see.
+__device__ __forceinline__ int2 tiles_of(const C& a, const Seq& s, int first, int last) {
+    const int lo = seen_by(a, s, first / a.G).x, hi = seen_by(a, s, last / a.G).y;
+    return lo < hi ? int2{lo / BN, (hi + BN - 1) / BN} : int2{0, 0};
+}
+
+constexpr int TL = 1024;
+
+// Lists the items of a kv head, sequence after sequence, and their places in its line.  One workgroup.
+__global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
+    __shared__ Scan<TL> lds;
+    int64_t before = 0, items = 0;
+    for (int c = 0; c < a.B; c += TL) {
+        const int b = c + threadIdx.x;
+        const int rows = b < a.B ? seq_of(a, b).n * a.G : 0;
+        int64_t all, sum;
+        lds.end[threadIdx.x] = (int)lds.sum(0, (rows + BM - 1) / BM, all);
+        __syncthreads();
+        for (int64_t k0 = 0; k0 < all; k0 += TL) {
+            const int k = (int)k0 + threadIdx.x;
+            Item e{0, 0, 0};
+            int tiles = 0;
+            if (k < all) {
+                const int i = first_above(lds.end, TL, k);
+                e.b = c + i;
+                e.t = k - (i ? lds.end[i - 1] : 0);
+                const Seq q = seq_of(a, e.b);
+                const int2 x = tiles_of(a, q, e.t * BM, min((e.t + 1) * BM, q.n * a.G) - 1);
+                tiles = max(1, x.y - x.x);       // an item that sees nothing still has outputs
+            }
+            e.at = before + lds.sum(1, tiles, sum) - tiles;
+            if (k < all) a.items[items + k] = e;
+            before += sum;
+            __syncthreads();
+        }
+        items += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        a.items[items] = Item{0, 0, before};
+        *a.line = Line{before, items};
+    }
+}
+
+// The item that holds place `at` of a head's line.
+__device__ __forceinline__ int item_at(const C& a, int items, int64_t at) {
+    int lo = 0, hi = items - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (fixed64(&a.items[mid + 1].at) > at) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+__device__ __forceinline__ int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
+
+// Row r of an item: its row of o and lse, and its head.
+__device__ __forceinline__ long long out_row(const C& a, const Seq& s, int h, int r) {
+    return ((long long)(s.row0 + r / a.G) * a.Hkv + h) * a.G + r % a.G;
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_kernel(C a) {
+    constexpr bool SPL = Split<DT>::on;
+    constexpr int KS = D / 16, NDB = D / 32, PKS = BN / 16;
+    constexpr int HALF = D * 64;               // bytes of 32 tokens of K or V
+    constexpr int TILE = 2 * HALF;
+    constexpr int NI = TILE / 1024 / kWaves;   // DMA requests of a wave, a tile of K or V
+    constexpr int NL = SPL ? PKS : 1;
+    __shared__ __attribute__((aligned(1024))) char smem[2][2][TILE];    // [K, V][buffer]
+
+    const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l32 = lane & 31, hi = lane >> 5;
+    const int items = (int)fixed64(&a.line->items);
+    if (!items) return;
+    const int64_t total = fixed64(&a.line->total), all = total * a.Hkv, each = div_up(all, a.workers);
+    // consecutive shares on one XCD, whose L2 their keys and values then share
+    const int place = a.workers % 8 ? blockIdx.x : (int)(blockIdx.x % 8 * (a.workers / 8) + blockIdx.x / 8);
+    int64_t at = place * each;
+    const int64_t last = min(at + each, all);
+    if (at >= last) return;
+    int h = (int)(at / total), e = item_at(a, items, at - h * total);
+
+    const uint32_t lds0 = lds_addr(smem);
+    // DMA: this wave's requests of a tile are 1024 bytes each, all of one half of 32 tokens
+    const int my_half = wave / (kWaves / 2);
+    uint32_t dma_v[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int c = ((wave % (kWaves / 2)) * NI + i) * 64 + lane;      // chunk of the half
+        dma_v[i] = (uint32_t)(c / 4 * 64 + (((c % 4) ^ (c / 16 % 4)) << 4));
+    }
+    const uint32_t dma_at = lds0 + (uint32_t)(wave * NI * 1024);
+    // operand reads: chunks (ks % 2) * 2 + hi of a 64-byte row
+    const int tok = (l32 & 19) | (l32 & 4) << 1 | (l32 & 8) >> 1;        // bits 2 and 3 swapped
+    int koff[2], voff[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        koff[j] = tok * 64 + (((j * 2 + hi) ^ (tok / 4 % 4)) << 4);
+        voff[j] = l32 * 64 + (((j * 2 + hi) ^ (l32 / 4 % 4)) << 4);
+    }
+
+    while (at < last) {
+        // ---- the item, and this workgroup's share of its tiles
+        const Item it = fixed_item(&a.items[e]);
+        const int64_t start = h * total + it.at, end = h * total + fixed64(&a.items[e + 1].at);
+        Seq s;
+        {
+            const int each_rows = a.rows / a.B;
+            s.row0 = a.row_start ? fixed(a.row_start, it.b) : it.b * each_rows;
+            const int n = a.n_new ? fixed(a.n_new, it.b) : each_rows;
+            s.len = fixed(a.len, it.b);
+            if ((unsigned)s.len > (unsigned)a.cap) s.len = -1;
+            s.n = s.row0 < 0 || s.row0 >= a.rows ? 0 : max(0, min(n, a.rows - s.row0));
+            s.pos = s.len - max(n, 0);
+        }
+        const int R = s.n * a.G, r0 = it.t * BM;
+        const int2 tiles = tiles_of(a, s, r0, min(r0 + BM, R) - 1);
+        const int ta = tiles.x + (int)(at - start), te = min(tiles.x + (int)(min(end, last) - start), tiles.y);
+        const bool whole = at == start && end <= last;
+
+        // this lane's row; those behind the sequence's rows act as its last
+        const int r = r0 + wave * 32 + l32;
+        const bool valid = r < R;
+        const int first = r0 + wave * 32, final = min(first + 31, R - 1);
+        const bool active = first < R;
+        const int2 seen = seen_by(a, s, min(r, max(R - 1, 0)) / a.G);
+        // tiles in [p0, p1) need no mask in this wave, those in [n0, n1) hold a token that one of its rows sees
+        int p0 = 0, p1 = 0, n0 = 0, n1 = 0;
+        if (active) {
+            const int2 x = seen_by(a, s, first / a.G), y = seen_by(a, s, final / a.G);
+            p0 = (y.x + BN - 1) / BN;
+            p1 = x.y / BN;
+            n0 = x.x / BN;
+            n1 = (y.y + BN - 1) / BN;
+        }
+        u32x4 qf[KS];
+        {
+            const uint16_t* qp = a.q + (s.row0 + r / a.G) * a.q_stride + (long long)(h * a.G + r % a.G) * D + hi * 8;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qf[ks] = valid ? ld_global16(qp + ks * 16) : u32x4{0u, 0u, 0u, 0u};
+        }
+        f32x16 o[NDB];
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[db] = f32x16{};
+        float m = -INFINITY, lsum = 0.f;     // m less the lift, log2 units
+        bool bad = s.len < 0;
+
+        // pages of a tile's halves, fetched a tile ahead
+        const int half_bits = a.page_shift - 5;
+        auto page_of = [&](int t, int x) {
+            const int p = (t * 2 + x) >> half_bits;
+            return fixed(a.table, (long long)it.b * a.max_pages + min(p, a.max_pages - 1));
+        };
+        int pg[2];
+        auto fetch = [&](int t) {
+            pg[0] = page_of(t, 0);
+            pg[1] = page_of(t, 1);
+        };
+        auto issue = [&](int t, int buf) __attribute__((always_inline)) {
+            int page[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                page[x] = pg[x];
+                const int from = t * BN + x * 32;
+                if ((unsigned)page[x] >= (unsigned)a.num_pages) {      // page 0 in its place; rows that see it become NaN
+                    page[x] = 0;
+                    bad |= from < seen.y && from + 32 > seen.x;
+                }
+            }
+            if (t * BN + my_half * 32 < s.len) {
+                const int half = t * 2 + my_half;
+                const long long sub = (((long long)(my_half ? page[1] : page[0]) * a.Hkv + h) << half_bits) + (half & ((1 << half_bits) - 1));
+                dma16_rows(make_rsrc((const char*)a.k + sub * HALF, HALF), dma_at + (uint32_t)(buf * TILE), dma_v);
+                dma16_rows(make_rsrc((const char*)a.v + sub * HALF, HALF), dma_at + (uint32_t)((2 + buf) * TILE), dma_v);
+            }
+        };
+        // values of tokens behind the sequence's last become 0: what is there may be anything
+        auto clear_tail = [&](int t, int buf) {
+            const int left = s.len - t * BN;
+            if (left >= BN) return;
+            for (int i = threadIdx.x; i < TILE / 64; i += 64 * kWaves) {     // rows of 32 tokens of one dim
+                char* row = smem[1][buf] + i * 64;
+                const int from = i * 64 >= HALF ? 32 : 0;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    u32x4* p = (u32x4*)(row + ((c ^ (i / 4 % 4)) << 4));
+                    u32x4 x = *p;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int j = from + c * 8 + 2 * w;
+                        x[w] &= (j < left ? 0xffffu : 0u) | (j + 1 < left ? 0xffff0000u : 0u);
+                    }
+                    *p = x;
+                }
+            }
+            __syncthreads();
+        };
+
+        f32x16 sr[2];
+        auto scores = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const u32x4 x = ld_lds16((const uint16_t*)(smem[0][buf] + kb * HALF + ks / 2 * 2048 + koff[ks & 1]));
+                    sr[kb] = mfma32<DT>(x, qf[ks], ks == 0 ? f32x16{} : sr[kb]);
+                }
+        };
+        // register x of block kb is token kb * 32 + x / 8 * 16 + hi * 8 + x % 8
+        auto mask = [&](int t) __attribute__((always_inline)) {
+            const int up = seen.y - t * BN - hi * 8, down = seen.x - t * BN - hi * 8;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const int j = kb * 32 + (x >> 3) * 16 + (x & 7);
+                    if (j >= up || j < down) sr[kb][x] = -INFINITY;
+                }
+        };
+        u32x4 pr[PKS], plr[NL];
+        auto expo = [&](float ref) __attribute__((always_inline)) {
+            float sum = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < PKS; ++ks)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int x = (ks & 1) * 8 + 2 * w;
+                    const float p0 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x], a.sl2, -ref));
+                    const float p1 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x + 1], a.sl2, -ref));
+                    if constexpr (SPL) {
+                        const u32x2 hl = pack_split_bf16(p0, p1);
+                        pr[ks][w] = hl[0];
+                        plr[ks][w] = hl[1];
+                    } else {
+                        pr[ks][w] = pack2<DT>(p0, p1);
+                    }
+                    sum += p0 + p1;
+                }
+            return sum;
+        };
+        auto tile = [&](int t, int buf) __attribute__((always_inline)) {
+            scores(buf);
+            if (t < p0 || t >= p1) mask(t);
+            float sum = expo(m);
+            if (__builtin_expect(__any(!(sum < kSumMax)), 0)) {        // also where m is not set yet
+                float v = sr[0][0];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int x = kb ? 0 : 1; x < 16; ++x) v = fmaxf(v, sr[kb][x]);
+                const float mn = fmaxf(m, half_max(v) * a.sl2 - kLift);
+                const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);      // nothing is there to be scaled if m is not set
+                lsum *= f;
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) o[db] *= f;
+                m = mn;
+                sum = expo(m == -INFINITY ? 0.f : m);
+            }
+            lsum += sum;
+#pragma unroll
+            for (int ks = 0; ks < PKS; ++ks)
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) {
+                    const u32x4 x = ld_lds16((const uint16_t*)(smem[1][buf] + ks / 2 * HALF + db * 2048 + voff[ks & 1]));
+                    o[db] = mfma32<DT>(x, pr[ks], o[db]);
+                    if constexpr (SPL) o[db] = mfma32<DT>(x, plr[ks], o[db]);
+                }
+        };
+
+        // ---- the walk: tile t + 1 comes while t is worked on
+        if (ta < te) {
+            fetch(ta);
+            issue(ta, 0);
+            if (ta + 1 < te) fetch(ta + 1);
+        }
+        wait_dma();
+        __syncthreads();
+        auto step = [&](int t, auto Buf) __attribute__((always_inline)) {
+            constexpr int buf = decltype(Buf)::value;
+            clear_tail(t, buf);
+            if (t + 1 < te) {
+                issue(t + 1, buf ^ 1);
+                if (t + 2 < te) fetch(t + 2);
+            }
+            if (t >= n0 && t < n1) tile(t, buf);
+            wait_dma();
+            __syncthreads();
+        };
+        for (int t = ta; t < te; t += 2) {
+            step(t, std::integral_constant<int, 0>{});
+            if (t + 1 < te) step(t + 1, std::integral_constant<int, 1>{});
+        }
+
+        // ---- out
+        float l = half_sum(lsum);
+        if (bad) l = NAN;
+        if (whole) {
+            if (valid) {
+                const long long row = out_row(a, s, h, r);
+                const float inv = l == 0.f ? 0.f : 1.0f / l;
+                uint16_t* orow = a.o + row * D;
+#pragma unroll
+                for (int db = 0; db < NDB; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const u32x2 w = {pack2<DT>(o[db][g * 4] * inv, o[db][g * 4 + 1] * inv), pack2<DT>(o[db][g * 4 + 2] * inv, o[db][g * 4 + 3] * inv)};
+                        *(u32x2*)(orow + db * 32 + g * 8 + hi * 4) = w;
+                    }
+                if (a.lse && hi == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
+            }
+        } else if (valid) {
+            const long long slot = (long long)place * 2 + (at == start ? 1 : 0);
+            float* p = a.part + (slot * BM + (r - r0)) * D;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *(f32x4*)(p + db * 32 + g * 8 + hi * 4) = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
+            if (hi == 0) a.part_ml[slot * BM + (r - r0)] = float2{m, l};
+        }
+        at = min(end, last);
+        if (++e == items) {
+            e = 0;
+            ++h;
+        }
+    }
+}
+
+// Joins the pieces of the items that several workgroups shared: a workgroup has 1024 / D rows of the item in which
+// worker blockIdx.x's share begins, if that is the first to begin in it.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void chunk_join_kernel(C a) {
+    constexpr int LANES = D / 4, ROWS = 256 / LANES;
+    const int items = (int)fixed64(&a.line->items), w = blockIdx.x + 1;
+    if (!items) return;
+    const int64_t total = fixed64(&a.line->total), all = total * a.Hkv, each = div_up(all, a.workers), at = w * each;
+    if (at >= all) return;
+    const int h = (int)(at / total), e = item_at(a, items, at - h * total);
+    const Item it = fixed_item(&a.items[e]);
+    const int64_t start = h * total + it.at, end = h * total + fixed64(&a.items[e + 1].at);
+    if (start == at || start / each + 1 != w) return;
+    const Seq s = seq_of(a, it.b);
+    const int r = (int)blockIdx.y * ROWS + threadIdx.x / LANES, R = s.n * a.G - it.t * BM, d = threadIdx.x % LANES * 4;
+    if (r >= min(R, BM)) return;
+    const int n = (int)((end - 1) / each) - (w - 1) + 1;      // pieces: workers w - 1 ..
+    auto slot = [&](int i) { return ((long long)(w - 1 + i) * 2 + (i ? 0 : 1)) * BM + r; };
+    float m = -INFINITY;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, a.part_ml[slot(i)].x);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int i = 0; i < n; ++i) {
+        const float2 ml = a.part_ml[slot(i)];
+        const f32x4 x = *(const f32x4*)(a.part + slot(i) * D + d);
+        // a piece without a finite score has nothing but perhaps a NaN in its sum
+        const bool none = ml.x == -INFINITY;
+        const float f = none ? 0.f : fast_exp2(ml.x - m);
+        l += none ? ml.y : f * ml.y;
+        if (!none) o += f * x;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const long long row = out_row(a, s, h, it.t * BM + r);
+    *(u32x2*)(a.o + row * D + d) = u32x2{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+    if (a.lse && d == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
+}
+
+// The most items that a kv head can have, and workers that a call can use.
+long long items_most(const tkm_attn_kv& kv, int rows, int Hq) {
+    const long long G = Hq / kv.Hkv;
+    return (rows * G + BM - 1) / BM + std::min<long long>(kv.B, rows);
+}
+int workers_of(const tkm_attn_kv& kv, int rows, int Hq) {
+    const double tiles = (double)items_most(kv, rows, Hq) * kv.Hkv * (kv.max_pages * (double)kv.page / BN + 1);
+    return tiles < kWorkers ? (int)tiles : kWorkers;
+}
+size_t align_up(size_t n) { return (n + 255) & ~(size_t)255; }
+size_t items_bytes(const tkm_attn_kv& kv, int rows, int Hq) {
+    return align_up(sizeof(Line) + (size_t)(items_most(kv, rows, Hq) + 1) * sizeof(Item));
+}
+
+template <int D, int DT>
+int launch_t(const C& a, hipStream_t stream) {
+    hipLaunchKernelGGL(chunk_items_kernel, dim3(1), dim3(TL), 0, stream, a);
+    if (hipGetLastError() != hipSuccess) return -1;
+    hipLaunchKernelGGL((chunk_kernel<D, DT>), dim3(a.workers), dim3(64 * kWaves), 0, stream, a);
+    if (hipGetLastError() != hipSuccess) return -1;
+    if (a.workers > 1) {
+        hipLaunchKernelGGL((chunk_join_kernel<D, DT>), dim3(a.workers - 1, BM / (1024 / D)), dim3(256), 0, stream, a);
+        if (hipGetLastError() != hipSuccess) return -1;
+    }
+    return 0;
+}
+
+}  // namespace
+
+bool chunk_fits(const tkm_attn_kv& kv, int rows, int Hq) {
+    // the rows of a kv head, and a head's line, in the integers that hold them
+    return (double)rows * (Hq / kv.Hkv) <= 1073741824.0;
+}
+
+size_t chunk_workspace(const tkm_attn_kv& kv, int rows, int Hq) {
+    const size_t pieces = (size_t)workers_of(kv, rows, Hq) * 2 * BM;
+    return items_bytes(kv, rows, Hq) + pieces * (kv.D + 2) * sizeof(float);
+}
+
+int launch_chunk(const ChunkArgs& x) {
+    const tkm_attn_kv& kv = x.kv;
+    const int workers = workers_of(kv, x.rows, x.Hq);
+    char* ws = (char*)x.ws;
+    float* part = (float*)(ws + items_bytes(kv, x.rows, x.Hq));
+    const size_t pieces = (size_t)workers * 2 * BM;
+    const C a{(const uint16_t*)kv.k, (const uint16_t*)kv.v, kv.table, kv.len, (const uint16_t*)x.q, x.row_start, x.n_new,
+              (uint16_t*)x.o, x.lse, (Line*)ws, (Item*)(ws + sizeof(Line)), part, (float2*)(part + pieces * kv.D), x.q_stride,
+              kv.B, kv.Hkv, x.Hq / kv.Hkv, kv.num_pages, __builtin_ctz(kv.page), kv.max_pages, kv.max_pages * kv.page, x.rows,
+              x.causal, x.window, workers, x.scale * 1.4426950408889634f};
+    note_kernels(kChunk | (workers > 1 ? kJoin : 0));
+    const hipStream_t stream = (hipStream_t)x.stream;
+    if (kv.D == 128) return kv.dtype == DT_F16 ? launch_t<128, DT_F16>(a, stream) : launch_t<128, DT_BF16>(a, stream);
+    return kv.dtype == DT_F16 ? launch_t<64, DT_F16>(a, stream) : launch_t<64, DT_BF16>(a, stream);
+}
+
+}  // namespace tkm

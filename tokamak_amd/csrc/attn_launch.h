@@ -36,7 +36,8 @@ struct BwdArgs {
 // include/tkm_attn.h.
 enum KernelBit : unsigned {
     kFwdAsm = 1u, kFwdHip = 2u, kDqAsm = 4u, kDqHip = 8u, kDkdvAsm = 16u, kDkdvHip = 32u,
-    kDeltaHip = 64u, kDecode = 128u, kJoin = 256u, kWeights = 512u, kAppend = 1024u, kEvict = 2048u
+    kDeltaHip = 64u, kDecode = 128u, kJoin = 256u, kWeights = 512u, kAppend = 1024u, kEvict = 2048u,
+    kRope = 4096u, kPlan = 8192u, kChunk = 16384u
 };
 void note_kernels(unsigned bits);  // ORs bits into the calling thread's record
 void reset_kernels();              // clears it, at the start of a call

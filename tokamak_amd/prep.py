@@ -56,6 +56,8 @@ def lib() -> ctypes.CDLL:
     L.tkm_prep_create.restype = _i
     L.tkm_prep_destroy.argtypes = [_vp]
     L.tkm_prep_destroy.restype = None
+    L.tkm_prep_rope.argtypes = [ctypes.POINTER(Desc), _vp]
+    L.tkm_prep_rope.restype = _i
     L.tkm_prep_fwd.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]
     L.tkm_prep_fwd.restype = _i
     L.tkm_prep_bwd_workspace_bytes.argtypes = [_vp, _i]
