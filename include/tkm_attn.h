@@ -277,8 +277,8 @@ TKM_ATTN_API int tkm_attn_kv_append_rows(const tkm_attn_kv *kv, const tkm_attn_r
                                          long long stride, void *q, long long q_stride, const tkm_attn_plan *plan,
                                          int rows, int Hq, void *stream);
 
-/* Bytes of device workspace tkm_attn_chunk needs; 0 also if it refuses the arguments.  It holds nothing
- * from call to call; calls that may overlap need one each. */
+/* Bytes of device workspace tkm_attn_chunk needs; 0 if none (short tables, few rows), also if it refuses
+ * the arguments.  It holds nothing from call to call; calls that may overlap need one each. */
 TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int rows, int Hq);
 
 /* Attention of each sequence's new rows over its len[b] cached positions, their own among them: row i
@@ -288,8 +288,10 @@ TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int ro
  * [rows][Hq] or NULL.  Sequence b has the rows row_start[b] .. row_start[b] + n_new[b] - 1; row_start
  * NULL: from b * (rows / B) on, n_new NULL (only then): rows / B.  Rows outside [0, rows) are passed
  * over, other sequences' rows must not be among them; rows of no sequence stay as they are in o and lse.
- * A row that sees nothing gets O = 0, LSE = -inf; NaN, infinities, lengths and pages outside their
- * bounds act as in tkm_attn_decode, and what a row does not see has no part in it, whatever it holds.
+ * A row that sees nothing gets O = 0, LSE = -inf.  What a row does not see has no part in it, whatever
+ * it holds; what it sees of NaN and infinities makes its O of that dim (values) or all of it (scores)
+ * one of them.  Lengths and pages outside their bounds act as in tkm_attn_decode.  Values of more than
+ * 2^100 may overflow in the sums, which hold weights of up to 2^16.
  * Scores, softmax and sums are fp32.  Results do not depend on timing. */
 TKM_ATTN_API int tkm_attn_chunk(const tkm_attn_kv *kv, const void *q, long long q_stride, const int32_t *row_start,
                                 const int32_t *n_new, int rows, void *o, float *lse, int Hq, float scale, int causal,

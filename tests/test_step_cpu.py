@@ -111,9 +111,18 @@ def test_rope_refuses(kw, status, msg):
     (dict(rows=1 << 30, wsb=1 << 60), EUNSUPPORTED, b"too large"),
 ])
 def test_chunk_refuses(kw, status, msg):
-    assert call_chunk(kv(), **kw) == status
+    assert call_chunk(kv(max_pages=100), **kw) == status
     assert msg in attn.lib().tkm_attn_last_error()
     assert attn.lib().tkm_attn_last_kernels() == 0
+
+
+def test_chunk_workspace():
+    L = attn.lib()
+    small, large = kv(max_pages=4), kv(max_pages=1000)
+    assert L.tkm_attn_chunk_workspace_bytes(ref(small), 6, 4) == 0 < L.tkm_attn_chunk_workspace_bytes(ref(large), 6, 4)
+    assert L.tkm_attn_chunk_workspace_bytes(ref(large), 1 << 20, 4) <= 1024 * 2 * 128 * 66 * 4 + (1 << 20)      # its pieces, and lists
+    for kw, rows, Hq in ((dict(D=80), 6, 4), ({}, 6, 5), ({}, -1, 4)):
+        assert L.tkm_attn_chunk_workspace_bytes(ref(kv(max_pages=1000, **kw)), rows, Hq) == 0
 
 
 def test_nothing_to_do_launches_nothing():

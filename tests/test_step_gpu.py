@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from kv_cases import DT, HALF, TINY, Case, dense
-from step_cases import check_chunk, check_rounded, freqs_ref, plan_ref, rope_ref
+from step_cases import check_chunk, check_rounded, chunk_ref, freqs_ref, plan_ref, rope_ref, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -326,3 +326,97 @@ def test_chunk_of_steep_scores(gpu, Hq, Hkv, D, page, dtype, mul, trend, scale):
     q = queries(140, Hq, Hkv, D, dtype, gpu, mul=mul)
     o, lse = attn.gqa_chunk(q, case.cache, Hq, scale=scale)
     check_chunk(case, lens, n_new, q, o, lse, Hq, scale=scale)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype,extra", [(2, 2, 64, 32, "f16", 1), (8, 2, 128, 64, "bf16", 1), (8, 1, 64, 64, "bf16", 40),
+                                                       (2, 2, 128, 32, "bf16", 60), (12, 2, 128, 64, "f16", 40), (1, 1, 128, 128, "f16", 1)])
+@pytest.mark.parametrize("n", [40, 20])
+def test_chunk_of_odd_values(gpu, Hq, Hkv, D, page, dtype, extra, n):
+    """NaN and infinities among keys and values: rows that see one have one of them there, the others nothing of it, in
+    calls of one launch and of three (extra pages make the tables long)."""
+    from tokamak_amd import attn
+    print(f"[case] odd values Hq{Hq} Hkv{Hkv} D{D} {dtype} n{n}", flush=True)
+    L, G = 300, Hq // Hkv
+    case = Case(gpu, [L, 33], Hkv, D, page, dtype, extra_pages=extra)
+    odd = [(281, 3, math.inf), (285, 5, math.nan), (290, 7, -math.inf), (293, 7, math.inf), (10, 9, -math.inf), (299, 11, math.inf)]
+    v = case.v[0].clone()
+    for j, d, x in odd:
+        v[Hkv - 1, j, d] = x
+        at, tok = case.cache.table[0, j // page], j % page
+        case.cache.v[at, Hkv - 1, tok // 32, d // 32, d % 32, tok % 32] = x
+        case.v[0][Hkv - 1, j, d] = 0.0
+    at, tok = case.cache.table[0, 296 // page], 296 % page
+    case.cache.k[at, 0, tok // 32, 0, tok % 32, 4] = math.nan
+    case.k[0][0, 296] = 0.0
+    q = queries(n + 5, Hq, Hkv, D, dtype, gpu)
+    for window in (0, 100):
+        o, lse = attn.gqa_chunk(q, case.cache, Hq, i32([0, n], gpu), i32([n, 5], gpu), window=window)
+        got, pos = o.cpu().double().reshape(-1, Hq, D), [L - n + i for i in range(n)]
+        see = lambda i, j: j <= pos[i] and (window == 0 or j > pos[i] - window)
+        for i in range(n):
+            for h in range(Hq):
+                if h // G == 0 and see(i, 296):
+                    assert torch.isnan(got[i, h]).all() and math.isnan(lse[i, h].item())
+                    got[i, h] = 0.0
+                elif h // G == Hkv - 1:
+                    for d in (3, 5, 7, 9, 11):
+                        hit = [x for j, dd, x in odd if dd == d and see(i, j)]
+                        if hit:
+                            assert not math.isfinite(got[i, h, d]), (i, h, d)
+                            got[i, h, d] = 0.0
+        for b, (length, m, first) in enumerate(((L, n, 0), (33, 5, n))):
+            qq = q.cpu().double()[first:first + m, :Hq * D].reshape(m, Hq, D)
+            ro, rl, eo, el = chunk_ref(qq, case.k[b], case.v[b], visible(length, m, True, window), Hkv, 1 / math.sqrt(D), dtype)
+            g = got[first:first + m]
+            same = torch.ones_like(g, dtype=torch.bool)
+            if b == 0:         # what was compared above is 0 in g
+                for i in range(m):
+                    if see(i, 296):
+                        same[i, :G] = False
+                    for j, d, x in odd:
+                        if see(i, j):
+                            same[i, (Hkv - 1) * G:, d] = False
+            assert torch.isfinite(g).all()
+            tol = eo + HALF[dtype] * (ro.abs() + eo) + TINY[dtype]
+            assert ((g - ro).abs() <= tol)[same].all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [(2, 2, 64, 32, "f16"), (16, 2, 128, 64, "bf16")])
+@pytest.mark.parametrize("extra", [1, 60])
+def test_chunk_of_bad_pages_and_lengths(gpu, Hq, Hkv, D, page, dtype, extra):
+    """A page outside the pool makes NaN of the rows that see it, a length outside the table of all the sequence's;
+    the others are as they were."""
+    from tokamak_amd import attn
+    lens, n_new = [200, 200, 90, 70, 200], [30, 30, 40, 5, 30]
+    case = Case(gpu, lens, Hkv, D, page, dtype, extra_pages=extra)
+    c = case.cache
+    c.table[0, (200 - 15) // page] = c.num_pages          # the page of row 15
+    c.table[1, 0] = -1
+    c.kv_len[2] = c.max_pages * page + 1
+    c.kv_len[3] = -1
+    q = queries(sum(n_new), Hq, Hkv, D, dtype, gpu)
+    row_start = [sum(n_new[:b]) for b in range(6)]
+    o, lse = attn.gqa_chunk(q, c, Hq, i32(row_start, gpu), i32(n_new, gpu))
+    first = (200 - 15) // page * page                     # rows from this position on see the bad page
+    clean = max(0, first - 170)
+    assert torch.isnan(o[clean:30]).all() and torch.isnan(lse[clean:30]).all()
+    for b in (1, 2, 3):
+        assert torch.isnan(o[row_start[b]:row_start[b + 1]]).all() and torch.isnan(lse[row_start[b]:row_start[b + 1]]).all()
+    check_chunk(case, lens, n_new, q, o, lse, Hq, skip=(0, 1, 2, 3))
+    if clean:
+        k, v = case.k[0], case.v[0]
+        case.k[0], case.v[0] = k[:, :170 + clean], v[:, :170 + clean]
+        check_chunk(case, [170 + clean], [clean], q, o, lse, Hq)
+    o2, _ = attn.gqa_chunk(q, c, Hq, i32(row_start, gpu), i32(n_new, gpu), window=10)      # the first page is not seen any more
+    assert torch.isfinite(o2[row_start[1]:row_start[2]]).all()
+
+
+def test_chunk_of_rows_outside(gpu):
+    """Rows that a batch does not have are passed over."""
+    from tokamak_amd import attn
+    case = Case(gpu, [100, 100, 100, 100], 2, 64, 64, "f16")
+    q = queries(20, 4, 2, 64, "f16", gpu)
+    out = torch.full((20, 256), 4.0, dtype=torch.float16, device=gpu)
+    o, lse = attn.gqa_chunk(q, case.cache, 4, i32([-5, 3, 18, 20], gpu), i32([4, 5, 7, 3], gpu), out=out)
+    check_chunk(case, [100] * 4, [0, 5, 0, 0], q, o, lse, 4, row_start=[0, 3, 0, 0])
+    assert (out[:3] == 4.0).all() and (out[8:18] == 4.0).all() and torch.isfinite(out[18:]).all()

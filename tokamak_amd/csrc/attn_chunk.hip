@@ -19,12 +19,17 @@
 //
 // Splitting: all items' tiles are numbered in one line, kv head after kv head, and every workgroup takes an equal
 // share, whatever the lengths are, which are read on the device: a first launch of one workgroup lists the items of a
-// kv head and their sums of tiles.  Items that no one workgroup has whole leave pieces in the workspace, which a third
-// launch joins in the order of the tokens: results do not depend on timing.
+// kv head, the place where each share begins, and the items that no one workgroup has whole.  These leave pieces in
+// the workspace, which a third launch joins in the order of the tokens: results do not depend on timing.  Where the
+// tables hold few tokens a workgroup has an item, and there is one launch.
+//
+// 0 times an infinity or NaN is NaN, also where P is 0 because its row does not see the token.  So a tile that an item's
+// rows do not see alike is searched for such values in LDS; they become 0 there, and a bit each, by which they are
+// added to the sums of the rows that see them.  (In tiles that all rows see an infinity may become NaN, by a part of P
+// that is 0 or negative.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "attn_common.h"
 #include "attn_kv.h"
@@ -47,9 +52,14 @@ struct Item {
     int b, t;
     int64_t at;
 };
-struct Line {
-    int64_t total;     // tiles of tokens of a kv head
-    int64_t items;
+// Where a worker's share begins: tile `tile` of item e of kv head h, and the tiles that are its; a kv head has `items`.
+struct Start {
+    int h, e, tile, items;
+    int64_t tiles;
+};
+// An item of which n workers have pieces, from worker w on.
+struct Joint {
+    int h, b, t, w, n, pad;
 };
 
 struct C {   // kernel arguments
@@ -59,12 +69,14 @@ struct C {   // kernel arguments
     const int32_t *row_start, *n_new;
     uint16_t* o;
     float* lse;
-    Line* line;
-    Item* items;       // and one behind the last
+    Start* starts;     // of the workers
+    Joint* joints;     // n is 0 behind the last
+    Item* items;       // of a kv head
     float* part;       // pieces: [slot][BM][D] unnormalised O, then [slot][BM] (m, l)
     float2* part_ml;
     long long q_stride;
-    int B, Hkv, G, num_pages, page_shift, max_pages, cap, rows, causal, window, workers;
+    int B, Hkv, G, num_pages, page_shift, max_pages, cap, rows, causal, window;
+    int workers;       // 0: a workgroup an item
     float sl2;         // scale * log2(e)
 };
 
@@ -73,28 +85,37 @@ __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlan
 __device__ __forceinline__ int fixed(const int32_t* p, long long i) {
     return *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p + i);
 }
-__device__ __forceinline__ int64_t fixed64(const int64_t* p) {
-    return *(const __attribute__((address_space(4))) int64_t*)(uintptr_t)p;
-}
 __device__ __forceinline__ Item fixed_item(const Item* p) {
-    Item e;
     const auto* q = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
-    e.b = q[0];
-    e.t = q[1];
-    e.at = fixed64(&p->at);
-    return e;
+    return Item{q[0], q[1], 0};
 }
+__device__ __forceinline__ Start fixed_start(const Start* p) {
+    const auto* q = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+    return Start{q[0], q[1], q[2], q[3], *(const __attribute__((address_space(4))) int64_t*)(uintptr_t)&p->tiles};
+}
+__device__ __forceinline__ Joint fixed_joint(const Joint* p) {
+    const auto* q = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+    return Joint{q[0], q[1], q[2], q[3], q[4], 0};
+}
+template <int DT>
+constexpr uint32_t kInf = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // A sequence's rows: `n` of them from row `row0` on, the first at position `pos`; len -1 if it lies outside the table.
 struct Seq {
     int n, row0, pos, len;
 };
+template <bool FIXED = false>
 __device__ __forceinline__ Seq seq_of(const C& a, int b) {
+    auto get = [&](const int32_t* p) {
+        if constexpr (FIXED) return fixed(p, b);
+        else return p[b];
+    };
     Seq s;
     const int each = a.rows / a.B;
-    s.row0 = a.row_start ? a.row_start[b] : b * each;
-    const int n = a.n_new ? a.n_new[b] : each;
-    s.len = a.len[b];
+    s.row0 = a.row_start ? get(a.row_start) : b * each;
+    const int n = a.n_new ? get(a.n_new) : each;
+    s.len = get(a.len);
     if ((unsigned)s.len > (unsigned)a.cap) s.len = -1;
     s.n = s.row0 < 0 || s.row0 >= a.rows ? 0 : max(0, min(n, a.rows - s.row0));
     s.pos = s.len - max(n, 0);       // above -2^31: neither is below -1, nor n above 2^31 - 1
@@ -114,9 +135,13 @@ __device__ __forceinline__ int2 tiles_of(const C& a, const Seq& s, int first, in
 
 constexpr int TL = 1024;
 
-// Lists the items of a kv head, sequence after sequence, and their places in its line.  One workgroup.
+__device__ __forceinline__ int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
+
+// Lists the items of a kv head, sequence after sequence, and their places in its line; then the workers' shares.  One
+// workgroup.
 __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
     __shared__ Scan<TL> lds;
+    __shared__ int64_t place[TL];      // of the first items
     int64_t before = 0, items = 0;
     for (int c = 0; c < a.B; c += TL) {
         const int b = c + threadIdx.x;
@@ -137,30 +162,52 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
                 tiles = max(1, x.y - x.x);       // an item that sees nothing still has outputs
             }
             e.at = before + lds.sum(1, tiles, sum) - tiles;
-            if (k < all) a.items[items + k] = e;
+            if (k < all) {
+                a.items[items + k] = e;
+                if (items + k < TL) place[items + k] = e.at;
+            }
             before += sum;
             __syncthreads();
         }
         items += all;
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        a.items[items] = Item{0, 0, before};
-        *a.line = Line{before, items};
+    const int64_t all = before * a.Hkv, each = div_up(all, a.workers);
+    auto begin = [&](int64_t e) { return e < TL ? place[e] : a.items[e].at; };
+    int64_t joints = 0;
+    for (int w0 = 0; w0 < a.workers; w0 += TL) {
+        const int w = w0 + threadIdx.x;
+        Start st{0, 0, 0, (int)items, 0};
+        Joint j{0, 0, 0, w - 1, 0, 0};
+        if (w < a.workers && w * each < all) {
+            const int64_t at = w * each % before;
+            st.h = (int)(w * each / before);
+            st.tiles = min(each, all - w * each);
+            int lo = 0, hi = (int)items - 1;          // the last item that begins at or before `at`
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (begin(mid) <= at) lo = mid;
+                else hi = mid - 1;
+            }
+            st.e = lo;
+            st.tile = (int)(at - begin(lo));
+            if (st.tile > 0 && st.tile <= each) {     // the first share that begins inside the item
+                const Item it = a.items[lo];
+                const int64_t left = (lo + 1 < items ? begin(lo + 1) : before) - at;
+                j.h = st.h;
+                j.b = it.b;
+                j.t = it.t;
+                j.n = 1 + (int)div_up(left, each);
+            }
+        }
+        int64_t sum;
+        const int64_t to = joints + lds.sum(w0 / TL % 2, j.n > 0, sum);
+        if (w < a.workers) a.starts[w] = st;
+        if (j.n > 0) a.joints[to - 1] = j;
+        joints += sum;
     }
+    for (int64_t i = joints + threadIdx.x; i < a.workers; i += TL) a.joints[i].n = 0;
 }
-
-// The item that holds place `at` of a head's line.
-__device__ __forceinline__ int item_at(const C& a, int items, int64_t at) {
-    int lo = 0, hi = items - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (fixed64(&a.items[mid + 1].at) > at) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
-}
-__device__ __forceinline__ int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
 
 // Row r of an item: its row of o and lse, and its head.
 __device__ __forceinline__ long long out_row(const C& a, const Seq& s, int h, int r) {
@@ -176,17 +223,19 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     constexpr int NI = TILE / 1024 / kWaves;   // DMA requests of a wave, a tile of K or V
     constexpr int NL = SPL ? PKS : 1;
     __shared__ __attribute__((aligned(1024))) char smem[2][2][TILE];    // [K, V][buffer]
+    __shared__ uint2 odds[2][D];               // [half][dim]: bits of the tokens whose value is inf or NaN, -inf or NaN
+    __shared__ int votes[kWaves];
 
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l32 = lane & 31, hi = lane >> 5;
-    const int items = (int)fixed64(&a.line->items);
-    if (!items) return;
-    const int64_t total = fixed64(&a.line->total), all = total * a.Hkv, each = div_up(all, a.workers);
     // consecutive shares on one XCD, whose L2 their keys and values then share
-    const int place = a.workers % 8 ? blockIdx.x : (int)(blockIdx.x % 8 * (a.workers / 8) + blockIdx.x / 8);
-    int64_t at = place * each;
-    const int64_t last = min(at + each, all);
-    if (at >= last) return;
-    int h = (int)(at / total), e = item_at(a, items, at - h * total);
+    const int place = a.workers % 8 || !a.workers ? blockIdx.x : (int)(blockIdx.x % 8 * (a.workers / 8) + blockIdx.x / 8);
+    Start st{(int)blockIdx.z, 0, 0, 0, 0};
+    if (a.workers) {
+        st = fixed_start(&a.starts[place]);
+        if (st.tiles == 0) return;
+    }
+    int h = st.h, e = st.e, from = st.tile;
+    int64_t left = st.tiles;
 
     const uint32_t lds0 = lds_addr(smem);
     // DMA: this wave's requests of a tile are 1024 bytes each, all of one half of 32 tokens
@@ -207,24 +256,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         voff[j] = l32 * 64 + (((j * 2 + hi) ^ (l32 / 4 % 4)) << 4);
     }
 
-    while (at < last) {
+    do {
         // ---- the item, and this workgroup's share of its tiles
-        const Item it = fixed_item(&a.items[e]);
-        const int64_t start = h * total + it.at, end = h * total + fixed64(&a.items[e + 1].at);
-        Seq s;
-        {
-            const int each_rows = a.rows / a.B;
-            s.row0 = a.row_start ? fixed(a.row_start, it.b) : it.b * each_rows;
-            const int n = a.n_new ? fixed(a.n_new, it.b) : each_rows;
-            s.len = fixed(a.len, it.b);
-            if ((unsigned)s.len > (unsigned)a.cap) s.len = -1;
-            s.n = s.row0 < 0 || s.row0 >= a.rows ? 0 : max(0, min(n, a.rows - s.row0));
-            s.pos = s.len - max(n, 0);
-        }
+        const Item it = a.workers ? fixed_item(&a.items[e]) : Item{(int)blockIdx.y, (int)blockIdx.x, 0};
+        const Seq s = seq_of<true>(a, it.b);
         const int R = s.n * a.G, r0 = it.t * BM;
+        if (r0 >= R) return;              // a workgroup an item: the sequence has fewer
         const int2 tiles = tiles_of(a, s, r0, min(r0 + BM, R) - 1);
-        const int ta = tiles.x + (int)(at - start), te = min(tiles.x + (int)(min(end, last) - start), tiles.y);
-        const bool whole = at == start && end <= last;
+        const int all = max(1, tiles.y - tiles.x);
+        if (!a.workers) left = all;
+        const int mine = (int)min(left, (int64_t)(all - from)), ta = tiles.x + from, te = min(ta + mine, tiles.y);
+        const bool whole = mine == all;
 
         // this lane's row; those behind the sequence's rows act as its last
         const int r = r0 + wave * 32 + l32;
@@ -241,6 +283,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             n0 = x.x / BN;
             n1 = (y.y + BN - 1) / BN;
         }
+        // tiles in [alike.x, alike.y) are seen whole by all rows of the item
+        const int2 alike{(seen_by(a, s, (min(r0 + BM, R) - 1) / a.G).x + BN - 1) / BN, seen_by(a, s, r0 / a.G).y / BN};
         u32x4 qf[KS];
         {
             const uint16_t* qp = a.q + (s.row0 + r / a.G) * a.q_stride + (long long)(h * a.G + r % a.G) * D + hi * 8;
@@ -282,26 +326,71 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 dma16_rows(make_rsrc((const char*)a.v + sub * HALF, HALF), dma_at + (uint32_t)((2 + buf) * TILE), dma_v);
             }
         };
-        // values of tokens behind the sequence's last become 0: what is there may be anything
-        auto clear_tail = [&](int t, int buf) {
+        // Values of tokens behind the sequence's last become 0, for what is there may be anything, and infinities and
+        // NaN, whose bits are left in `odds`.  True if there were any of these.
+        auto search = [&](int t, int buf) {
             const int left = s.len - t * BN;
-            if (left >= BN) return;
-            for (int i = threadIdx.x; i < TILE / 64; i += 64 * kWaves) {     // rows of 32 tokens of one dim
+            bool any = false;
+            for (int i = threadIdx.x; i < 2 * D; i += 64 * kWaves) {         // rows of 32 tokens of one dim
                 char* row = smem[1][buf] + i * 64;
-                const int from = i * 64 >= HALF ? 32 : 0;
+                const int from = i < D ? 0 : 32;
+                u16x2 most = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     u32x4* p = (u32x4*)(row + ((c ^ (i / 4 % 4)) << 4));
                     u32x4 x = *p;
+                    if (left < BN) {
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int j = from + c * 8 + 2 * w;
-                        x[w] &= (j < left ? 0xffffu : 0u) | (j + 1 < left ? 0xffff0000u : 0u);
+                        for (int w = 0; w < 4; ++w) {
+                            const int j = from + c * 8 + 2 * w;
+                            x[w] &= (j < left ? 0xffffu : 0u) | (j + 1 < left ? 0xffff0000u : 0u);
+                        }
+                        *p = x;
                     }
-                    *p = x;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[w] & 0x7fff7fffu));
                 }
+                uint2 bits = {0u, 0u};
+                if (max(most[0], most[1]) >= kInf<DT>) {
+                    any = true;
+#pragma unroll 1
+                    for (int j = 0; j < 32; ++j) {
+                        uint16_t* p = (uint16_t*)(row + ((j / 8 ^ (i / 4 % 4)) << 4)) + j % 8;
+                        const uint32_t x = *p, e = x & 0x7fffu;
+                        if (e < kInf<DT>) continue;
+                        if (x != (kInf<DT> | 0x8000u)) bits.x |= 1u << j;
+                        if (x != kInf<DT>) bits.y |= 1u << j;
+                        *p = 0;
+                    }
+                }
+                odds[i / D][i % D] = bits;
             }
+            any = __any(any);
+            if (lane == 0) votes[wave] = any;
             __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) all |= votes[w];
+            return uni(all) != 0;
+        };
+        // the values that `search` took out, for the rows that see them
+        auto add_odd = [&](int t) __attribute__((always_inline)) {
+            uint32_t sees[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int to = min(max(seen.y - t * BN - x * 32, 0), 32), from = min(max(seen.x - t * BN - x * 32, 0), 32);
+                sees[x] = (uint32_t)((1ull << to) - 1) & ~(uint32_t)((1ull << from) - 1);
+            }
+#pragma unroll
+            for (int db = 0; db < NDB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int d = db * 32 + i / 4 * 8 + hi * 4 + i % 4;
+                    const uint2 a0 = odds[0][d], a1 = odds[1][d];
+                    if ((a0.x & sees[0]) | (a1.x & sees[1])) o[db][i] += INFINITY;
+                    if ((a0.y & sees[0]) | (a1.y & sees[1])) o[db][i] -= INFINITY;
+                    __builtin_amdgcn_sched_barrier(0);       // it is seldom run, and is to take few registers
+                }
         };
 
         f32x16 sr[2];
@@ -383,20 +472,19 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         }
         wait_dma();
         __syncthreads();
-        auto step = [&](int t, auto Buf) __attribute__((always_inline)) {
-            constexpr int buf = decltype(Buf)::value;
-            clear_tail(t, buf);
+        for (int t = ta; t < te; ++t) {
+            const int buf = (t - ta) & 1;
+            const bool odd = (t < alike.x || t >= alike.y) && search(t, buf);
             if (t + 1 < te) {
                 issue(t + 1, buf ^ 1);
                 if (t + 2 < te) fetch(t + 2);
             }
-            if (t >= n0 && t < n1) tile(t, buf);
+            if (t >= n0 && t < n1) {
+                tile(t, buf);
+                if (__builtin_expect(odd, 0)) add_odd(t);
+            }
             wait_dma();
             __syncthreads();
-        };
-        for (int t = ta; t < te; t += 2) {
-            step(t, std::integral_constant<int, 0>{});
-            if (t + 1 < te) step(t + 1, std::integral_constant<int, 1>{});
         }
 
         // ---- out
@@ -417,7 +505,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 if (a.lse && hi == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
             }
         } else if (valid) {
-            const long long slot = (long long)place * 2 + (at == start ? 1 : 0);
+            const long long slot = (long long)place * 2 + (from == 0 ? 1 : 0);
             float* p = a.part + (slot * BM + (r - r0)) * D;
 #pragma unroll
             for (int db = 0; db < NDB; ++db)
@@ -426,73 +514,110 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                     *(f32x4*)(p + db * 32 + g * 8 + hi * 4) = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
             if (hi == 0) a.part_ml[slot * BM + (r - r0)] = float2{m, l};
         }
-        at = min(end, last);
-        if (++e == items) {
+        left -= mine;
+        from = 0;
+        if (++e == st.items) {
             e = 0;
             ++h;
         }
-    }
+    } while (left > 0);
 }
 
-// Joins the pieces of the items that several workgroups shared: a workgroup has 1024 / D rows of the item in which
-// worker blockIdx.x's share begins, if that is the first to begin in it.
+// Joins the pieces of the items that several workers shared, a wave a row: each of its lanes weighs a piece, of 64 at a
+// time, and has four dims of every (256 / D)th.
 template <int D, int DT>
 __global__ __launch_bounds__(256) void chunk_join_kernel(C a) {
-    constexpr int LANES = D / 4, ROWS = 256 / LANES;
-    const int items = (int)fixed64(&a.line->items), w = blockIdx.x + 1;
-    if (!items) return;
-    const int64_t total = fixed64(&a.line->total), all = total * a.Hkv, each = div_up(all, a.workers), at = w * each;
-    if (at >= all) return;
-    const int h = (int)(at / total), e = item_at(a, items, at - h * total);
-    const Item it = fixed_item(&a.items[e]);
-    const int64_t start = h * total + it.at, end = h * total + fixed64(&a.items[e + 1].at);
-    if (start == at || start / each + 1 != w) return;
-    const Seq s = seq_of(a, it.b);
-    const int r = (int)blockIdx.y * ROWS + threadIdx.x / LANES, R = s.n * a.G - it.t * BM, d = threadIdx.x % LANES * 4;
-    if (r >= min(R, BM)) return;
-    const int n = (int)((end - 1) / each) - (w - 1) + 1;      // pieces: workers w - 1 ..
-    auto slot = [&](int i) { return ((long long)(w - 1 + i) * 2 + (i ? 0 : 1)) * BM + r; };
+    constexpr int LANES = D / 4, EACH = 64 / LANES;
+    const Joint it = fixed_joint(&a.joints[blockIdx.x]);
+    if (it.n == 0) return;
+    const Seq s = seq_of<true>(a, it.b);
+    const int lane = threadIdx.x & 63, r = (int)blockIdx.y * 4 + uni(threadIdx.x >> 6);
+    if (r >= min(s.n * a.G - it.t * BM, BM)) return;
+    // the first worker's piece is of the item that its share ends with, the others' of the one that theirs begin with
+    auto slot = [&](int i) { return ((long long)(it.w + i) * 2 + (i ? 0 : 1)) * BM + r; };
     float m = -INFINITY;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, a.part_ml[slot(i)].x);
+    for (int i = lane; i < it.n; i += 64) m = fmaxf(m, a.part_ml[slot(i)].x);
+#pragma unroll
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+    const int d = lane % LANES * 4;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-    for (int i = 0; i < n; ++i) {
-        const float2 ml = a.part_ml[slot(i)];
-        const f32x4 x = *(const f32x4*)(a.part + slot(i) * D + d);
-        // a piece without a finite score has nothing but perhaps a NaN in its sum
-        const bool none = ml.x == -INFINITY;
-        const float f = none ? 0.f : fast_exp2(ml.x - m);
-        l += none ? ml.y : f * ml.y;
-        if (!none) o += f * x;
+    for (int i0 = 0; i0 < it.n; i0 += 64) {
+        float f = 0.f;
+        if (i0 + lane < it.n) {
+            const float2 ml = a.part_ml[slot(i0 + lane)];
+            // a piece without a finite score has nothing but perhaps a NaN in its sum
+            f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m);
+            l += ml.x == -INFINITY ? ml.y : f * ml.y;
+        }
+        const int n = min(64, it.n - i0);
+        for (int i = 0; i < n; i += 4 * EACH) {
+            f32x4 x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = *(const f32x4*)(a.part + slot(i0 + min(i + k * EACH + lane / LANES, n - 1)) * D + d);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float w = __shfl(f, i + k * EACH + lane / LANES, 64);      // 0 behind the last
+                if (w != 0.f) o += w * x[k];       // what has no weight may be anything
+            }
+        }
     }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x, 64);
+#pragma unroll
+    for (int x = 32; x >= LANES; x >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
+    if (lane >= LANES) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const long long row = out_row(a, s, h, it.t * BM + r);
+    const long long row = out_row(a, s, it.h, it.t * BM + r);
     *(u32x2*)(a.o + row * D + d) = u32x2{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
-    if (a.lse && d == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
+    if (a.lse && lane == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
 }
 
-// The most items that a kv head can have, and workers that a call can use.
-long long items_most(const tkm_attn_kv& kv, int rows, int Hq) {
-    const long long G = Hq / kv.Hkv;
-    return (rows * G + BM - 1) / BM + std::min<long long>(kv.B, rows);
-}
+// The most items that a sequence and that a kv head can have.
+long long items_each(const tkm_attn_kv& kv, int rows, int Hq) { return ((long long)rows * (Hq / kv.Hkv) + BM - 1) / BM; }
+long long items_most(const tkm_attn_kv& kv, int rows, int Hq) { return items_each(kv, rows, Hq) + std::min<long long>(kv.B, rows); }
+
+// A workgroup an item, where none has more than 16 tiles and the grid, which is laid out for all rows being one
+// sequence's, is not much larger than the card.
+constexpr long long kFewTokens = 1024, kFewItems = 1024;
+
+// The workers of a split call; 0 for the other.
 int workers_of(const tkm_attn_kv& kv, int rows, int Hq) {
+    if ((long long)kv.max_pages * kv.page <= kFewTokens && items_each(kv, rows, Hq) * kv.B <= kFewItems / kv.Hkv) return 0;
     const double tiles = (double)items_most(kv, rows, Hq) * kv.Hkv * (kv.max_pages * (double)kv.page / BN + 1);
-    return tiles < kWorkers ? (int)tiles : kWorkers;
+    return tiles < kWorkers ? std::max((int)tiles, 1) : kWorkers;
+}
+// Items that several workers can share: each holds a place where a share begins.
+int joints_of(const tkm_attn_kv& kv, int rows, int Hq) {
+    return (int)std::min<long long>(workers_of(kv, rows, Hq) - 1, items_most(kv, rows, Hq) * kv.Hkv);
 }
 size_t align_up(size_t n) { return (n + 255) & ~(size_t)255; }
-size_t items_bytes(const tkm_attn_kv& kv, int rows, int Hq) {
-    return align_up(sizeof(Line) + (size_t)(items_most(kv, rows, Hq) + 1) * sizeof(Item));
+struct Place {      // of the workspace's parts
+    size_t joints, items, part, ml, end;
+};
+Place places(const tkm_attn_kv& kv, int rows, int Hq) {
+    const size_t workers = workers_of(kv, rows, Hq), rows_of = workers * 2 * BM;
+    Place p;
+    p.joints = align_up(workers * sizeof(Start));
+    p.items = p.joints + align_up(workers * sizeof(Joint));
+    p.part = p.items + align_up((size_t)items_most(kv, rows, Hq) * sizeof(Item));
+    p.ml = p.part + rows_of * kv.D * sizeof(float);
+    p.end = p.ml + rows_of * sizeof(float2);
+    return p;
 }
 
 template <int D, int DT>
-int launch_t(const C& a, hipStream_t stream) {
-    hipLaunchKernelGGL(chunk_items_kernel, dim3(1), dim3(TL), 0, stream, a);
+int launch_t(const C& a, dim3 grid, int joints, hipStream_t stream) {
+    if (a.workers) {
+        hipLaunchKernelGGL(chunk_items_kernel, dim3(1), dim3(TL), 0, stream, a);
+        if (hipGetLastError() != hipSuccess) return -1;
+    }
+    hipLaunchKernelGGL((chunk_kernel<D, DT>), grid, dim3(64 * kWaves), 0, stream, a);
     if (hipGetLastError() != hipSuccess) return -1;
-    hipLaunchKernelGGL((chunk_kernel<D, DT>), dim3(a.workers), dim3(64 * kWaves), 0, stream, a);
-    if (hipGetLastError() != hipSuccess) return -1;
-    if (a.workers > 1) {
-        hipLaunchKernelGGL((chunk_join_kernel<D, DT>), dim3(a.workers - 1, BM / (1024 / D)), dim3(256), 0, stream, a);
+    if (joints > 0) {
+        hipLaunchKernelGGL((chunk_join_kernel<D, DT>), dim3(joints, BM / 4), dim3(256), 0, stream, a);
         if (hipGetLastError() != hipSuccess) return -1;
     }
     return 0;
@@ -506,24 +631,23 @@ bool chunk_fits(const tkm_attn_kv& kv, int rows, int Hq) {
 }
 
 size_t chunk_workspace(const tkm_attn_kv& kv, int rows, int Hq) {
-    const size_t pieces = (size_t)workers_of(kv, rows, Hq) * 2 * BM;
-    return items_bytes(kv, rows, Hq) + pieces * (kv.D + 2) * sizeof(float);
+    return workers_of(kv, rows, Hq) ? places(kv, rows, Hq).end : 0;
 }
 
 int launch_chunk(const ChunkArgs& x) {
     const tkm_attn_kv& kv = x.kv;
-    const int workers = workers_of(kv, x.rows, x.Hq);
+    const int workers = workers_of(kv, x.rows, x.Hq), joints = joints_of(kv, x.rows, x.Hq);
     char* ws = (char*)x.ws;
-    float* part = (float*)(ws + items_bytes(kv, x.rows, x.Hq));
-    const size_t pieces = (size_t)workers * 2 * BM;
+    const Place p = places(kv, x.rows, x.Hq);
     const C a{(const uint16_t*)kv.k, (const uint16_t*)kv.v, kv.table, kv.len, (const uint16_t*)x.q, x.row_start, x.n_new,
-              (uint16_t*)x.o, x.lse, (Line*)ws, (Item*)(ws + sizeof(Line)), part, (float2*)(part + pieces * kv.D), x.q_stride,
-              kv.B, kv.Hkv, x.Hq / kv.Hkv, kv.num_pages, __builtin_ctz(kv.page), kv.max_pages, kv.max_pages * kv.page, x.rows,
-              x.causal, x.window, workers, x.scale * 1.4426950408889634f};
-    note_kernels(kChunk | (workers > 1 ? kJoin : 0));
+              (uint16_t*)x.o, x.lse, (Start*)ws, (Joint*)(ws + p.joints), (Item*)(ws + p.items), (float*)(ws + p.part),
+              (float2*)(ws + p.ml), x.q_stride, kv.B, kv.Hkv, x.Hq / kv.Hkv, kv.num_pages, __builtin_ctz(kv.page), kv.max_pages,
+              kv.max_pages * kv.page, x.rows, x.causal, x.window, workers, x.scale * 1.4426950408889634f};
+    note_kernels(kChunk | (joints > 0 ? kJoin : 0));
+    const dim3 grid = workers ? dim3(workers) : dim3(items_each(kv, x.rows, x.Hq), kv.B, kv.Hkv);
     const hipStream_t stream = (hipStream_t)x.stream;
-    if (kv.D == 128) return kv.dtype == DT_F16 ? launch_t<128, DT_F16>(a, stream) : launch_t<128, DT_BF16>(a, stream);
-    return kv.dtype == DT_F16 ? launch_t<64, DT_F16>(a, stream) : launch_t<64, DT_BF16>(a, stream);
+    if (kv.D == 128) return kv.dtype == DT_F16 ? launch_t<128, DT_F16>(a, grid, joints, stream) : launch_t<128, DT_BF16>(a, grid, joints, stream);
+    return kv.dtype == DT_F16 ? launch_t<64, DT_F16>(a, grid, joints, stream) : launch_t<64, DT_BF16>(a, grid, joints, stream);
 }
 
 }  // namespace tkm

@@ -182,9 +182,9 @@ TKM_ATTN_API int tkm_attn_chunk(const tkm_attn_kv* kv, const void* q, long long 
     if (!(scale > 0.f) || scale * 1.4426950408889634f == INFINITY)     // scores are in log2 units
         return fail(TKM_ATTN_EINVAL, "scale must be positive and finite, also times log2(e)");
     const size_t need = tkm::chunk_workspace(*kv, rows, Hq);
-    if (!workspace || workspace_bytes < need)
+    if (need && (!workspace || workspace_bytes < need))
         return fail(TKM_ATTN_EWORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
-    if (!aligned(workspace, 16)) return fail(TKM_ATTN_EALIGN, "workspace must be 16-byte aligned");
+    if (need && !aligned(workspace, 16)) return fail(TKM_ATTN_EALIGN, "workspace must be 16-byte aligned");
     const tkm::ChunkArgs a{*kv, q, q_stride, row_start, n_new, rows, o, lse, Hq, scale, causal, window, workspace, stream};
     if (tkm::launch_chunk(a)) return fail(TKM_ATTN_ELAUNCH, "chunk: kernel launch failed");
     return TKM_ATTN_OK;
