@@ -30,6 +30,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.h"
 #include "attn_kv.h"
@@ -42,7 +43,7 @@ namespace {
 constexpr int BM = 128;           // rows of an item
 constexpr int BN = 64;            // tokens of a tile
 constexpr int kWaves = 4;
-constexpr int kWorkers = 512;     // workgroups: two on each compute unit
+constexpr int workers_at(int D) { return D == 64 ? 768 : 512; }     // three or two workgroups on each compute unit
 constexpr float kLift = 8.0f;
 constexpr float kSumMax = 65504.0f;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -57,9 +58,10 @@ struct Start {
     int h, e, tile, items;
     int64_t tiles;
 };
-// An item of which n workers have pieces, from worker w on.
+// An item of which n workers have pieces, from worker w on: `rows` rows of kv head h, the first of them row r0 of a
+// sequence whose first token is row `row0` of the call.
 struct Joint {
-    int h, b, t, w, n, pad;
+    int h, row0, r0, rows, w, n, pad[2];
 };
 
 struct C {   // kernel arguments
@@ -95,7 +97,7 @@ __device__ __forceinline__ Start fixed_start(const Start* p) {
 }
 __device__ __forceinline__ Joint fixed_joint(const Joint* p) {
     const auto* q = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
-    return Joint{q[0], q[1], q[2], q[3], q[4], 0};
+    return Joint{q[0], q[1], q[2], q[3], q[4], q[5], {}};
 }
 template <int DT>
 constexpr uint32_t kInf = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
@@ -178,7 +180,7 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
     for (int w0 = 0; w0 < a.workers; w0 += TL) {
         const int w = w0 + threadIdx.x;
         Start st{0, 0, 0, (int)items, 0};
-        Joint j{0, 0, 0, w - 1, 0, 0};
+        Joint j{0, 0, 0, 0, w - 1, 0, {}};
         if (w < a.workers && w * each < all) {
             const int64_t at = w * each % before;
             st.h = (int)(w * each / before);
@@ -194,9 +196,11 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
             if (st.tile > 0 && st.tile <= each) {     // the first share that begins inside the item
                 const Item it = a.items[lo];
                 const int64_t left = (lo + 1 < items ? begin(lo + 1) : before) - at;
+                const Seq s = seq_of(a, it.b);
                 j.h = st.h;
-                j.b = it.b;
-                j.t = it.t;
+                j.row0 = s.row0;
+                j.r0 = it.t * BM;
+                j.rows = min(s.n * a.G - j.r0, BM);
                 j.n = 1 + (int)div_up(left, each);
             }
         }
@@ -210,12 +214,12 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
 }
 
 // Row r of an item: its row of o and lse, and its head.
-__device__ __forceinline__ long long out_row(const C& a, const Seq& s, int h, int r) {
-    return ((long long)(s.row0 + r / a.G) * a.Hkv + h) * a.G + r % a.G;
+__device__ __forceinline__ long long out_row(const C& a, int row0, int h, int r) {
+    return ((long long)(row0 + r / a.G) * a.Hkv + h) * a.G + r % a.G;
 }
 
 template <int D, int DT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_kernel(C a) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void chunk_kernel(C a) {
     constexpr bool SPL = Split<DT>::on;
     constexpr int KS = D / 16, NDB = D / 32, PKS = BN / 16;
     constexpr int HALF = D * 64;               // bytes of 32 tokens of K or V
@@ -472,8 +476,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         }
         wait_dma();
         __syncthreads();
-        for (int t = ta; t < te; ++t) {
-            const int buf = (t - ta) & 1;
+        auto step = [&](int t, auto Buf) __attribute__((always_inline)) {
+            const int buf = Buf;
             const bool odd = (t < alike.x || t >= alike.y) && search(t, buf);
             if (t + 1 < te) {
                 issue(t + 1, buf ^ 1);
@@ -485,6 +489,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             }
             wait_dma();
             __syncthreads();
+        };
+        if constexpr (D == 64) {       // one body: two would take more registers than three waves a SIMD leave
+            for (int t = ta; t < te; ++t) step(t, (t - ta) & 1);
+        } else {                       // 3% faster than one at 128 rows an item
+            for (int t = ta; t < te; t += 2) {
+                step(t, std::integral_constant<int, 0>{});
+                if (t + 1 < te) step(t + 1, std::integral_constant<int, 1>{});
+            }
         }
 
         // ---- out
@@ -492,7 +504,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         if (bad) l = NAN;
         if (whole) {
             if (valid) {
-                const long long row = out_row(a, s, h, r);
+                const long long row = out_row(a, s.row0, h, r);
                 const float inv = l == 0.f ? 0.f : 1.0f / l;
                 uint16_t* orow = a.o + row * D;
 #pragma unroll
@@ -523,56 +535,86 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     } while (left > 0);
 }
 
-// Joins the pieces of the items that several workers shared, a wave a row: each of its lanes weighs a piece, of 64 at a
-// time, and has four dims of every (256 / D)th.
 template <int D, int DT>
-__global__ __launch_bounds__(256) void chunk_join_kernel(C a) {
-    constexpr int LANES = D / 4, EACH = 64 / LANES;
+__device__ __forceinline__ void put_joined(const C& a, const Joint& it, int r, int d, f32x4 o, float m, float l) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const long long row = out_row(a, it.row0, it.h, it.r0 + r);
+    *(u32x2*)(a.o + row * D + d) = u32x2{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+    if (a.lse && d == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
+}
+
+// Joins the pieces of the items that several workers shared, `each` rows a workgroup.  Few pieces: a row for each D / 4
+// lanes, whose loads are all under way at once.  Else a wave has a row: each lane weighs a piece, of 64 at a time, and
+// has four dims of every (256 / D)th.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void chunk_join_kernel(C a, int each) {
+    constexpr int LANES = D / 4, EACH = 64 / LANES, FEW = 4;
     const Joint it = fixed_joint(&a.joints[blockIdx.x]);
-    if (it.n == 0) return;
-    const Seq s = seq_of<true>(a, it.b);
-    const int lane = threadIdx.x & 63, r = (int)blockIdx.y * 4 + uni(threadIdx.x >> 6);
-    if (r >= min(s.n * a.G - it.t * BM, BM)) return;
+    const int first = (int)blockIdx.y * each, end = min(first + each, it.rows);
+    if (it.n == 0 || first >= end) return;
+    const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), d = lane % LANES * 4;
     // the first worker's piece is of the item that its share ends with, the others' of the one that theirs begin with
-    auto slot = [&](int i) { return ((long long)(it.w + i) * 2 + (i ? 0 : 1)) * BM + r; };
-    float m = -INFINITY;
-    for (int i = lane; i < it.n; i += 64) m = fmaxf(m, a.part_ml[slot(i)].x);
+    auto slot = [&](int i, int r) { return ((long long)(it.w + i) * 2 + (i ? 0 : 1)) * BM + r; };
+    // a piece without a finite score has nothing but perhaps a NaN in its sum
+    auto weight = [](float2 ml, float m) { return ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m); };
+    if (it.n <= FEW) {
+        for (int r = first + wave * EACH + lane / LANES; r < end; r += 4 * EACH) {
+            float2 ml[FEW];
+            f32x4 x[FEW], o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-    const int d = lane % LANES * 4;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int i0 = 0; i0 < it.n; i0 += 64) {
-        float f = 0.f;
-        if (i0 + lane < it.n) {
-            const float2 ml = a.part_ml[slot(i0 + lane)];
-            // a piece without a finite score has nothing but perhaps a NaN in its sum
-            f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m);
-            l += ml.x == -INFINITY ? ml.y : f * ml.y;
+            for (int i = 0; i < FEW; ++i) {
+                const long long from = slot(min(i, it.n - 1), r);
+                ml[i] = a.part_ml[from];
+                x[i] = *(const f32x4*)(a.part + from * D + d);
+            }
+            float m = ml[0].x, l = 0.f;
+#pragma unroll
+            for (int i = 1; i < FEW; ++i) m = fmaxf(m, ml[i].x);
+#pragma unroll
+            for (int i = 0; i < FEW; ++i) {
+                if (i >= it.n) break;
+                const float f = weight(ml[i], m);
+                l += ml[i].x == -INFINITY ? ml[i].y : f * ml[i].y;
+                if (f != 0.f) o += f * x[i];       // what has no weight may be anything
+            }
+            put_joined<D, DT>(a, it, r, d, o, m, l);
         }
-        const int n = min(64, it.n - i0);
-        for (int i = 0; i < n; i += 4 * EACH) {
-            f32x4 x[4];
+        return;
+    }
+    for (int r = first + wave; r < end; r += 4) {
+        float m = -INFINITY;
+        for (int i = lane; i < it.n; i += 64) m = fmaxf(m, a.part_ml[slot(i, r)].x);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = *(const f32x4*)(a.part + slot(i0 + min(i + k * EACH + lane / LANES, n - 1)) * D + d);
+        for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+        for (int i0 = 0; i0 < it.n; i0 += 64) {
+            float f = 0.f;
+            if (i0 + lane < it.n) {
+                const float2 ml = a.part_ml[slot(i0 + lane, r)];
+                f = weight(ml, m);
+                l += ml.x == -INFINITY ? ml.y : f * ml.y;
+            }
+            const int n = min(64, it.n - i0);
+            for (int i = 0; i < n; i += 4 * EACH) {
+                f32x4 x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float w = __shfl(f, i + k * EACH + lane / LANES, 64);      // 0 behind the last
-                if (w != 0.f) o += w * x[k];       // what has no weight may be anything
+                for (int k = 0; k < 4; ++k) x[k] = *(const f32x4*)(a.part + slot(i0 + min(i + k * EACH + lane / LANES, n - 1), r) * D + d);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float w = __shfl(f, i + k * EACH + lane / LANES, 64);      // 0 behind the last
+                    if (w != 0.f) o += w * x[k];
+                }
             }
         }
+#pragma unroll
+        for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x, 64);
+#pragma unroll
+        for (int x = 32; x >= LANES; x >>= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
+        if (lane < LANES) put_joined<D, DT>(a, it, r, d, o, m, l);
     }
-#pragma unroll
-    for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x, 64);
-#pragma unroll
-    for (int x = 32; x >= LANES; x >>= 1)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
-    if (lane >= LANES) return;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const long long row = out_row(a, s, it.h, it.t * BM + r);
-    *(u32x2*)(a.o + row * D + d) = u32x2{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
-    if (a.lse && lane == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
 }
 
 // The most items that a sequence and that a kv head can have.
@@ -587,7 +629,7 @@ constexpr long long kFewTokens = 1024, kFewItems = 1024;
 int workers_of(const tkm_attn_kv& kv, int rows, int Hq) {
     if ((long long)kv.max_pages * kv.page <= kFewTokens && items_each(kv, rows, Hq) * kv.B <= kFewItems / kv.Hkv) return 0;
     const double tiles = (double)items_most(kv, rows, Hq) * kv.Hkv * (kv.max_pages * (double)kv.page / BN + 1);
-    return tiles < kWorkers ? std::max((int)tiles, 1) : kWorkers;
+    return (int)std::max(std::min(tiles, (double)workers_at(kv.D)), 1.0);
 }
 // Items that several workers can share: each holds a place where a share begins.
 int joints_of(const tkm_attn_kv& kv, int rows, int Hq) {
@@ -617,7 +659,9 @@ int launch_t(const C& a, dim3 grid, int joints, hipStream_t stream) {
     hipLaunchKernelGGL((chunk_kernel<D, DT>), grid, dim3(64 * kWaves), 0, stream, a);
     if (hipGetLastError() != hipSuccess) return -1;
     if (joints > 0) {
-        hipLaunchKernelGGL((chunk_join_kernel<D, DT>), dim3(joints, BM / 4), dim3(256), 0, stream, a);
+        // few items in many pieces: a wave a row; else workgroups enough without it
+        const int each = joints * (BM / 4) <= 4096 ? 4 : 32;
+        hipLaunchKernelGGL((chunk_join_kernel<D, DT>), dim3(joints, BM / each), dim3(256), 0, stream, a, each);
         if (hipGetLastError() != hipSuccess) return -1;
     }
     return 0;
