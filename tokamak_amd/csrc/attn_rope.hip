@@ -6,7 +6,9 @@
 // of a circle whatever the position is.  A row's rot/2 sines and cosines are formed once, in fp32, and shared by its
 // heads through LDS; products and sums are fp32, rounded once on the way out.
 //
-// Both kernels move data and are bound by HBM, or by the launch where rows are few.
+// Both kernels move data and are bound by HBM, or by the launch where rows are few.  A thread has a chunk of 8 dims, 16
+// bytes, of one head at a time, and forms its side of the pairs; a head's chunks are one wave's, at one time, which
+// reads the other sides before it writes, so that rows may be rotated in place.
 #include <hip/hip_runtime.h>
 
 #include "attn_common.h"
@@ -24,17 +26,17 @@ template <> struct Vec<8> { typedef u32x4 T; };
 template <> struct Vec<4> { typedef u32x2 T; };
 template <> struct Vec<2> { typedef uint32_t T; };
 template <> struct Vec<1> { typedef uint16_t T; };
-template <int N>
-struct Part {
-    uint16_t e[N];
-    __device__ __forceinline__ void load(const uint16_t* p) {
+struct Chunk {
+    uint16_t e[8];
+    template <int N>
+    __device__ __forceinline__ void load(int i, const uint16_t* p) {
         const typename Vec<N>::T v = *(const typename Vec<N>::T*)p;
-        __builtin_memcpy(e, &v, 2 * N);
+        __builtin_memcpy(e + i, &v, 2 * N);
     }
     __device__ __forceinline__ void store(uint16_t* p) const {
-        typename Vec<N>::T v;
-        __builtin_memcpy(&v, e, 2 * N);
-        *(typename Vec<N>::T*)p = v;
+        u32x4 v;
+        __builtin_memcpy(&v, e, 16);
+        *(u32x4*)p = v;
     }
 };
 template <int DT>
@@ -49,27 +51,39 @@ __device__ __forceinline__ float2 turn(const tkm_attn_rope& rope, int i, int pos
     return float2{c * rope.factor, s * rope.factor * sign};
 }
 
-// A unit: V pairs of one head, as two parts of V values (HALVES: rot/2 apart) or as one of 2 V (PAIRS).
+// Dims d .. d + 7 of a rotated head at p.  HALVES: pairs (i, i + rot / 2), whose other sides come V at a time, the
+// largest power of two that divides rot / 2 (of up to 8), so that all V have the same place in their pairs.
 template <int DT, int LAYOUT, int V>
-struct Unit {
-    static constexpr int N = LAYOUT == TKM_ROPE_HALVES ? V : 2 * V;
-    Part<N> x, y;
-    __device__ __forceinline__ static int first(int u) { return u * N; }      // dim of x; y's is rot/2 behind it
-    __device__ __forceinline__ void load(const uint16_t* p, int half) {
-        x.load(p);
-        if constexpr (LAYOUT == TKM_ROPE_HALVES) y.load(p + half);
-    }
-    __device__ __forceinline__ void rotate(const float2* cs) {
+__device__ __forceinline__ Chunk rotated(const uint16_t* p, int d, int rot, const float2* cs) {
+    Chunk x, y;
+    x.load<8>(0, p + d);
+    if constexpr (LAYOUT == TKM_ROPE_HALVES) {
+        const int half = rot / 2;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            uint16_t& e0 = LAYOUT == TKM_ROPE_HALVES ? x.e[j] : x.e[(2 * j) % N];
-            uint16_t& e1 = LAYOUT == TKM_ROPE_HALVES ? y.e[j] : x.e[(2 * j + 1) % N];
-            const float a = to_f32<DT>(e0), b = to_f32<DT>(e1);
-            e0 = to_16<DT>(a * cs[j].x - b * cs[j].y);
-            e1 = to_16<DT>(a * cs[j].y + b * cs[j].x);
+        for (int i = 0; i < 8; i += V)
+            if (d + i < rot) y.load<V>(i, p + (d + i < half ? d + i + half : d + i - half));
+#pragma unroll
+        for (int i = 0; i < 8; i += V) {
+            if (d + i >= rot) continue;
+            const bool low = d + i < half;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float2 t = cs[d + i + j - (low ? 0 : half)];
+                x.e[i + j] = to_16<DT>(to_f32<DT>(x.e[i + j]) * t.x + to_f32<DT>(y.e[i + j]) * (low ? -t.y : t.y));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            if (d + j >= rot) continue;
+            const float2 t = cs[(d + j) / 2];
+            const float a = to_f32<DT>(x.e[j]), b = to_f32<DT>(x.e[j + 1]);
+            x.e[j] = to_16<DT>(a * t.x - b * t.y);
+            x.e[j + 1] = to_16<DT>(a * t.y + b * t.x);
         }
     }
-};
+    return x;
+}
 
 // `T` threads have a row: their place in it, and the row's sines and cosines in LDS.
 struct Row {
@@ -108,38 +122,17 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeK a) {
     if (w.pos < 0) return;
     const uint16_t* in = a.in + w.r * a.in_stride;
     uint16_t* out = a.out + w.r * a.out_stride;
-    const int half = a.rope.rot / 2, units = half / V, lanes = w.T / units, u = w.t % units;
-    typedef Unit<DT, LAYOUT, V> U;
-    if (w.t < lanes * units)
-        for (int h = w.t / units; h < a.heads; h += lanes) {
-            const int at = h * a.D + U::first(u);
-            U x;
-            x.load(in + at, half);
-            x.rotate(w.cs + u * V);
-            x.x.store(out + at);
-            if constexpr (LAYOUT == TKM_ROPE_HALVES) x.y.store(out + at + half);
+    const int chunks = a.D / 8, rotate = a.heads * chunks, all = in == out ? rotate : a.all * chunks;
+    for (int i = w.t; i < all; i += w.T) {
+        Chunk x;
+        if (i < rotate) {
+            const int d = i % chunks * 8;
+            x = rotated<DT, LAYOUT, V>(in + i * 8 - d, d, a.rope.rot, w.cs);
+        } else {
+            x.load<8>(0, in + i * 8);
         }
-    if (in == out) return;
-    // what is not rotated: the heads' other dims, and whole heads
-    const int rest = a.D - a.rope.rot, from = a.heads * a.D;
-    auto copy = [&](auto Nc) {
-        constexpr int N = decltype(Nc)::value;
-        const int each = rest / N, n = a.heads * each;
-        for (int i = w.t; i < n; i += w.T) {
-            const int at = i / each * a.D + a.rope.rot + i % each * N;
-            Part<N> p;
-            p.load(in + at);
-            p.store(out + at);
-        }
-    };
-    if (rest) {
-        if (a.rope.rot % 8 == 0) copy(std::integral_constant<int, 8>{});
-        else copy(std::integral_constant<int, 2>{});
-    }
-    for (int i = w.t * 8; i < (a.all - a.heads) * a.D; i += w.T * 8) {
-        Part<8> p;
-        p.load(in + from + i);
-        p.store(out + from + i);
+        __builtin_amdgcn_wave_barrier();      // all lanes have read before one writes
+        x.store(out + i * 8);
     }
 }
 
@@ -202,45 +195,18 @@ __global__ __launch_bounds__(kThreads) void store_rows_kernel(StoreK a) {
     if (w.pos < 0) return;
     const int64_t slot = a.slot[w.r];
     const bool kept = in_pool(kv, slot);
-    const int tok = (int)(slot & 31), rot = a.rope.rot, D = kv.D;
+    const int tok = (int)(slot & 31), rot = a.rope.rot, D = kv.D, chunks = D / 8;
     const uint16_t* in = a.qkv + w.r * a.stride;
     uint16_t* q = a.q ? a.q + w.r * a.q_stride : nullptr;
-    // where dim d of head h (Q heads, then K heads) goes
-    auto to = [&](int h, int d) {
-        if (h < a.Hq) return q + h * D + d;
-        return (uint16_t*)kv.k + tile_of(kv, slot, h - a.Hq) + (d >> 5) * 1024 + tok * 32 + (d & 31);
-    };
-    const int h0 = a.q ? 0 : a.Hq, h1 = a.Hq + (kept ? kv.Hkv : 0);
-    if (rot) {
-        const int half = rot / 2, units = half / V, lanes = w.T / units, u = w.t % units;
-        typedef Unit<DT, LAYOUT, V> U;
-        if (w.t < lanes * units)
-            for (int h = h0 + w.t / units; h < h1; h += lanes) {
-                U x;
-                x.load(in + h * D + U::first(u), half);
-                x.rotate(w.cs + u * V);
-                x.x.store(to(h, U::first(u)));
-                if constexpr (LAYOUT == TKM_ROPE_HALVES) x.y.store(to(h, U::first(u) + half));
-            }
-    }
-    const int rest = D - rot, c0 = q == in ? a.Hq : h0;        // Q's other dims are in place already
-    auto copy = [&](auto Nc) {
-        constexpr int N = decltype(Nc)::value;
-        const int each = rest / N;
-        for (int i = w.t; i < (h1 - c0) * each; i += w.T) {
-            const int h = c0 + i / each, d = rot + i % each * N;
-            Part<N> p;
-            p.load(in + h * D + d);
-            p.store(to(h, d));
-        }
-    };
-    if (rest) {
-        if (rot % 8 == 0) copy(std::integral_constant<int, 8>{});
-        else copy(std::integral_constant<int, 2>{});
+    for (int i = (a.q ? 0 : a.Hq * chunks) + w.t; i < (a.Hq + (kept ? kv.Hkv : 0)) * chunks; i += w.T) {
+        const int h = i / chunks, d = i % chunks * 8;
+        const Chunk x = rotated<DT, LAYOUT, V>(in + h * D, d, rot, w.cs);
+        __builtin_amdgcn_wave_barrier();      // all lanes have read before one writes
+        if (h < a.Hq) x.store(q + h * D + d);
+        else x.store((uint16_t*)kv.k + tile_of(kv, slot, h - a.Hq) + (d >> 5) * 1024 + tok * 32 + (d & 31));
     }
     if (!kept) return;
     if (a.T == kThreads) {             // few rows: V here too, its values to 64-byte rows of their own
-        const int chunks = D / 8;
         for (int i = w.t; i < kv.Hkv * chunks; i += w.T) {
             const int h = i / chunks, c = i % chunks;
             const u32x4 x = ld_global16(in + (long long)(a.Hq + kv.Hkv + h) * D + c * 8);
@@ -267,30 +233,22 @@ unsigned row_blocks(int rows) {
     return ((unsigned)rows + each - 1) / each;
 }
 
-// Pairs of a unit: as many as keep its parts aligned, of up to 16 bytes.
-int unit_pairs(const tkm_attn_rope& r) {
-    const int n = r.layout == TKM_ROPE_HALVES ? r.rot / 2 : r.rot;
-    int v = n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1;
-    return r.layout == TKM_ROPE_HALVES ? v : v / 2;
+// Other sides of pairs that are one access.
+int sides(const tkm_attn_rope& r) {
+    const int n = r.layout == TKM_ROPE_HALVES ? r.rot / 2 : 8;
+    return n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1;
 }
 
 template <class A, class F>
 void pick(int dtype, const tkm_attn_rope& r, const A& a, F launch) {
-    const int v = unit_pairs(r);
+    const int v = sides(r);
     auto with = [&](auto DT) {
-        auto go = [&](auto L, auto V) { launch(DT, L, V); };
         using H = std::integral_constant<int, TKM_ROPE_HALVES>;
-        using Pr = std::integral_constant<int, TKM_ROPE_PAIRS>;
-        if (r.layout == TKM_ROPE_HALVES) {
-            if (v == 8) go(H{}, std::integral_constant<int, 8>{});
-            else if (v == 4) go(H{}, std::integral_constant<int, 4>{});
-            else if (v == 2) go(H{}, std::integral_constant<int, 2>{});
-            else go(H{}, std::integral_constant<int, 1>{});
-        } else {
-            if (v == 4) go(Pr{}, std::integral_constant<int, 4>{});
-            else if (v == 2) go(Pr{}, std::integral_constant<int, 2>{});
-            else go(Pr{}, std::integral_constant<int, 1>{});
-        }
+        if (r.layout != TKM_ROPE_HALVES) launch(DT, std::integral_constant<int, TKM_ROPE_PAIRS>{}, std::integral_constant<int, 8>{});
+        else if (v == 8) launch(DT, H{}, std::integral_constant<int, 8>{});
+        else if (v == 4) launch(DT, H{}, std::integral_constant<int, 4>{});
+        else if (v == 2) launch(DT, H{}, std::integral_constant<int, 2>{});
+        else launch(DT, H{}, std::integral_constant<int, 1>{});
     };
     if (dtype == TKM_ATTN_F16) with(std::integral_constant<int, DT_F16>{});
     else with(std::integral_constant<int, DT_BF16>{});
