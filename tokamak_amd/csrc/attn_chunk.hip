@@ -218,8 +218,16 @@ __device__ __forceinline__ long long out_row(const C& a, int row0, int h, int r)
     return ((long long)(row0 + r / a.G) * a.Hkv + h) * a.G + r % a.G;
 }
 
+// The arguments of the kernel that runs, read where they are used: those of its whole life would not fit into the scalar
+// registers, and every tile would move some of them from and to vector registers.
+__device__ __forceinline__ const C& arguments() {
+    auto p = (const __attribute__((address_space(4))) C*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const C*)p;
+}
+
 template <int D, int DT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void chunk_kernel(C a) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void chunk_kernel(C args) {
     constexpr bool SPL = Split<DT>::on;
     constexpr int KS = D / 16, NDB = D / 32, PKS = BN / 16;
     constexpr int HALF = D * 64;               // bytes of 32 tokens of K or V
@@ -232,10 +240,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l32 = lane & 31, hi = lane >> 5;
     // consecutive shares on one XCD, whose L2 their keys and values then share
-    const int place = a.workers % 8 || !a.workers ? blockIdx.x : (int)(blockIdx.x % 8 * (a.workers / 8) + blockIdx.x / 8);
+    const int workers = args.workers;
+    const int place = workers % 8 || !workers ? blockIdx.x : (int)(blockIdx.x % 8 * (workers / 8) + blockIdx.x / 8);
     Start st{(int)blockIdx.z, 0, 0, 0, 0};
-    if (a.workers) {
-        st = fixed_start(&a.starts[place]);
+    if (workers) {
+        st = fixed_start(&args.starts[place]);
         if (st.tiles == 0) return;
     }
     int h = st.h, e = st.e, from = st.tile;
@@ -262,13 +271,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 
     do {
         // ---- the item, and this workgroup's share of its tiles
-        const Item it = a.workers ? fixed_item(&a.items[e]) : Item{(int)blockIdx.y, (int)blockIdx.x, 0};
+        const C& a = arguments();
+        const Item it = workers ? fixed_item(&a.items[e]) : Item{(int)blockIdx.y, (int)blockIdx.x, 0};
         const Seq s = seq_of<true>(a, it.b);
         const int R = s.n * a.G, r0 = it.t * BM;
         if (r0 >= R) return;              // a workgroup an item: the sequence has fewer
         const int2 tiles = tiles_of(a, s, r0, min(r0 + BM, R) - 1);
         const int all = max(1, tiles.y - tiles.x);
-        if (!a.workers) left = all;
+        if (!workers) left = all;
         const int mine = (int)min(left, (int64_t)(all - from)), ta = tiles.x + from, te = min(ta + mine, tiles.y);
         const bool whole = mine == all;
 
@@ -302,11 +312,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         bool bad = s.len < 0;
 
         // pages of a tile's halves, fetched a tile ahead
-        const int half_bits = a.page_shift - 5;
-        auto page_of = [&](int t, int x) {
-            const int p = (t * 2 + x) >> half_bits;
-            return fixed(a.table, (long long)it.b * a.max_pages + min(p, a.max_pages - 1));
-        };
+        const int half_bits = a.page_shift - 5, last_page = a.max_pages - 1, num_pages = a.num_pages, Hkv = a.Hkv;
+        const int32_t* pages = a.table + (long long)it.b * a.max_pages;
+        const char *keys = (const char*)a.k, *values = (const char*)a.v;
+        const float sl2 = a.sl2;
+        auto page_of = [&](int t, int x) { return fixed(pages, min((t * 2 + x) >> half_bits, last_page)); };
         int pg[2];
         auto fetch = [&](int t) {
             pg[0] = page_of(t, 0);
@@ -318,16 +328,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
             for (int x = 0; x < 2; ++x) {
                 page[x] = pg[x];
                 const int from = t * BN + x * 32;
-                if ((unsigned)page[x] >= (unsigned)a.num_pages) {      // page 0 in its place; rows that see it become NaN
+                if ((unsigned)page[x] >= (unsigned)num_pages) {      // page 0 in its place; rows that see it become NaN
                     page[x] = 0;
                     bad |= from < seen.y && from + 32 > seen.x;
                 }
             }
             if (t * BN + my_half * 32 < s.len) {
                 const int half = t * 2 + my_half;
-                const long long sub = (((long long)(my_half ? page[1] : page[0]) * a.Hkv + h) << half_bits) + (half & ((1 << half_bits) - 1));
-                dma16_rows(make_rsrc((const char*)a.k + sub * HALF, HALF), dma_at + (uint32_t)(buf * TILE), dma_v);
-                dma16_rows(make_rsrc((const char*)a.v + sub * HALF, HALF), dma_at + (uint32_t)((2 + buf) * TILE), dma_v);
+                const long long sub = (((long long)(my_half ? page[1] : page[0]) * Hkv + h) << half_bits) + (half & ((1 << half_bits) - 1));
+                dma16_rows(make_rsrc(keys + sub * HALF, HALF), dma_at + (uint32_t)(buf * TILE), dma_v);
+                dma16_rows(make_rsrc(values + sub * HALF, HALF), dma_at + (uint32_t)((2 + buf) * TILE), dma_v);
             }
         };
         // Values of tokens behind the sequence's last become 0, for what is there may be anything, and infinities and
@@ -426,8 +436,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const int x = (ks & 1) * 8 + 2 * w;
-                    const float p0 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x], a.sl2, -ref));
-                    const float p1 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x + 1], a.sl2, -ref));
+                    const float p0 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x], sl2, -ref));
+                    const float p1 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x + 1], sl2, -ref));
                     if constexpr (SPL) {
                         const u32x2 hl = pack_split_bf16(p0, p1);
                         pr[ks][w] = hl[0];
@@ -442,14 +452,15 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         auto tile = [&](int t, int buf) __attribute__((always_inline)) {
             scores(buf);
             if (t < p0 || t >= p1) mask(t);
-            float sum = expo(m);
-            if (__builtin_expect(__any(!(sum < kSumMax)), 0)) {        // also where m is not set yet
+            float sum = INFINITY;
+            if (!__any(m == -INFINITY)) sum = expo(m);                 // m is not set yet in an item's first tile
+            if (__builtin_expect(__any(!(sum < kSumMax)), 0)) {
                 float v = sr[0][0];
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int x = kb ? 0 : 1; x < 16; ++x) v = fmaxf(v, sr[kb][x]);
-                const float mn = fmaxf(m, half_max(v) * a.sl2 - kLift);
+                const float mn = fmaxf(m, half_max(v) * sl2 - kLift);
                 const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);      // nothing is there to be scaled if m is not set
                 lsum *= f;
 #pragma unroll
@@ -500,13 +511,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         }
 
         // ---- out
+        const C& z = arguments();
         float l = half_sum(lsum);
         if (bad) l = NAN;
         if (whole) {
             if (valid) {
-                const long long row = out_row(a, s.row0, h, r);
+                const long long row = out_row(z, s.row0, h, r);
                 const float inv = l == 0.f ? 0.f : 1.0f / l;
-                uint16_t* orow = a.o + row * D;
+                uint16_t* orow = z.o + row * D;
 #pragma unroll
                 for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -514,17 +526,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                         const u32x2 w = {pack2<DT>(o[db][g * 4] * inv, o[db][g * 4 + 1] * inv), pack2<DT>(o[db][g * 4 + 2] * inv, o[db][g * 4 + 3] * inv)};
                         *(u32x2*)(orow + db * 32 + g * 8 + hi * 4) = w;
                     }
-                if (a.lse && hi == 0) a.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
+                if (z.lse && hi == 0) z.lse[row] = l > 0.f ? m * kLn2 + logf(l) : l == 0.f ? -INFINITY : NAN;
             }
         } else if (valid) {
             const long long slot = (long long)place * 2 + (from == 0 ? 1 : 0);
-            float* p = a.part + (slot * BM + (r - r0)) * D;
+            float* p = z.part + (slot * BM + (r - r0)) * D;
 #pragma unroll
             for (int db = 0; db < NDB; ++db)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                     *(f32x4*)(p + db * 32 + g * 8 + hi * 4) = f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
-            if (hi == 0) a.part_ml[slot * BM + (r - r0)] = float2{m, l};
+            if (hi == 0) z.part_ml[slot * BM + (r - r0)] = float2{m, l};
         }
         left -= mine;
         from = 0;
