@@ -199,3 +199,14 @@ def test_plan_by_a_loop():
     assert p["n_new"] == [40, 0, 0, 3] and p["row_start"] == [0, 40, 40, 40, 43] and p["kv_len"] == [70, 0, 20, 7]
     assert p["table"] == [[5, 7, 6], [-1, -1, -1], [8, -1, -1], [9, -1, -1]] and p["n_free"] == [2] and p["held"] == [3, 0, 1, 1]
     assert p["slot"][:4] == [5 * 32 + 30, 5 * 32 + 31, 7 * 32, 7 * 32 + 1] and p["slot"][40:44] == [9 * 32 + 4, 9 * 32 + 5, 9 * 32 + 6, -1]
+
+
+def test_tensors_off_the_gpu_are_refused():
+    import torch
+    x, dt = torch.zeros(4, 3 * 64, dtype=torch.float16), torch.int32
+    with pytest.raises(ValueError, match="GPU"):
+        attn.rope_fwd(x, attn.Rope(64), 1, 1, 64, S=4)
+    with pytest.raises(ValueError, match="must be on"):
+        attn.KvPages(torch.zeros(8, dtype=dt), torch.zeros(1, dtype=dt), torch.zeros(2, dtype=dt))
+    with pytest.raises(ValueError, match="must be on"):
+        attn.KvPlan.empty(2, 4, "cpu")

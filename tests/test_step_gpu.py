@@ -420,3 +420,253 @@ def test_chunk_of_rows_outside(gpu):
     o, lse = attn.gqa_chunk(q, case.cache, 4, i32([-5, 3, 18, 20], gpu), i32([4, 5, 7, 3], gpu), out=out)
     check_chunk(case, [100] * 4, [0, 5, 0, 0], q, o, lse, 4, row_start=[0, 3, 0, 0])
     assert (out[:3] == 4.0).all() and (out[8:18] == 4.0).all() and torch.isfinite(out[18:]).all()
+
+
+# ---- together ---------------------------------------------------------------------------------------------------
+
+
+def rewound(case, b, n):
+    """The case's sequence b cut to its first n tokens."""
+    case.k[b], case.v[b] = case.k[b][:, :n], case.v[b][:, :n]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype,most,rope", [(8, 2, 64, 32, "f16", 12, (64, "halves", None)), (4, 4, 128, 64, "bf16", 40, (96, "pairs", "yarn")),
+                                                           (6, 1, 64, 64, "bf16", 30, None)])
+def test_steps_of_a_server(gpu, Hq, Hkv, D, page, dtype, most, rope):
+    """Prompts, drafts of which a part is kept, single tokens, sequences that end and others in their place, a request
+    too long for its table: two layers that share pages and lengths, each step planned once, appended and attended in both."""
+    from tokamak_amd import attn
+    print(f"[case] server Hq{Hq} Hkv{Hkv} D{D} page{page} {dtype}", flush=True)
+    B, rows, W = 4, 400, (Hq + 2 * Hkv) * D
+    layers = [Case(gpu, [0] * B, Hkv, D, page, dtype, spare=24, extra_pages=most - 1, seed=i) for i in range(2)]
+    c = layers[0].cache
+    layers[1].cache = attn.KvCache(layers[1].cache.k, layers[1].cache.v, c.table, c.kv_len)
+    pages = attn.KvPages.all_free(c)
+    assert pages.free.tolist() == list(range(c.num_pages - 1, -1, -1)) and int(pages.n_free) == c.num_pages
+    r, (freqs, factor) = rope_of(*rope) if rope else (None, (None, None))
+    plan = attn.KvPlan.empty(B, rows, gpu)
+    lens, tokens = [0] * B, c.num_pages * page
+    steps = [([130, 40, 0, 7], None), ([5, 5, 0, 5], None), ([1, 1, 90, 1], [132, 45, 0, 9]), ([1, 1, 1, 1], None), ([0, 0, 3, 3], [0, 46, 91, 11]),
+             ([170, tokens, 1, 1], None), ([1, 1, 1, 1], None)]
+    for i, (want, start) in enumerate(steps):
+        start = list(lens) if start is None else start
+        ref = plan_ref(c.table.tolist(), pages.free.tolist(), int(pages.n_free), pages.held.tolist(), want, start, page, c.num_pages, rows)
+        attn.kv_plan(c, pages, i32(want, gpu), start=i32(start, gpu), plan=plan)
+        n_new, row_start, lens = ref["n_new"], ref["row_start"], ref["kv_len"]
+        assert plan.n_new.tolist() == n_new and plan.row_start.tolist() == row_start and plan.pos.tolist() == ref["pos"]
+        assert c.kv_len.tolist() == lens and pages.held.tolist() == ref["held"]
+        assert i != 5 or n_new == [170, 0, 1, 1]         # more than its table holds
+        total = row_start[-1]
+        for x, case in enumerate(layers):
+            qkv = randn((rows, W), dtype, 10 * i + x).to(gpu)
+            q = attn.kv_append_rows(qkv, case.cache, Hq, plan, rope=r)
+            o, lse = attn.gqa_chunk(q, case.cache, Hq, plan.row_start, plan.n_new)
+            new = qkv[:total].cpu().double().reshape(total, Hq + 2 * Hkv, D)
+            err = torch.zeros_like(new)
+            if rope:
+                new[:, :Hq + Hkv], err[:, :Hq + Hkv] = rope_ref(new[:, :Hq + Hkv], ref["pos"][:total], freqs, factor, rope[1])
+            check_rounded(q[:total, :Hq * D].cpu().double().reshape(total, Hq, D), new[:, :Hq], err[:, :Hq], dtype, "q")
+            for b in range(B):
+                rewound(case, b, start[b])
+                at = slice(row_start[b], row_start[b + 1])
+                k, v = case.held(b, case.cache)
+                assert torch.equal(k[:, :start[b]], case.k[b]) and torch.equal(v[:, :start[b]], case.v[b])       # what was there
+                check_rounded(k[:, start[b]:], new[at, Hq:Hq + Hkv].transpose(0, 1), err[at, Hq:Hq + Hkv].transpose(0, 1), dtype, "k")
+                assert torch.equal(v[:, start[b]:], new[at, Hq + Hkv:].transpose(0, 1))
+                case.k[b], case.v[b] = k, v
+            check_chunk(case, lens, n_new, q, o, lse, Hq)
+            if all(n == 1 for n in n_new):           # a token each: the decoding call has the same to do
+                check_chunk(case, lens, n_new, q, *attn.gqa_decode(q[:B], case.cache, Hq), Hq)
+
+
+def test_steps_captured_and_replayed(gpu):
+    """Plan, append in place and attention of two layers as one graph, replayed on requests and rows that change, with
+    eager work between, every replay against the eager calls bit for bit; two graphs use one workspace in turn."""
+    from tokamak_amd import attn
+    B, Hq, Hkv, D, page, dtype, rows = 5, 8, 2, 128, 64, "bf16", 96
+    r, _ = rope_of(128, "halves", "bands")
+    k = [randn((300, Hkv, page // 32, D // 32, 32, 32), dtype, s).to(gpu) for s in range(4)]
+    x = randn((2, rows, (Hq + 2 * Hkv) * D), dtype, 9).to(gpu)
+    want = torch.zeros(B, dtype=torch.int32, device=gpu)
+
+    def world():
+        table, length = torch.full((B, 50), -1, dtype=torch.int32, device=gpu), torch.zeros(B, dtype=torch.int32, device=gpu)
+        layers = [attn.KvCache(k[2 * i].clone(), k[2 * i + 1].clone(), table, length) for i in range(2)]
+        return layers, attn.KvPages.all_free(layers[0]), attn.KvPlan.empty(B, rows, gpu)
+
+    ws = torch.empty(attn.chunk_workspace_bytes(world()[0][0], rows, Hq), dtype=torch.uint8, device=gpu)
+    assert ws.numel() > 0
+
+    def step(layers, pages, plan):
+        attn.kv_plan(layers[0], pages, want, plan=plan)
+        outs = []
+        for i, c in enumerate(layers):
+            qkv = x[i].clone()
+            attn.kv_append_rows(qkv, c, Hq, plan, rope=r, q=qkv)
+            outs += [qkv, *attn.gqa_chunk(qkv, c, Hq, plan.row_start, plan.n_new, out=torch.zeros(rows, Hq * D, dtype=DT[dtype], device=gpu),
+                                          lse=torch.zeros(rows, Hq, device=gpu), workspace=ws)]
+        return outs
+
+    def state(w):
+        layers, pages, plan = w
+        return [layers[0].table, layers[0].kv_len, pages.free[:int(pages.n_free)], pages.n_free, pages.held, plan.n_new, plan.row_start, plan.seq, plan.pos,
+                plan.slot] + [t for c in layers for t in (c.k, c.v)]
+
+    step(*world())
+    worlds, graphs, outs = [world(), world()], [], []
+    for w in worlds:
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(*w))
+        graphs.append(g)
+    eager = world()
+    for i, n in enumerate([[60, 0, 30, 1, 0], [1, 50, 1, 1, 0], [0, 1, 1, 40, 1], [1, 1, 1, 1, 1], [20, 20, 20, 20, 20]]):
+        want.copy_(i32(n, gpu))
+        x.normal_()
+        ref = step(*eager)
+        torch.cuda.synchronize()
+        for w, g, out in zip(worlds, graphs, outs):
+            g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out + state(w), ref + state(eager)):
+                assert torch.equal(a, b), i
+    assert int(eager[2].row_start[-1]) == 80       # of 100 rows in a plan of 96
+
+
+def test_step_on_streams_of_their_own(gpu):
+    """Chunks of one cache on streams of their own at once, and a step on a stream that is not the current one."""
+    from tokamak_amd import attn
+    case = Case(gpu, [3000, 777, 2048], 4, 64, 64, "bf16")
+    n = i32([30, 9, 200], gpu)
+    start = i32([0, 30, 39], gpu)
+    qs = [queries(239, 16, 4, 64, "bf16", gpu, seed=s) for s in range(4)]
+    ref = [attn.gqa_chunk(q, case.cache, 16, start, n) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [attn.gqa_chunk(q, case.cache, 16, start, n, stream=s) for _ in range(4) for q, s in zip(qs, streams)]
+    torch.cuda.synchronize()
+    for i, (o, lse) in enumerate(got):
+        assert torch.equal(o, ref[i % 4][0]) and torch.equal(lse, ref[i % 4][1])
+    r, _ = rope_of(64, "halves", None)
+    small = Case(gpu, [0, 0], 4, 64, 64, "bf16", spare=8, extra_pages=4)
+    pages, x = attn.KvPages.all_free(small.cache), queries(50, 16, 4, 64, "bf16", gpu)
+    rot = attn.rope_fwd(x, r, 16, 4, 64, pos=torch.arange(50, dtype=torch.int32, device=gpu) % 30)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        plan = attn.kv_plan(small.cache, pages, i32([30, 20], gpu), rows=50)
+        q = attn.kv_append_rows(x, small.cache, 16, plan, rope=r)
+        o, lse = attn.gqa_chunk(q, small.cache, 16, plan.row_start, plan.n_new)
+    torch.cuda.synchronize()
+    assert torch.equal(q, rot[:, :16 * 64])
+    for b, at in ((0, slice(0, 30)), (1, slice(30, 50))):
+        small.k[b], small.v[b] = small.held(b)
+        assert torch.equal(small.k[b].transpose(0, 1).reshape(-1, 256), rot[at, 1024:1280].cpu().double())
+    check_chunk(small, [30, 20], [30, 20], q, o, lse, 16)
+
+
+def test_step_beyond_32_bit_offsets(gpu):
+    """A pool of 5 GB of K and as much of V, the sequences' pages at its end: the same results as from a small one."""
+    from tokamak_amd import attn
+    case = Case(gpu, [700, 90], 8, 128, 256, "bf16", weights=True, spare=4)
+    c, n = case.cache, 9600
+    shape = (n,) + tuple(c.k.shape[1:])
+    big = attn.KvCache(torch.empty(shape, dtype=c.dtype, device=gpu), torch.empty(shape, dtype=c.dtype, device=gpu),
+                       torch.where(c.table >= 0, c.table + (n - c.num_pages), c.table), c.kv_len.clone(), c.weight.clone())
+    assert big.k.numel() * 2 > 4 << 30
+    big.k[-c.num_pages:], big.v[-c.num_pages:] = c.k, c.v
+    r, _ = rope_of(128, "pairs", None)
+    for rows, want in ((3, [2, 1]), (1200, [40, 160])):
+        x, got = queries(rows, 16, 8, 128, "bf16", gpu), []
+        for one in (c, big):
+            held = i32([(int(m) + 255) // 256 for m in one.kv_len], gpu)
+            free = torch.zeros(one.num_pages, dtype=torch.int32, device=gpu)
+            used = one.table[one.table >= 0].tolist()
+            left = [p for p in range(one.num_pages - c.num_pages, one.num_pages) if p not in used]
+            free[:len(left)] = i32(left, gpu)
+            plan = attn.kv_plan(one, attn.KvPages(free, i32([len(left)], gpu), held), i32(want, gpu), rows=rows)
+            assert plan.n_new.tolist() == want
+            q = attn.kv_append_rows(x, one, 16, plan, rope=r)
+            o, lse = attn.gqa_chunk(q, one, 16, plan.row_start, plan.n_new)
+            total = sum(want)
+            got.append((q[:total], o[:total], lse[:total], one.weight, one.kv_len, *case.held(0, one), *case.held(1, one)))
+        for a, b in zip(*got):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,dtype,window", [(4, 1, 128, "bf16", 0), (2, 2, 64, "f16", 0), (4, 2, 64, "bf16", 40000)])
+def test_chunk_of_a_long_sequence(gpu, Hq, Hkv, D, dtype, window):
+    from tokamak_amd import attn
+    print(f"[case] long Hq{Hq} Hkv{Hkv} D{D} {dtype} window {window}", flush=True)
+    lens, n_new = [131085, 5], [13, 2]
+    case = Case(gpu, lens, Hkv, D, 256, dtype)
+    q = queries(15, Hq, Hkv, D, dtype, gpu)
+    o, lse = attn.gqa_chunk(q, case.cache, Hq, i32([0, 13], gpu), i32(n_new, gpu), window=window)
+    check_chunk(case, lens, n_new, q, o, lse, Hq, window=window)
+
+
+@pytest.mark.parametrize("layout,rot", [("halves", 64), ("halves", 40), ("halves", 18), ("halves", 126), ("pairs", 50)])
+@pytest.mark.parametrize("rows", [5, 3000])
+def test_rope_in_place_is_rope(gpu, layout, rot, rows):
+    """In place as into another tensor, where the other sides of a pair come from a thread's neighbours, in rows that are
+    further apart than they are long; the way back is the gradient's, up to two roundings."""
+    from tokamak_amd import attn
+    r = attn.Rope(rot, layout=layout)
+    x = queries(rows, 6, 2, 128, "bf16", gpu)
+    wide = torch.full((rows, 10 * 128 + 24), 3.0, dtype=torch.bfloat16, device=gpu)
+    wide[:, :1280] = x
+    y = attn.rope_fwd(x, r, 6, 2, 128, S=rows)
+    assert attn.rope_fwd(wide[:, :1280], r, 6, 2, 128, S=rows, out=wide[:, :1280]) is not None
+    assert torch.equal(wide[:, :1280], y) and (wide[:, 1280:] == 3.0).all()
+    back = attn.rope_bwd(y, r, 6, 2, 128, S=rows).float().cpu()
+    # a side is at most |x0| + |x1|, and so is the sum of both; each rounding is of that times 2^-8, twice and once more
+    x = x.float().cpu()
+    heads = x.reshape(rows, 10, 128)
+    i = torch.arange(rot // 2)
+    i0, i1 = (i, i + rot // 2) if layout == "halves" else (2 * i, 2 * i + 1)
+    size = torch.zeros_like(heads)
+    size[:, :8, i0] = size[:, :8, i1] = heads[:, :8, i0].abs() + heads[:, :8, i1].abs()
+    assert ((back - x).abs() <= (2.0 ** -8 * 3.1 * size).reshape(x.shape)).all()
+
+
+def test_the_binding_refuses(gpu):
+    from tokamak_amd import attn
+    case = Case(gpu, [5, 9], 1, 64, 64, "f16", spare=6, extra_pages=3)
+    c, dt = case.cache, torch.int32
+    n = c.num_pages
+
+    def z(*shape, d=dt):
+        return torch.zeros(*shape, dtype=d, device=gpu)
+
+    for args in ((z(n, d=torch.int64), z(1), z(2)), (z(n), z(2), z(2)), (z(n), z(1), z(2, d=torch.int64))):
+        with pytest.raises(ValueError, match="dtype|elements"):
+            attn.KvPages(*args)
+    slot = z(4, d=torch.int64)
+    for args in ((z(2), z(2), z(4), z(4), slot), (z(2), z(3), z(3), z(4), slot), (z(2), z(3), z(4), z(5), slot), (z(2), z(3), z(4), z(4), z(4))):
+        with pytest.raises(ValueError, match="dtype|elements"):
+            attn.KvPlan(*args)
+    plan, pages, want = attn.KvPlan.empty(2, 4, gpu), attn.KvPages.all_free(c), z(2)
+    for pg, kw, match in ((pages, {}, "how many"), (pages, dict(rows=3, plan=plan), "4 rows"), (attn.KvPages(z(n), z(1), z(3)), dict(plan=plan), "2 sequences"),
+                          (attn.KvPages(z(n - 1), z(1), z(2)), dict(plan=plan), "pages"), (pages, dict(plan=attn.KvPlan.empty(3, 4, gpu)), "2 sequences"),
+                          (pages, dict(plan=plan, start=z(3)), "start")):
+        with pytest.raises(ValueError, match=match):
+            attn.kv_plan(c, pg, want, **kw)
+    with pytest.raises(ValueError, match="want"):
+        attn.kv_plan(c, pages, z(2, d=torch.int64), plan=plan)
+    x = z(4, 3 * 64, d=torch.float16)
+    for bad, match in ((x[:3], "plan must be"), (x[:, :128], "192"), (x.float(), "float16"), (z(192, 4, d=torch.float16).t(), "contiguous")):
+        with pytest.raises(ValueError, match=match):
+            attn.kv_append_rows(bad, c, 1, plan)
+    with pytest.raises(ValueError, match="rows, expected"):
+        attn.kv_append_rows(x, c, 1, plan, q=x[:2])
+    for q, kw, match in ((x[0], {}, "rows"), (x, dict(row_start=z(1), n_new=z(2)), "row_start"), (x, dict(n_new=z(3)), "n_new"),
+                         (x, dict(out=z(4, 128, d=torch.float16)), "out"), (x, dict(lse=z(4, d=torch.float16)), "lse"),
+                         (x, dict(workspace=z(3, 2, d=torch.uint8).t()), "workspace")):
+        with pytest.raises(ValueError, match=match):
+            attn.gqa_chunk(q, c, 1, **kw)
+    r = attn.Rope(64)
+    for bad, kw, match in ((x, {}, "positions"), (x[:, :64], dict(S=4), "192"), (x, dict(pos=z(3)), "pos"), (x, dict(S=4, out=x[:3]), "rows, expected"),
+                           (x, dict(pos=z(4, d=torch.int64)), "pos")):
+        with pytest.raises(ValueError, match=match):
+            attn.rope_fwd(bad, r, 1, 1, 64, **kw)
+    assert case.held(0)[0].shape[1] == 5 and c.kv_len.tolist() == [5, 9]
