@@ -670,3 +670,18 @@ def test_the_binding_refuses(gpu):
         with pytest.raises(ValueError, match=match):
             attn.rope_fwd(bad, r, 1, 1, 64, **kw)
     assert case.held(0)[0].shape[1] == 5 and c.kv_len.tolist() == [5, 9]
+
+
+@pytest.mark.parametrize("B,extra,dtype", [(1100, 20, "f16"), (2300, 40, "bf16")])
+def test_chunk_of_many_sequences(gpu, B, extra, dtype):
+    """More sequences, and items, than a workgroup has threads."""
+    from tokamak_amd import attn
+    print(f"[case] {B} sequences", flush=True)
+    lens, n_new = [(7 * i) % 50 + 2 for i in range(B)], [i % 3 for i in range(B)]
+    lens[B - 1], n_new[B - 1] = 900, 300
+    case = Case(gpu, lens, 1, 64, 64, dtype, extra_pages=extra)
+    q = queries(sum(n_new), 2, 1, 64, dtype, gpu)
+    row_start = [sum(n_new[:b]) for b in range(B + 1)]
+    for window in (0, 20):
+        o, lse = attn.gqa_chunk(q, case.cache, 2, i32(row_start, gpu), i32(n_new, gpu), window=window)
+        check_chunk(case, lens, n_new, q, o, lse, 2, window=window)
