@@ -685,3 +685,20 @@ def test_chunk_of_many_sequences(gpu, B, extra, dtype):
     for window in (0, 20):
         o, lse = attn.gqa_chunk(q, case.cache, 2, i32(row_start, gpu), i32(n_new, gpu), window=window)
         check_chunk(case, lens, n_new, q, o, lse, 2, window=window)
+
+
+def test_chunk_of_rows_that_sequences_share(gpu):
+    """Rows that several sequences name, which the call does not promise anything of, leave what is beside o, lse and the
+    workspace alone."""
+    from tokamak_amd import attn
+    case = Case(gpu, [310] * 60, 2, 64, 64, "f16", extra_pages=20)
+    q = queries(300, 4, 2, 64, "f16", gpu)
+    need = attn.chunk_workspace_bytes(case.cache, 300, 4)
+    assert need > 0
+    ws = torch.full((need + 8192,), 0x5a, dtype=torch.uint8, device=gpu)
+    out, lse = torch.full((340, 256), 4.0, dtype=torch.float16, device=gpu), torch.full((340, 4), 4.0, device=gpu)
+    attn.gqa_chunk(q, case.cache, 4, i32([0] * 60, gpu), i32([300] * 60, gpu), out=out[20:320], lse=lse[20:320], workspace=ws[4096:4096 + need])
+    assert (ws[:4096] == 0x5a).all() and (ws[4096 + need:] == 0x5a).all()
+    for t in (out, lse):
+        assert (t[:20] == 4.0).all() and (t[320:] == 4.0).all()
+    assert torch.isfinite(out).all()

@@ -538,10 +538,11 @@ def _rope(x, rope, Hq, Hkv, D, pos, S, out, inverse, st):
     else:
         _check_dtype("pos", pos, rows, dev, "int32")
     if out is None:
-        out = x.new_empty(x.shape)
-    n, ostride = _rows_of("out", out, width, dev, x.dtype)
-    if n != rows:
-        raise ValueError(f"out has {n} rows, expected {rows}")
+        out, ostride = x.new_empty(x.shape), width
+    else:
+        n, ostride = _rows_of("out", out, width, dev, x.dtype)
+        if n != rows:
+            raise ValueError(f"out has {n} rows, expected {rows}")
     _check("tkm_attn_rope_rows", lib().tkm_attn_rope_rows(rope._ref, x.data_ptr(), stride, out.data_ptr(), ostride, _ptr(pos),
                                                           1 if S is None else S, rows, Hq, Hkv, D, dt, inverse, st))
     return out

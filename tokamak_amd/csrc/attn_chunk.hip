@@ -73,12 +73,13 @@ struct C {   // kernel arguments
     float* lse;
     Start* starts;     // of the workers
     Joint* joints;     // n is 0 behind the last
-    Item* items;       // of a kv head
+    Item* items;       // of a kv head, up to `most`
     float* part;       // pieces: [slot][BM][D] unnormalised O, then [slot][BM] (m, l)
     float2* part_ml;
     long long q_stride;
     int B, Hkv, G, num_pages, page_shift, max_pages, cap, rows, causal, window;
     int workers;       // 0: a workgroup an item
+    int most;          // items that the rows can make, if no two sequences have one of them; more are passed over
     float sl2;         // scale * log2(e)
 };
 
@@ -149,7 +150,8 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
         const int b = c + threadIdx.x;
         const int rows = b < a.B ? seq_of(a, b).n * a.G : 0;
         int64_t all, sum;
-        lds.end[threadIdx.x] = (int)lds.sum(0, (rows + BM - 1) / BM, all);
+        lds.end[threadIdx.x] = (int)min(lds.sum(0, (rows + BM - 1) / BM, all), (int64_t)INT_MAX);
+        all = min(all, a.most - items);
         __syncthreads();
         for (int64_t k0 = 0; k0 < all; k0 += TL) {
             const int k = (int)k0 + threadIdx.x;
@@ -698,7 +700,7 @@ int launch_chunk(const ChunkArgs& x) {
     const C a{(const uint16_t*)kv.k, (const uint16_t*)kv.v, kv.table, kv.len, (const uint16_t*)x.q, x.row_start, x.n_new,
               (uint16_t*)x.o, x.lse, (Start*)ws, (Joint*)(ws + p.joints), (Item*)(ws + p.items), (float*)(ws + p.part),
               (float2*)(ws + p.ml), x.q_stride, kv.B, kv.Hkv, x.Hq / kv.Hkv, kv.num_pages, __builtin_ctz(kv.page), kv.max_pages,
-              kv.max_pages * kv.page, x.rows, x.causal, x.window, workers, x.scale * 1.4426950408889634f};
+              kv.max_pages * kv.page, x.rows, x.causal, x.window, workers, (int)items_most(kv, x.rows, x.Hq), x.scale * 1.4426950408889634f};
     note_kernels(kChunk | (joints > 0 ? kJoin : 0));
     const dim3 grid = workers ? dim3(workers) : dim3(items_each(kv, x.rows, x.Hq), kv.B, kv.Hkv);
     const hipStream_t stream = (hipStream_t)x.stream;
