@@ -48,9 +48,11 @@ constexpr float kLift = 8.0f;
 constexpr float kSumMax = 65504.0f;
 constexpr float kLn2 = 0.69314718055994531f;
 
-// An item of a kv head: tile t of sequence b's rows, and the tiles of tokens before it in the head's line.
+// An item of a kv head: rows [r0, rows) of sequence b, up to BM of them, which begins at row row0 of the call and at
+// position pos of len; the tiles [x, y) of tokens that they see, of which all see [alike, alike_end) whole; and its
+// place in the head's line.
 struct Item {
-    int b, t;
+    int b, r0, row0, rows, pos, len, x, y, alike, alike_end;
     int64_t at;
 };
 // Where a worker's share begins: tile `tile` of item e of kv head h, and the tiles that are its; a kv head has `items`.
@@ -78,6 +80,9 @@ struct C {   // kernel arguments
     float2* part_ml;
     long long q_stride;
     int B, Hkv, G, num_pages, page_shift, max_pages, cap, rows, causal, window;
+    uint32_t per_g;    // a number is divided by G by this and a shift
+    int g_shift;
+    int each;          // rows of a sequence where n_new is NULL
     int workers;       // 0: a workgroup an item
     int most;          // items that the rows can make, if no two sequences have one of them; more are passed over
     float sl2;         // scale * log2(e)
@@ -90,7 +95,7 @@ __device__ __forceinline__ int fixed(const int32_t* p, long long i) {
 }
 __device__ __forceinline__ Item fixed_item(const Item* p) {
     const auto* q = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
-    return Item{q[0], q[1], 0};
+    return Item{q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7], q[8], q[9], 0};
 }
 __device__ __forceinline__ Start fixed_start(const Start* p) {
     const auto* q = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
@@ -115,25 +120,35 @@ __device__ __forceinline__ Seq seq_of(const C& a, int b) {
         else return p[b];
     };
     Seq s;
-    const int each = a.rows / a.B;
-    s.row0 = a.row_start ? get(a.row_start) : b * each;
-    const int n = a.n_new ? get(a.n_new) : each;
+    s.row0 = a.row_start ? get(a.row_start) : b * a.each;
+    const int n = a.n_new ? get(a.n_new) : a.each;
     s.len = get(a.len);
     if ((unsigned)s.len > (unsigned)a.cap) s.len = -1;
     s.n = s.row0 < 0 || s.row0 >= a.rows ? 0 : max(0, min(n, a.rows - s.row0));
     s.pos = s.len - max(n, 0);       // above -2^31: neither is below -1, nor n above 2^31 - 1
     return s;
 }
-// The positions that the row of token i sees: [lo, hi).
-__device__ __forceinline__ int2 seen_by(const C& a, const Seq& s, int i) {
-    if (!a.causal) return int2{0, max(s.len, 0)};
-    const int p = s.pos + i;
-    return int2{a.window ? max(0, p - a.window + 1) : 0, max(0, min(p + 1, s.len))};
+// r / G of r in [0, 2^31): per_g is ceil(2^(31 + g_shift) / G) with 2^g_shift >= G, so G per_g exceeds the power by less
+// than G, and r per_g / 2^(31 + g_shift) exceeds r / G by less than 1 / G.
+__device__ __forceinline__ int over_g(const C& a, int r) { return (int)(__umulhi(2u * (uint32_t)r, a.per_g) >> a.g_shift); }
+
+// The positions that the row of token i sees, of a sequence whose first is at pos of len: [lo, hi).
+__device__ __forceinline__ int2 seen_by(const C& a, int pos, int len, int i) {
+    if (!a.causal) return int2{0, max(len, 0)};
+    const int p = pos + i;
+    return int2{a.window ? max(0, p - a.window + 1) : 0, max(0, min(p + 1, len))};
 }
-// The tiles [x, y) of tokens that rows [first, last] see.
-__device__ __forceinline__ int2 tiles_of(const C& a, const Seq& s, int first, int last) {
-    const int lo = seen_by(a, s, first / a.G).x, hi = seen_by(a, s, last / a.G).y;
-    return lo < hi ? int2{lo / BN, (hi + BN - 1) / BN} : int2{0, 0};
+// Item t of a sequence.
+__device__ __forceinline__ Item item_of(const C& a, const Seq& s, int b, int t) {
+    Item e{b, t * BM, s.row0, s.n * a.G, s.pos, s.len, 0, 0, 0, 0, 0};
+    const int2 first = seen_by(a, s.pos, s.len, over_g(a, e.r0)), last = seen_by(a, s.pos, s.len, over_g(a, max(min(e.r0 + BM, e.rows) - 1, 0)));
+    if (first.x < last.y) {
+        e.x = first.x / BN;
+        e.y = (last.y + BN - 1) / BN;
+    }
+    e.alike = (last.x + BN - 1) / BN;
+    e.alike_end = first.y / BN;
+    return e;
 }
 
 constexpr int TL = 1024;
@@ -155,15 +170,13 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
         __syncthreads();
         for (int64_t k0 = 0; k0 < all; k0 += TL) {
             const int k = (int)k0 + threadIdx.x;
-            Item e{0, 0, 0};
+            Item e{};
             int tiles = 0;
             if (k < all) {
                 const int i = first_above(lds.end, TL, k);
-                e.b = c + i;
-                e.t = k - (i ? lds.end[i - 1] : 0);
-                const Seq q = seq_of(a, e.b);
-                const int2 x = tiles_of(a, q, e.t * BM, min((e.t + 1) * BM, q.n * a.G) - 1);
-                tiles = max(1, x.y - x.x);       // an item that sees nothing still has outputs
+                const int b = c + i;
+                e = item_of(a, seq_of(a, b), b, k - (i ? lds.end[i - 1] : 0));
+                tiles = max(1, e.y - e.x);       // an item that sees nothing still has outputs
             }
             e.at = before + lds.sum(1, tiles, sum) - tiles;
             if (k < all) {
@@ -198,11 +211,10 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
             if (st.tile > 0 && st.tile <= each) {     // the first share that begins inside the item
                 const Item it = a.items[lo];
                 const int64_t left = (lo + 1 < items ? begin(lo + 1) : before) - at;
-                const Seq s = seq_of(a, it.b);
                 j.h = st.h;
-                j.row0 = s.row0;
-                j.r0 = it.t * BM;
-                j.rows = min(s.n * a.G - j.r0, BM);
+                j.row0 = it.row0;
+                j.r0 = it.r0;
+                j.rows = min(it.rows - it.r0, BM);
                 j.n = 1 + (int)div_up(left, each);
             }
         }
@@ -217,7 +229,8 @@ __global__ __launch_bounds__(TL) void chunk_items_kernel(C a) {
 
 // Row r of an item: its row of o and lse, and its head.
 __device__ __forceinline__ long long out_row(const C& a, int row0, int h, int r) {
-    return ((long long)(row0 + r / a.G) * a.Hkv + h) * a.G + r % a.G;
+    const int i = over_g(a, r);
+    return ((long long)(row0 + i) * a.Hkv + h) * a.G + (r - i * a.G);
 }
 
 // The arguments of the kernel that runs, read where they are used: those of its whole life would not fit into the scalar
@@ -274,14 +287,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     do {
         // ---- the item, and this workgroup's share of its tiles
         const C& a = arguments();
-        const Item it = workers ? fixed_item(&a.items[e]) : Item{(int)blockIdx.y, (int)blockIdx.x, 0};
-        const Seq s = seq_of<true>(a, it.b);
-        const int R = s.n * a.G, r0 = it.t * BM;
+        const Item it = workers ? fixed_item(&a.items[e]) : item_of(a, seq_of<true>(a, blockIdx.y), blockIdx.y, blockIdx.x);
+        const int R = it.rows, r0 = it.r0;
         if (r0 >= R) return;              // a workgroup an item: the sequence has fewer
-        const int2 tiles = tiles_of(a, s, r0, min(r0 + BM, R) - 1);
-        const int all = max(1, tiles.y - tiles.x);
+        const int all = max(1, it.y - it.x);
         if (!workers) left = all;
-        const int mine = (int)min(left, (int64_t)(all - from)), ta = tiles.x + from, te = min(ta + mine, tiles.y);
+        const int mine = (int)min(left, (int64_t)(all - from)), ta = it.x + from, te = min(ta + mine, it.y);
         const bool whole = mine == all;
 
         // this lane's row; those behind the sequence's rows act as its last
@@ -289,21 +300,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         const bool valid = r < R;
         const int first = r0 + wave * 32, final = min(first + 31, R - 1);
         const bool active = first < R;
-        const int2 seen = seen_by(a, s, min(r, max(R - 1, 0)) / a.G);
+        const int2 seen = seen_by(a, it.pos, it.len, over_g(a, min(r, R - 1)));
         // tiles in [p0, p1) need no mask in this wave, those in [n0, n1) hold a token that one of its rows sees
         int p0 = 0, p1 = 0, n0 = 0, n1 = 0;
         if (active) {
-            const int2 x = seen_by(a, s, first / a.G), y = seen_by(a, s, final / a.G);
+            const int2 x = seen_by(a, it.pos, it.len, over_g(a, first)), y = seen_by(a, it.pos, it.len, over_g(a, final));
             p0 = (y.x + BN - 1) / BN;
             p1 = x.y / BN;
             n0 = x.x / BN;
             n1 = (y.y + BN - 1) / BN;
         }
-        // tiles in [alike.x, alike.y) are seen whole by all rows of the item
-        const int2 alike{(seen_by(a, s, (min(r0 + BM, R) - 1) / a.G).x + BN - 1) / BN, seen_by(a, s, r0 / a.G).y / BN};
         u32x4 qf[KS];
         {
-            const uint16_t* qp = a.q + (s.row0 + r / a.G) * a.q_stride + (long long)(h * a.G + r % a.G) * D + hi * 8;
+            const int i = over_g(a, r);
+            const uint16_t* qp = a.q + (it.row0 + i) * a.q_stride + (long long)(h * a.G + (r - i * a.G)) * D + hi * 8;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) qf[ks] = valid ? ld_global16(qp + ks * 16) : u32x4{0u, 0u, 0u, 0u};
         }
@@ -311,7 +321,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 #pragma unroll
         for (int db = 0; db < NDB; ++db) o[db] = f32x16{};
         float m = -INFINITY, lsum = 0.f;     // m less the lift, log2 units
-        bool bad = s.len < 0;
+        bool bad = it.len < 0;
 
         // pages of a tile's halves, fetched a tile ahead
         const int half_bits = a.page_shift - 5, last_page = a.max_pages - 1, num_pages = a.num_pages, Hkv = a.Hkv;
@@ -335,7 +345,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                     bad |= from < seen.y && from + 32 > seen.x;
                 }
             }
-            if (t * BN + my_half * 32 < s.len) {
+            if (t * BN + my_half * 32 < it.len) {
                 const int half = t * 2 + my_half;
                 const long long sub = (((long long)(my_half ? page[1] : page[0]) * Hkv + h) << half_bits) + (half & ((1 << half_bits) - 1));
                 dma16_rows(make_rsrc(keys + sub * HALF, HALF), dma_at + (uint32_t)(buf * TILE), dma_v);
@@ -345,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         // Values of tokens behind the sequence's last become 0, for what is there may be anything, and infinities and
         // NaN, whose bits are left in `odds`.  True if there were any of these.
         auto search = [&](int t, int buf) {
-            const int left = s.len - t * BN;
+            const int left = it.len - t * BN;
             bool any = false;
             for (int i = threadIdx.x; i < 2 * D; i += 64 * kWaves) {         // rows of 32 tokens of one dim
                 char* row = smem[1][buf] + i * 64;
@@ -491,7 +501,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         __syncthreads();
         auto step = [&](int t, auto Buf) __attribute__((always_inline)) {
             const int buf = Buf;
-            const bool odd = (t < alike.x || t >= alike.y) && search(t, buf);
+            const bool odd = (t < it.alike || t >= it.alike_end) && search(t, buf);
             if (t + 1 < te) {
                 issue(t + 1, buf ^ 1);
                 if (t + 2 < te) fetch(t + 2);
@@ -518,7 +528,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         if (bad) l = NAN;
         if (whole) {
             if (valid) {
-                const long long row = out_row(z, s.row0, h, r);
+                const long long row = out_row(z, it.row0, h, r);
                 const float inv = l == 0.f ? 0.f : 1.0f / l;
                 uint16_t* orow = z.o + row * D;
 #pragma unroll
@@ -697,10 +707,14 @@ int launch_chunk(const ChunkArgs& x) {
     const int workers = workers_of(kv, x.rows, x.Hq), joints = joints_of(kv, x.rows, x.Hq);
     char* ws = (char*)x.ws;
     const Place p = places(kv, x.rows, x.Hq);
+    const int G = x.Hq / kv.Hkv;
+    int shift = 0;
+    while (1u << shift < (unsigned)G) ++shift;
+    const uint32_t per_g = (uint32_t)(((1ull << (31 + shift)) + G - 1) / G);
     const C a{(const uint16_t*)kv.k, (const uint16_t*)kv.v, kv.table, kv.len, (const uint16_t*)x.q, x.row_start, x.n_new,
               (uint16_t*)x.o, x.lse, (Start*)ws, (Joint*)(ws + p.joints), (Item*)(ws + p.items), (float*)(ws + p.part),
               (float2*)(ws + p.ml), x.q_stride, kv.B, kv.Hkv, x.Hq / kv.Hkv, kv.num_pages, __builtin_ctz(kv.page), kv.max_pages,
-              kv.max_pages * kv.page, x.rows, x.causal, x.window, workers, (int)items_most(kv, x.rows, x.Hq), x.scale * 1.4426950408889634f};
+              kv.max_pages * kv.page, x.rows, x.causal, x.window, per_g, shift, x.rows / kv.B, workers, (int)items_most(kv, x.rows, x.Hq), x.scale * 1.4426950408889634f};
     note_kernels(kChunk | (joints > 0 ? kJoin : 0));
     const dim3 grid = workers ? dim3(workers) : dim3(items_each(kv, x.rows, x.Hq), kv.B, kv.Hkv);
     const hipStream_t stream = (hipStream_t)x.stream;
