@@ -702,3 +702,18 @@ def test_chunk_of_rows_that_sequences_share(gpu):
     for t in (out, lse):
         assert (t[:20] == 4.0).all() and (t[320:] == 4.0).all()
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("lens,n_new,Hq,Hkv,D,page,dtype,window", [
+    ([1900, 700], [1900, 200], 32, 4, 64, 64, "bf16", 0), ([1000, 33, 0, 900, 1000], [1000, 1, 0, 500, 900], 16, 16, 128, 32, "f16", 0),
+    ([5000, 3000, 64], [1200, 900, 3], 16, 2, 64, 128, "bf16", 300), ([2500, 1300], [1250, 1300], 24, 24, 64, 64, "f16", 1000)])
+def test_chunk_of_many_rows_in_one_launch(gpu, lens, n_new, Hq, Hkv, D, page, dtype, window):
+    """Prompts whose items are workgroups enough, and short enough, that none is split."""
+    from tokamak_amd import attn
+    print(f"[case] {lens} Hq{Hq} Hkv{Hkv} D{D} {dtype} window {window}", flush=True)
+    case = Case(gpu, lens, Hkv, D, page, dtype)
+    q = queries(sum(n_new), Hq, Hkv, D, dtype, gpu)
+    row_start = [sum(n_new[:b]) for b in range(len(lens) + 1)]
+    o, lse = attn.gqa_chunk(q, case.cache, Hq, i32(row_start, gpu), i32(n_new, gpu), window=window)
+    assert attn.last_kernels() == ["chunk"]
+    check_chunk(case, lens, n_new, q, o, lse, Hq, window=window)

@@ -645,13 +645,24 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(C a, int each) {
 long long items_each(const tkm_attn_kv& kv, int rows, int Hq) { return ((long long)rows * (Hq / kv.Hkv) + BM - 1) / BM; }
 long long items_most(const tkm_attn_kv& kv, int rows, int Hq) { return items_each(kv, rows, Hq) + std::min<long long>(kv.B, rows); }
 
-// A workgroup an item, where none has more than 16 tiles and the grid, which is laid out for all rows being one
-// sequence's, is not much larger than the card.
-constexpr long long kFewTokens = 1024, kFewItems = 1024;
+// A workgroup an item, in one launch, of a grid laid out for all rows being one sequence's:
+//   where no item has more than 10 tiles, which take a lone workgroup about 1.4 us each (kernels, one launch or three: 4
+//     times 5 rows over up to 300 tokens 12 and 16 us, 500 15 and 16, 900 24 and 16);
+//   where full items are workgroups enough for the card and the longest, by the table or the window, has a 16th as
+//     many tiles, and at most 32 (32 heads of 128, 4 prompts of up to 500 tokens 33 and 52 us, 1000 78 and 99, 1900 194
+//     and 216; 12 heads of 64, 5 prompts in windows of 256 36 and 53, 1024 68 and 76, 2048 110 and 109; but 64 rows
+//     over up to 990 57 and 45).
+constexpr long long kFewTiles = 10, kFewItems = 1024, kMoreTiles = 32, kMoreItems = 16384, kFill = 16;
 
-// The workers of a split call; 0 for the other.
+bool item_each(const tkm_attn_kv& kv, int rows, int Hq, int window) {
+    const long long G = Hq / kv.Hkv, table = (long long)kv.max_pages * kv.page, seen = window + (BM + G - 1) / G + BN;
+    const long long tiles = (std::min(table, window ? seen : table) + BN - 1) / BN, grid = items_each(kv, rows, Hq) * kv.B;
+    return (tiles <= kFewTiles && grid <= kFewItems / kv.Hkv) ||
+           (tiles <= kMoreTiles && grid <= kMoreItems / kv.Hkv && tiles * kFill <= (long long)rows * Hq / BM);
+}
+
+// The workers of a split call.
 int workers_of(const tkm_attn_kv& kv, int rows, int Hq) {
-    if ((long long)kv.max_pages * kv.page <= kFewTokens && items_each(kv, rows, Hq) * kv.B <= kFewItems / kv.Hkv) return 0;
     const double tiles = (double)items_most(kv, rows, Hq) * kv.Hkv * (kv.max_pages * (double)kv.page / BN + 1);
     return (int)std::max(std::min(tiles, (double)workers_at(kv.D)), 1.0);
 }
@@ -699,12 +710,13 @@ bool chunk_fits(const tkm_attn_kv& kv, int rows, int Hq) {
 }
 
 size_t chunk_workspace(const tkm_attn_kv& kv, int rows, int Hq) {
-    return workers_of(kv, rows, Hq) ? places(kv, rows, Hq).end : 0;
+    return item_each(kv, rows, Hq, 0) ? 0 : places(kv, rows, Hq).end;      // a window only ever saves it
 }
 
 int launch_chunk(const ChunkArgs& x) {
     const tkm_attn_kv& kv = x.kv;
-    const int workers = workers_of(kv, x.rows, x.Hq), joints = joints_of(kv, x.rows, x.Hq);
+    const bool split = !item_each(kv, x.rows, x.Hq, x.window);
+    const int workers = split ? workers_of(kv, x.rows, x.Hq) : 0, joints = split ? joints_of(kv, x.rows, x.Hq) : 0;
     char* ws = (char*)x.ws;
     const Place p = places(kv, x.rows, x.Hq);
     const int G = x.Hq / kv.Hkv;
