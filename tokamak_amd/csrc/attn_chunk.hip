@@ -20,8 +20,13 @@
 // Splitting: all items' tiles are numbered in one line, kv head after kv head, and every workgroup takes an equal
 // share, whatever the lengths are, which are read on the device: a first launch of one workgroup lists the items of a
 // kv head, the place where each share begins, and the items that no one workgroup has whole.  These leave pieces in
-// the workspace, which a third launch joins in the order of the tokens: results do not depend on timing.  Where the
-// tables hold few tokens a workgroup has an item, and there is one launch.
+// the workspace, which a third launch joins in the order of the tokens: results do not depend on timing.  Where items
+// are short, or fill the card, a workgroup has one, and there is one launch.  (Shares weighted by what a tile has of
+// rows were slower: on a full card a tile takes 2 us, be it one row's, from HBM, or 128 rows', whose keys are in L2.)
+//
+// What bounds it: for few rows HBM (13 tokens, 32 heads of 128 on 8, about 131000: 101 us for 537 MB, 5.3 TB/s; listing and
+// joining 15 more); for prompts of 128 dims the power that products draw (1.6 GHz; 707 GFLOP seen, 854 done in tiles, in
+// 960 us); at 64 dims the issue of exponentials and sums, three waves a SIMD, and a part's beginning and end.
 //
 // 0 times an infinity or NaN is NaN, also where P is 0 because its row does not see the token.  So a tile that an item's
 // rows do not see alike is searched for such values in LDS; they become 0 there, and a bit each, by which they are
@@ -43,7 +48,8 @@ namespace {
 constexpr int BM = 128;           // rows of an item
 constexpr int BN = 64;            // tokens of a tile
 constexpr int kWaves = 4;
-constexpr int workers_at(int D) { return D == 64 ? 768 : 512; }     // three or two workgroups on each compute unit
+// Three or two workgroups on each compute unit (5 prompts in windows of 1024, 12 heads of 64: 63 and 71 us).
+constexpr int workers_at(int D) { return D == 64 ? 768 : 512; }
 constexpr float kLift = 8.0f;
 constexpr float kSumMax = 65504.0f;
 constexpr float kLn2 = 0.69314718055994531f;

@@ -133,7 +133,8 @@ __global__ __launch_bounds__(256) void slots_kernel(PlanArgs a) {
     put_row(a, r, b, a.kv.len[b] - (end[b] - r));
 }
 
-// Rows up to which the planning workgroup lays them out itself.
+// Rows up to which the planning workgroup lays them out itself, in one launch (kernels, one launch and two: 64 rows 6.0 and
+// 7.1 us, 3000 7.8 and 8.3, 6000 9.7 and 8.3, 12500 14.2 and 8.2).
 constexpr int kOwnRows = 4096;
 
 }  // namespace

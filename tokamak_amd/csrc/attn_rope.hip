@@ -8,7 +8,10 @@
 //
 // Both kernels move data and are bound by HBM, or by the launch where rows are few.  A thread has a chunk of 8 dims, 16
 // bytes, of one head at a time, and forms its side of the pairs; a head's chunks are one wave's, at one time, which
-// reads the other sides before it writes, so that rows may be rotated in place.
+// reads the other sides before it writes, so that rows may be rotated in place.  (With a pair's sides in one thread, stores
+// were as wide as the largest power of two in rot / 2: 16384 rows of 40 heads of 64 with 40 dims rotated took 41 us for
+// 27.)  A training batch of 8192 rows of 48 heads of 128: 45 us of operands from HBM, 4.4 TB/s; 7600 prompt rows of 28 heads
+// of 128 into the cache: 52 us, 4.4 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "attn_common.h"
@@ -225,11 +228,13 @@ __global__ __launch_bounds__(kThreads) void store_rows_kernel(StoreK a) {
     }
 }
 
-// Rows up to which one has a whole workgroup.
-constexpr int kFewRows = 1024;
-int threads_a_row(int rows) { return rows <= kFewRows ? kThreads : 64; }
-unsigned row_blocks(int rows) {
-    const unsigned each = kThreads / threads_a_row(rows);
+// Rows up to which one has a whole workgroup, else a wave (32 + 2 * 8 heads of 128, kernels, workgroup and wave: rotation of
+// 64 rows 4.7 and 8.0 us, 1024 7.5 and 9.3, 2048 10.4 and 12.6, 4096 17 and 17; into the cache, where the many have V in
+// tiles of 32 rows, 64 rows 6.7 and 9.6, 256 8.9 and 11.8, 450 10.8 and 10.1, 900 15.5 and 11.4).
+constexpr int kFewTurned = 4096, kFewStored = 400;
+int threads_a_row(int rows, int few) { return rows <= few ? kThreads : 64; }
+unsigned row_blocks(int rows, int few) {
+    const unsigned each = kThreads / threads_a_row(rows, few);
     return ((unsigned)rows + each - 1) / each;
 }
 
@@ -257,17 +262,17 @@ void pick(int dtype, const tkm_attn_rope& r, const A& a, F launch) {
 }  // namespace
 
 bool rows_fit(const tkm_attn_kv* kv, int rows) {
-    double blocks = row_blocks(rows);
+    double blocks = row_blocks(rows, kv ? kFewStored : kFewTurned);
     if (kv) blocks += (rows + 31.0) / 32.0 * kv->Hkv;
     return launch_fits(blocks, kThreads);
 }
 
 int launch_rope(const RopeArgs& a) {
     RopeK k{a.rope, (const uint16_t*)a.in, (uint16_t*)a.out, a.pos, a.in_stride, a.out_stride, a.S, a.rows, a.Hq + a.Hkv,
-            a.Hq + 2 * a.Hkv, a.D, threads_a_row(a.rows), a.inverse ? -1.0f : 1.0f};
+            a.Hq + 2 * a.Hkv, a.D, threads_a_row(a.rows, kFewTurned), a.inverse ? -1.0f : 1.0f};
     note_kernels(kRope);
     pick(a.dtype, a.rope, k, [&](auto DT, auto L, auto V) {
-        hipLaunchKernelGGL((rope_kernel<decltype(DT)::value, decltype(L)::value, decltype(V)::value>), dim3(row_blocks(a.rows)),
+        hipLaunchKernelGGL((rope_kernel<decltype(DT)::value, decltype(L)::value, decltype(V)::value>), dim3(row_blocks(a.rows, kFewTurned)),
                            dim3(kThreads), 0, (hipStream_t)a.stream, k);
     });
     return hipGetLastError() == hipSuccess ? 0 : -1;
@@ -275,7 +280,7 @@ int launch_rope(const RopeArgs& a) {
 
 int launch_store(const StoreArgs& a) {
     StoreK k{a.kv, {}, (const uint16_t*)a.qkv, (uint16_t*)a.q, a.seq, a.pos, a.slot, a.stride, a.q_stride, a.rows, a.Hq,
-             threads_a_row(a.rows), (int)row_blocks(a.rows)};
+             threads_a_row(a.rows, kFewStored), (int)row_blocks(a.rows, kFewStored)};
     if (a.rope) k.rope = *a.rope;
     else if (a.q == a.qkv) k.q = nullptr;       // Q stays as it is
     const int tiles = k.T == kThreads ? 0 : (a.rows + 31) / 32 * a.kv.Hkv;
