@@ -25,8 +25,8 @@
 // rows were slower: on a full card a tile takes 2 us, be it one row's, from HBM, or 128 rows', whose keys are in L2.)
 //
 // What bounds it: for few rows HBM (13 tokens, 32 heads of 128 on 8, about 131000: 101 us for 537 MB, 5.3 TB/s; listing and
-// joining 15 more); for prompts of 128 dims the power that products draw (1.6 GHz; 707 GFLOP seen, 854 done in tiles, in
-// 960 us); at 64 dims the issue of exponentials and sums, three waves a SIMD, and a part's beginning and end.
+// joining 15 more); for prompts of 128 dims products and exponentials one after the other (46 and 36% of the clocks at 1.86
+// GHz; 707 GFLOP seen, 854 done in tiles, in 940 us); at 64 dims the issue of exponentials and sums, three waves a SIMD, and a part's beginning and end.
 //
 // 0 times an infinity or NaN is NaN, also where P is 0 because its row does not see the token.  So a tile that an item's
 // rows do not see alike is searched for such values in LDS; they become 0 there, and a bit each, by which they are
@@ -425,6 +425,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                 }
         };
 
+        // Operand reads four ahead of their products: prompts in fp16 960 -> 938 us; in bf16, which has two of the second products
+        // a read, it is 1% slower.
+        auto reads_ahead = [](auto N) __attribute__((always_inline)) {
+            constexpr int n = decltype(N)::value;
+            if constexpr (!SPL) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                for (int i = 0; i < n - 4; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+            }
+        };
         f32x16 sr[2];
         auto scores = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -434,6 +448,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                     const u32x4 x = ld_lds16((const uint16_t*)(smem[0][buf] + kb * HALF + ks / 2 * 2048 + koff[ks & 1]));
                     sr[kb] = mfma32<DT>(x, qf[ks], ks == 0 ? f32x16{} : sr[kb]);
                 }
+            reads_ahead(std::integral_constant<int, 2 * KS>{});
         };
         // register x of block kb is token kb * 32 + x / 8 * 16 + hi * 8 + x % 8
         auto mask = [&](int t) __attribute__((always_inline)) {
@@ -495,6 +510,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                     o[db] = mfma32<DT>(x, pr[ks], o[db]);
                     if constexpr (SPL) o[db] = mfma32<DT>(x, plr[ks], o[db]);
                 }
+            reads_ahead(std::integral_constant<int, PKS * NDB>{});
         };
 
         // ---- the walk: tile t + 1 comes while t is worked on
