@@ -293,7 +293,8 @@ TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int ro
  * it holds; what it sees of NaN and infinities makes its O of that dim (values) or all of it (scores)
  * one of them.  Lengths and pages outside their bounds act as in tkm_attn_decode.  Values of more than
  * 2^100 may overflow in the sums, which hold weights of up to 2^16.
- * Scores, softmax and sums are fp32.  Results do not depend on timing. */
+ * Scores, softmax and sums are fp32; the weights are multiplied with the values as 16-bit parts of together 22 bits (fp16)
+ * or 24 (bf16), as in tkm_attn_decode.  Results do not depend on timing. */
 TKM_ATTN_API int tkm_attn_chunk(const tkm_attn_kv *kv, const void *q, long long q_stride, const int32_t *row_start,
                                 const int32_t *n_new, int rows, void *o, float *lse, int Hq, float scale, int causal,
                                 int window, void *workspace, size_t workspace_bytes, void *stream);

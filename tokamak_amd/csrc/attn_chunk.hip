@@ -10,12 +10,14 @@
 // reads of 16 rows then meet all banks once.  Per tile and wave:
 //   S^T = K Q^T        32 tokens x 32 rows an MFMA block; lane = row.  K's tokens are dealt to the block's rows with
 //                      bits 2 and 3 swapped, so that the 8 registers of a k-step are 8 consecutive tokens:
-//   P^T                stays in its registers, as the B operand of
+//   P^T                takes its place, and goes in 16-bit parts, k-step by k-step, as the B operand to
 //   O^T += V^T P^T     whose A operand is 8 consecutive tokens of a dim, one 16-byte read of a V block.
 //
-// P = 2^(s - m + 8): m moves only when a lane's sum of a tile reaches fp16's largest value, and the 8 keep weights of
-// down to 2^-22 of the row's largest in fp16's normal range.  In fp16 P goes to the second product as one number (11
-// bits, as in the kernels of whole sequences), in bf16 as two (16 bits).
+// P = 2^(s - m + 8): m moves only when a lane's sum of a tile reaches fp16's largest value (the tile's scores are then
+// formed once more), and the 8 keep weights of down to 2^-22 of the row's largest in fp16's normal range.  P goes to the
+// second product in parts that hold what decoding (attn_decode.hip) keeps of it, two in fp16 (22 bits) and three in bf16
+// (24), so that a row has the same precision in either.  One part in fp16 and two in bf16 lost 2^-11 and 2^-16 of a P, and
+// took 929 us for 1226 (prompts in fp16, limited by the products' power), 309 for 365 (a mixed step in bf16).
 //
 // Splitting: all items' tiles are numbered in one line, kv head after kv head, and every workgroup takes an equal
 // share, whatever the lengths are, which are read on the device: a first launch of one workgroup lists the items of a
@@ -113,6 +115,35 @@ __device__ __forceinline__ Joint fixed_joint(const Joint* p) {
 }
 template <int DT>
 constexpr uint32_t kInf = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
+// Two P as 16-bit parts, each what the ones before leave, rounded: the words w[0], w[1], ..  Two parts in fp16 hold 22
+// bits, three in bf16 the 24 of fp32 (as in attn_decode.hip).  What a part leaves is exact: by a mixed-precision fma in
+// fp16, which also rounds the last part, by a dot product with (-1, 0) or (0, -1) in bf16: 3 and 7 instructions a pair (8
+// and 13 where the compiler converts the parts back).
+template <int DT>
+constexpr int kParts = DT == DT_BF16 ? 3 : 2;
+template <int DT>
+__device__ __forceinline__ void split_p(float x, float y, uint32_t (&w)[kParts<DT>]) {
+    // constants that the compiler does not know: it would make a subtraction of -1, and in bf16 has the wrong half
+    float minus = -1.0f;
+    uint32_t of_x = 0xbf80u, of_y = 0xbf800000u;
+    if constexpr (DT == DT_BF16) asm("" : "+s"(of_x), "+s"(of_y));
+    else asm("" : "+s"(minus));
+#pragma unroll
+    for (int i = 0; i < kParts<DT>; ++i) {
+        w[i] = pack2<DT>(x, y);
+        if (i + 1 == kParts<DT>) break;
+        asm("" : "+v"(w[i]));      // both from the one word
+        if constexpr (DT == DT_BF16) {
+            const bf16x2 h = __builtin_bit_cast(bf16x2, w[i]);
+            x = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, of_x), x, false);
+            y = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, of_y), y, false);
+        } else {
+            const f16x2 h = as_f16x2(w[i]);
+            x = __builtin_fmaf((float)h[0], minus, x);
+            y = __builtin_fmaf((float)h[1], minus, y);
+        }
+    }
+}
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // A sequence's rows: `n` of them from row `row0` on, the first at position `pos`; len -1 if it lies outside the table.
@@ -249,12 +280,10 @@ __device__ __forceinline__ const C& arguments() {
 
 template <int D, int DT>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void chunk_kernel(C args) {
-    constexpr bool SPL = Split<DT>::on;
     constexpr int KS = D / 16, NDB = D / 32, PKS = BN / 16;
     constexpr int HALF = D * 64;               // bytes of 32 tokens of K or V
     constexpr int TILE = 2 * HALF;
     constexpr int NI = TILE / 1024 / kWaves;   // DMA requests of a wave, a tile of K or V
-    constexpr int NL = SPL ? PKS : 1;
     __shared__ __attribute__((aligned(1024))) char smem[2][2][TILE];    // [K, V][buffer]
     __shared__ uint2 odds[2][D];               // [half][dim]: bits of the tokens whose value is inf or NaN, -inf or NaN
     __shared__ int votes[kWaves];
@@ -425,20 +454,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                 }
         };
 
-        // Operand reads four ahead of their products: prompts in fp16 960 -> 938 us; in bf16, which has two of the second products
-        // a read, it is 1% slower.
-        auto reads_ahead = [](auto N) __attribute__((always_inline)) {
-            constexpr int n = decltype(N)::value;
-            if constexpr (!SPL) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-                for (int i = 0; i < n - 4; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-            }
-        };
         f32x16 sr[2];
         auto scores = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -448,7 +463,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                     const u32x4 x = ld_lds16((const uint16_t*)(smem[0][buf] + kb * HALF + ks / 2 * 2048 + koff[ks & 1]));
                     sr[kb] = mfma32<DT>(x, qf[ks], ks == 0 ? f32x16{} : sr[kb]);
                 }
-            reads_ahead(std::integral_constant<int, 2 * KS>{});
+            if constexpr (DT == DT_F16) sched_reads_mfma<2 * KS, 1, 4>();      // drafts of 64 dims 13.85 -> 13.67 us; in bf16 slower
         };
         // register x of block kb is token kb * 32 + x / 8 * 16 + hi * 8 + x % 8
         auto mask = [&](int t) __attribute__((always_inline)) {
@@ -461,33 +476,48 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                     if (j >= up || j < down) sr[kb][x] = -INFINITY;
                 }
         };
-        u32x4 pr[PKS], plr[NL];
+        // P in the scores' place
         auto expo = [&](float ref) __attribute__((always_inline)) {
             float sum = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < PKS; ++ks)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int x = (ks & 1) * 8 + 2 * w;
-                    const float p0 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x], sl2, -ref));
-                    const float p1 = fast_exp2(__builtin_fmaf(sr[ks >> 1][x + 1], sl2, -ref));
-                    if constexpr (SPL) {
-                        const u32x2 hl = pack_split_bf16(p0, p1);
-                        pr[ks][w] = hl[0];
-                        plr[ks][w] = hl[1];
-                    } else {
-                        pr[ks][w] = pack2<DT>(p0, p1);
-                    }
-                    sum += p0 + p1;
+                for (int x = 0; x < 16; ++x) {
+                    sr[kb][x] = fast_exp2(__builtin_fmaf(sr[kb][x], sl2, -ref));
+                    sum += sr[kb][x];
                 }
             return sum;
         };
+        // the parts of P of a k-step
+        constexpr int NP = kParts<DT>;
+        auto parts = [&](int ks, u32x4 (&pr)[NP]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int x = (ks & 1) * 8 + 2 * i;
+                uint32_t w[NP];
+                split_p<DT>(sr[ks >> 1][x], sr[ks >> 1][x + 1], w);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) pr[j][i] = w[j];
+            }
+        };
         auto tile = [&](int t, int buf) __attribute__((always_inline)) {
-            scores(buf);
-            if (t < p0 || t >= p1) mask(t);
+            auto masked = [&](int t, int buf) __attribute__((always_inline)) {
+                scores(buf);
+                if (t < p0 || t >= p1) mask(t);
+            };
+            masked(t, buf);
             float sum = INFINITY;
-            if (!__any(m == -INFINITY)) sum = expo(m);                 // m is not set yet in an item's first tile
-            if (__builtin_expect(__any(!(sum < kSumMax)), 0)) {
+            bool move = __any(m == -INFINITY);                         // m is not set yet in an item's first tile
+            if (!move) {
+                sum = expo(m);
+                if (__builtin_expect(__any(!(sum < kSumMax)), 0)) {    // the scores once more, P having taken their place
+                    int again = t, from = buf;
+                    asm volatile("" : "+s"(again), "+s"(from));        // and not what the compiler would keep of the first ones
+                    masked(again, from);
+                    move = true;
+                }
+            }
+            if (__builtin_expect(move, 0)) {
                 float v = sr[0][0];
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -502,15 +532,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                 sum = expo(m == -INFINITY ? 0.f : m);
             }
             lsum += sum;
+            u32x4 pr[2][NP];
+            parts(0, pr[0]);
 #pragma unroll
-            for (int ks = 0; ks < PKS; ++ks)
+            for (int ks = 0; ks < PKS; ++ks) {
+                if (ks + 1 < PKS) parts(ks + 1, pr[(ks + 1) & 1]);
 #pragma unroll
                 for (int db = 0; db < NDB; ++db) {
                     const u32x4 x = ld_lds16((const uint16_t*)(smem[1][buf] + ks / 2 * HALF + db * 2048 + voff[ks & 1]));
-                    o[db] = mfma32<DT>(x, pr[ks], o[db]);
-                    if constexpr (SPL) o[db] = mfma32<DT>(x, plr[ks], o[db]);
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) o[db] = mfma32<DT>(x, pr[ks & 1][j], o[db]);
                 }
-            reads_ahead(std::integral_constant<int, PKS * NDB>{});
+            }
         };
 
         // ---- the walk: tile t + 1 comes while t is worked on
