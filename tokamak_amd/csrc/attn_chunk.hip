@@ -173,7 +173,8 @@ __device__ __forceinline__ int over_g(const C& a, int r) { return (int)(__umulhi
 __device__ __forceinline__ int2 seen_by(const C& a, int pos, int len, int i) {
     if (!a.causal) return int2{0, max(len, 0)};
     const int p = pos + i;
-    return int2{a.window ? max(0, p - a.window + 1) : 0, max(0, min(p + 1, len))};
+    // windows reach up to 2^31 - 1, and p below 0 where a sequence has more rows than tokens
+    return int2{a.window && p >= a.window ? p - a.window + 1 : 0, max(0, min(p + 1, len))};
 }
 // Item t of a sequence.
 __device__ __forceinline__ Item item_of(const C& a, const Seq& s, int b, int t) {
