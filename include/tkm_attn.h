@@ -290,8 +290,8 @@ TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int ro
  * [0, rows) has no rows, and rows behind them are passed over; no two sequences may have a row, and o
  * must not overlap q.  Rows of no sequence stay as they are in o and lse.
  * A row that sees nothing gets O = 0, LSE = -inf.  What a row does not see has no part in it, whatever
- * it holds; what it sees of NaN and infinities makes its O of that dim (values) or all of it (scores)
- * one of them.  Lengths and pages outside their bounds act as in tkm_attn_decode.  Values of more than
+ * it holds; what it sees of NaN and infinities acts as in tkm_attn_decode, and so do lengths and pages
+ * outside their bounds.  Infinities and NaN among the values cost a second walk.  Values of more than
  * 2^100 may overflow in the sums, which hold weights of up to 2^16.
  * Scores, softmax and sums are fp32; the weights are multiplied with the values as 16-bit parts of together 22 bits (fp16)
  * or 24 (bf16), as in tkm_attn_decode.  Results do not depend on timing. */

@@ -4,8 +4,9 @@ import math
 import pytest
 import torch
 
-from kv_cases import DT, Case
+from kv_cases import DT, HALF, TINY, Case
 from step_cases import check_chunk
+from test_kv_odd_values_gpu import LENS, formula, plant, same_kind
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,42 @@ def test_windows_as_wide_as_an_int(gpu, Hq, Hkv, D, page, dtype, extra):
         assert torch.equal(wo, o) and torch.equal(wl, lse), window
     for window in (301, 300, 294, 293, 20):      # ends inside the sequences
         check_chunk(case, lens, n_new, q, *attn.gqa_chunk(q, case.cache, Hq, *where, window=window), Hq, window=window)
+
+
+@pytest.mark.parametrize("D,dtype,G", [(64, "f16", 3), (128, "bf16", 33), (64, "bf16", 8), (128, "f16", 2)])
+@pytest.mark.parametrize("cap,window", [("tight", 0), ("tight", 200), ("wide", 0), ("wide", 500)])
+@pytest.mark.parametrize("q0", ["up", "mixed"])
+def test_infinities_are_those_of_decoding(gpu, D, dtype, G, cap, window, q0):
+    """Infinities and NaN among keys and values go where the formula takes them, in tiles that all rows see and in those on
+    an edge, in calls of one launch and of three: which outputs are NaN, or infinite, agrees with gqa_decode's formula for
+    each row over what it sees, and the others are within its bounds."""
+    from tokamak_amd import attn
+    print(f"[case] D{D} {dtype} G{G} {cap} window {window} {q0}", flush=True)
+    Hkv, Hq, scale = 2, 2 * G, 1.0 / math.sqrt(D)
+    lens, n_new = LENS[cap], [1, 3, 9, 4, 1, 13, 5, 2]
+    case = Case(gpu, lens, Hkv, D, 64, dtype, extra_pages=100 if cap == "wide" else 0)
+    plant(case)
+    total, row_start = sum(n_new), [sum(n_new[:b]) for b in range(len(lens) + 1)]
+    q = randn((total, Hkv, G, D), dtype, G)
+    q[..., 0] = 0.5
+    if q0 == "mixed":
+        q[:, :, 1, 0] = -0.5         # -inf keys give +inf
+        if G > 2:
+            q[:, :, 2, 0] = 0.0      # and 0 * inf = NaN
+    o, lse = attn.gqa_chunk(q.reshape(total, -1).to(gpu), case.cache, Hq, i32(row_start, gpu), i32(n_new, gpu), window=window)
+    assert window or ("join" in attn.last_kernels()) == (cap == "wide")       # a window can make items short
+    o, lse = o.cpu().double().reshape(total, Hkv, G, D), lse.cpu().double().reshape(total, Hkv, G)
+    worst = [0.0, 0.0]
+    for b, n in enumerate(n_new):
+        for i in range(n):
+            r, up = row_start[b] + i, lens[b] - n + i + 1
+            lo = max(0, up - window) if window else 0
+            for h in range(Hkv):
+                ro, rl, _, eo, el, _ = [x.cpu() for x in formula(*(x.to(gpu) for x in (q[r, h].double(), case.k[b][h, lo:up], case.v[b][h, lo:up])), scale)]
+                assert same_kind(lse[r, h], rl), (b, i, h)
+                assert same_kind(o[r, h], ro), (b, i, h, torch.nonzero(o[r, h].isnan() != ro.isnan()).tolist()[:9])
+                some = torch.isfinite(ro)
+                worst[0] = max([worst[0], *((o[r, h] - ro).abs() / (eo + HALF[dtype] * (ro.abs() + eo) + TINY[dtype]))[some].tolist()])
+                worst[1] = max([worst[1], *((lse[r, h] - rl).abs() / el)[torch.isfinite(rl)].tolist()])
+    print("    o %.3f, lse %.3f of their bounds" % tuple(worst), flush=True)
+    assert max(worst) <= 1.0

@@ -30,10 +30,11 @@
 // joining 15 more); for prompts of 128 dims products and exponentials one after the other (46 and 36% of the clocks at 1.86
 // GHz; 707 GFLOP seen, 854 done in tiles, in 940 us); at 64 dims the issue of exponentials and sums, three waves a SIMD, and a part's beginning and end.
 //
-// 0 times an infinity or NaN is NaN, also where P is 0 because its row does not see the token.  So a tile that an item's
-// rows do not see alike is searched for such values in LDS; they become 0 there, and a bit each, by which they are
-// added to the sums of the rows that see them.  (In tiles that all rows see an infinity may become NaN, by a part of P
-// that is 0 or negative.)
+// 0 times an infinity or NaN is NaN, also where P is 0 because its row does not see the token, and an infinity times a part
+// of P that is 0 or negative is NaN where the whole of P makes it infinite.  So a tile that an item's rows do not see alike
+// is searched for such values in LDS, where they become 0.  If there were any, or sums have become NaN, the workgroup
+// goes through its tiles once more, searches all of them, and adds what it finds, kept as a bit each, to the sums of
+// the rows that see them: an infinity, or NaN where P is 0, as in attn_decode.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -388,12 +389,22 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                 dma16_rows(make_rsrc(values + sub * HALF, HALF), dma_at + (uint32_t)((2 + buf) * TILE), dma_v);
             }
         };
+        // Whether a thread of the workgroup has it.  The next question comes behind a barrier.
+        auto any_of = [&](bool mine) {
+            mine = __any(mine);
+            if (lane == 0) votes[wave] = mine;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) all |= votes[w];
+            return uni(all) != 0;
+        };
         // Values of tokens behind the sequence's last become 0, for what is there may be anything, and infinities and
-        // NaN, whose bits are left in `odds`.  True if there were any of these.
-        auto search = [&](int t, int buf) {
+        // NaN, whose bits are left in `odds`.  True if there were any of these.  `me`: this thread.
+        auto search = [&](int t, int buf, int me) __attribute__((always_inline)) {
             const int left = it.len - t * BN;
             bool any = false;
-            for (int i = threadIdx.x; i < 2 * D; i += 64 * kWaves) {         // rows of 32 tokens of one dim
+            for (int i = me; i < 2 * D; i += 64 * kWaves) {         // rows of 32 tokens of one dim
                 char* row = smem[1][buf] + i * 64;
                 const int from = i < D ? 0 : 32;
                 u16x2 most = {0, 0};
@@ -427,21 +438,25 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                 }
                 odds[i / D][i % D] = bits;
             }
-            any = __any(any);
-            if (lane == 0) votes[wave] = any;
-            __syncthreads();
-            int all = 0;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) all |= votes[w];
-            return uni(all) != 0;
+            return any_of(any);
         };
-        // the values that `search` took out, for the rows that see them
+        f32x16 sr[2];
+        // In the second walk: the values that `search` took out, for the rows that see them; NaN where P is 0.  Of numbers
+        // of its own, as that walk's search: what is formed of a thread's place would keep registers in the first walk (at
+        // 64 dims the products' operands were then read one by one, 1.14 us a tile for 1.01).
         auto add_odd = [&](int t) __attribute__((always_inline)) {
-            uint32_t sees[2];
+            uint32_t sees[2], none[2];
+            int hi = lane >> 5;
+            asm volatile("" : "+v"(hi));
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int to = min(max(seen.y - t * BN - x * 32, 0), 32), from = min(max(seen.x - t * BN - x * 32, 0), 32);
                 sees[x] = (uint32_t)((1ull << to) - 1) & ~(uint32_t)((1ull << from) - 1);
+                none[x] = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) none[x] |= sr[x][i] == 0.f ? 1u << ((i >> 3) * 16 + (i & 7)) : 0u;
+                none[x] <<= hi * 8;
+                none[x] = sees[x] & (none[x] | (uint32_t)__shfl_xor((int)none[x], 32, 64));      // the other half's tokens
             }
 #pragma unroll
             for (int db = 0; db < NDB; ++db)
@@ -449,13 +464,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                 for (int i = 0; i < 16; ++i) {
                     const int d = db * 32 + i / 4 * 8 + hi * 4 + i % 4;
                     const uint2 a0 = odds[0][d], a1 = odds[1][d];
-                    if ((a0.x & sees[0]) | (a1.x & sees[1])) o[db][i] += INFINITY;
-                    if ((a0.y & sees[0]) | (a1.y & sees[1])) o[db][i] -= INFINITY;
+                    const uint32_t lost = ((a0.x | a0.y) & none[0]) | ((a1.x | a1.y) & none[1]);
+                    if (lost | (a0.x & sees[0]) | (a1.x & sees[1])) o[db][i] += INFINITY;
+                    if (lost | (a0.y & sees[0]) | (a1.y & sees[1])) o[db][i] -= INFINITY;
                     __builtin_amdgcn_sched_barrier(0);       // it is seldom run, and is to take few registers
                 }
         };
 
-        f32x16 sr[2];
         auto scores = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
@@ -547,35 +562,55 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
             }
         };
 
-        // ---- the walk: tile t + 1 comes while t is worked on
-        if (ta < te) {
-            fetch(ta);
-            issue(ta, 0);
-            if (ta + 1 < te) fetch(ta + 1);
-        }
-        wait_dma();
-        __syncthreads();
-        auto step = [&](int t, auto Buf) __attribute__((always_inline)) {
-            const int buf = Buf;
-            const bool odd = (t < it.alike || t >= it.alike_end) && search(t, buf);
-            if (t + 1 < te) {
-                issue(t + 1, buf ^ 1);
-                if (t + 2 < te) fetch(t + 2);
-            }
-            if (t >= n0 && t < n1) {
-                tile(t, buf);
-                if (__builtin_expect(odd, 0)) add_odd(t);
+        // ---- the walk: tile t + 1 comes while t is worked on.  True if infinities or NaN were found (and, but for ODD,
+        // left out).
+        auto walk = [&](auto Odd) __attribute__((always_inline)) {
+            constexpr bool ODD = decltype(Odd)::value;
+            bool odd = false;
+            if (ta < te) {
+                fetch(ta);
+                issue(ta, 0);
+                if (ta + 1 < te) fetch(ta + 1);
             }
             wait_dma();
             __syncthreads();
-        };
-        if constexpr (D == 64) {       // one body: two would take more registers than three waves a SIMD leave
-            for (int t = ta; t < te; ++t) step(t, (t - ta) & 1);
-        } else {                       // 3% faster than one at 128 rows an item
-            for (int t = ta; t < te; t += 2) {
-                step(t, std::integral_constant<int, 0>{});
-                if (t + 1 < te) step(t + 1, std::integral_constant<int, 1>{});
+            auto step = [&](int t, auto Buf) __attribute__((always_inline)) {
+                const int buf = Buf;
+                int me = threadIdx.x;
+                if constexpr (ODD) asm volatile("" : "+v"(me));
+                if (ODD || t < it.alike || t >= it.alike_end) odd |= search(t, buf, me);
+                if (t + 1 < te) {
+                    issue(t + 1, buf ^ 1);
+                    if (t + 2 < te) fetch(t + 2);
+                }
+                if (t >= n0 && t < n1) {
+                    tile(t, buf);
+                    if constexpr (ODD) add_odd(t);
+                }
+                wait_dma();
+                __syncthreads();
+            };
+            if constexpr (D == 64 || ODD) {       // one body: two would take more registers than three waves a SIMD leave
+                for (int t = ta; t < te; ++t) step(t, (t - ta) & 1);
+            } else {                              // 3% faster than one at 128 rows an item
+                for (int t = ta; t < te; t += 2) {
+                    step(t, std::integral_constant<int, 0>{});
+                    if (t + 1 < te) step(t + 1, std::integral_constant<int, 1>{});
+                }
             }
+            return odd;
+        };
+        bool odd = walk(std::false_type{}), lost = false;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) lost |= __builtin_isunordered(o[db][i], o[db][i + 1]);
+        if (__builtin_expect(any_of(odd || (lost && valid && lsum == lsum)), 0)) {
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) o[db] = f32x16{};
+            m = -INFINITY;
+            lsum = 0.f;
+            walk(std::true_type{});
         }
 
         // ---- out
@@ -655,7 +690,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(C a, int each) {
                 if (i >= it.n) break;
                 const float f = weight(ml[i], m);
                 l += ml[i].x == -INFINITY ? ml[i].y : f * ml[i].y;
-                if (f != 0.f) o += f * x[i];       // what has no weight may be anything
+                o += f * x[i];
             }
             put_joined<D, DT>(a, it, r, d, o, m, l);
         }
@@ -683,7 +718,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(C a, int each) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float w = __shfl(f, i + k * EACH + lane / LANES, 64);      // 0 behind the last
-                    if (w != 0.f) o += w * x[k];
+                    if (i + k * EACH + lane / LANES < n) o += w * x[k];
                 }
             }
         }
