@@ -258,10 +258,12 @@ typedef struct {
  * back, in the order of sequences and positions, and their table entries become -1: want 0 and start 0
  * end a sequence, want 0 after an eviction frees what it left.  Then, in the order of sequences, each
  * takes the pages that it lacks, if the free ones suffice for it and all that lacked pages before it,
- * and its rows if they fit into `rows` behind those of the sequences before it that got theirs; else it
- * gets no page and no row (and from the first whose pages are missing on, only those that lack none go
- * on).  So does one that would outgrow its table, wants less than 1, or whose start lies outside the
- * table.  len[b] becomes start[b] + n_new[b].
+ * and its rows, if they fit into `rows` behind the rows of all before it for whom there were pages; else
+ * it gets no page and no row.  So from the first whose pages are missing on, only those that lack none go
+ * on, and from the first whose rows do not fit on, none does: a want of more than `rows` holds up all
+ * behind it, step after step, until it is cut into pieces.  One that would outgrow its table, wants less
+ * than 1, or whose start lies outside the table gets none either, and is not counted.  len[b] becomes
+ * start[b] + n_new[b].
  * The tables' pages must be theirs alone.  With start given, a second call of the same step changes
  * nothing.  kv's table and len are written; its k and v are not touched and may be any layer's. */
 TKM_ATTN_API int tkm_attn_kv_plan(const tkm_attn_kv *kv, const tkm_attn_pages *pages, const int32_t *want,

@@ -1,0 +1,12 @@
+"""Limits of a serving step's calls without a GPU, with results written out by hand."""
+import pytest
+
+from step_cases import plan_ref
+
+
+@pytest.mark.parametrize("rows,want,n_new", [(10, [8, 5, 2], [8, 0, 0]), (10, [8, 2, 5], [8, 2, 0]), (10, [30, 1, 1], [0, 0, 0]),
+                                             (10, [-1, 11, 1], [0, 0, 0]), (40, [33, 300, 7], [33, 0, 7])])
+def test_rows_that_do_not_fit_hold_up_those_behind(rows, want, n_new):
+    """What the helper of the GPU tests gives is what include/tkm_attn.h says."""
+    p = plan_ref([[-1] * 4 for _ in range(3)], [2, 1, 0], 3, [0, 0, 0], want, [0, 0, 0], 32, 3, rows)
+    assert p["n_new"] == n_new and p["row_start"] == [0, n_new[0], n_new[0] + n_new[1], sum(n_new)]

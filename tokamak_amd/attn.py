@@ -597,7 +597,8 @@ def kv_plan(cache, pages, want, rows=None, start=None, plan=None, stream=None):
     """Makes room for want [B] int32 more tokens of each sequence behind start [B] int32 (None: kv_len itself), takes
     pages from the pool and gives back what sequences no longer need, advances kv_len, and lays out the step's packed
     rows, at most `rows` of them (or as many as the given plan has).  A sequence whose pages or rows are not there gets
-    none: its plan.n_new is 0.  include/tkm_attn.h has the rules.  Returns the plan."""
+    none: its plan.n_new is 0.  From the first whose rows do not fit on, none gets any: cut a want of more than `rows`
+    into pieces.  include/tkm_attn.h has the rules.  Returns the plan."""
     st = _current(cache.device, stream)
     if st is None:
         with _On(cache.device, stream) as st:

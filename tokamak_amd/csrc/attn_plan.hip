@@ -2,7 +2,7 @@
 //
 // For sequences b in order, t_b = ceil((start_b + want_b) / page), held_b the pages of its table row:
 //   back_b = max(0, held_b - t_b)     go on the stack of free pages, positions ascending
-//   need_b = max(0, t_b - held_b)     if sum_{c <= b} need_c <= free + sum back, and the rows fit
+//   need_b = max(0, t_b - held_b)     if sum_{c <= b} need_c <= free + sum back, and the rows fit behind all that had pages
 //   row_start_b = sum_{c < b} n_c;  row r of b: position start_b + r - row_start_b, slot page * size + token
 // Four prefix sums over the sequences, and two lists (pages and rows) whose elements find their sequence in a prefix
 // sum by bisection.  Bound by latency: one workgroup goes through the sequences, 1024 at a time, so that the
