@@ -646,6 +646,8 @@ def _kv_append_rows(qkv, cache, Hq, plan, rope, q, st):
     n, q_stride = _rows_of("q", q, Hq * D, dev, cache.dtype, least=True)
     if n != rows:
         raise ValueError(f"q has {n} rows, expected {rows}")
+    if rows < 2:
+        q_stride = stride      # a single row has none of its own: in place it may be of another width
     _check("tkm_attn_kv_append_rows", lib().tkm_attn_kv_append_rows(
         cache._ref, None if rope is None else rope._ref, qkv.data_ptr(), stride, q.data_ptr(), q_stride, plan._ref, rows, Hq, st))
     return q
