@@ -79,3 +79,25 @@ def test_infinities_are_those_of_decoding(gpu, D, dtype, G, cap, window, q0):
                 worst[1] = max([worst[1], *((lse[r, h] - rl).abs() / el)[torch.isfinite(rl)].tolist()])
     print("    o %.3f, lse %.3f of their bounds" % tuple(worst), flush=True)
     assert max(worst) <= 1.0
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [(4, 2, 64, 32, "f16"), (16, 2, 128, 64, "bf16")])
+@pytest.mark.parametrize("extra", [1, 60])
+def test_padded_rows_are_clamped(gpu, Hq, Hkv, D, page, dtype, extra):
+    """A batch of S rows a sequence, of which n_new says more: S of them, as kv_append stores them, and none of the next
+    sequence's."""
+    from tokamak_amd import attn
+    print(f"[case] Hq{Hq} Hkv{Hkv} D{D} page{page} {dtype} extra {extra}", flush=True)
+    lens, S = [100, 33, 400, 20], 11
+    case = Case(gpu, lens, Hkv, D, page, dtype, extra_pages=extra)
+    q = randn((4 * S, Hq * D), dtype, 2).to(gpu)
+    o, lse = attn.gqa_chunk(q, case.cache, Hq)
+    check_chunk(case, lens, [S] * 4, q, o, lse, Hq)
+    for n in ([S + 1] * 4, [4 * S, INT_MAX, S, S + 5], [INT_MAX] * 4):
+        for _ in range(3):
+            co, cl = attn.gqa_chunk(q, case.cache, Hq, n_new=i32(n, gpu))
+            assert torch.equal(co, o) and torch.equal(cl, lse), n
+    out = torch.full_like(o, 4.0)
+    co, cl = attn.gqa_chunk(q, case.cache, Hq, n_new=i32([S + 9, -3, 5, INT_MAX], gpu), out=out)
+    check_chunk(case, lens, [S, 0, 5, S], q, co, cl, Hq, row_start=[0, S, 2 * S, 3 * S])
+    assert (out[S:2 * S] == 4.0).all() and (out[2 * S + 5:3 * S] == 4.0).all()

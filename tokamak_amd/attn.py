@@ -666,8 +666,8 @@ def gqa_chunk(q, cache, Hq, row_start=None, n_new=None, scale=None, causal=True,
               stream=None):
     """O [rows, Hq*D] and LSE [rows, Hq] (fp32) of each sequence's new rows over its cached positions, their own
     among them (append first).  q: [rows, >= Hq*D] with the Q heads first.  Sequence b has n_new[b] int32 rows from
-    row_start[b] int32 on (a plan's; row_start None: from b * (rows / B), n_new None: rows / B), and the last of them
-    stands at its last position.  causal: a row sees the positions up to its own, with a window only the last `window`
+    row_start[b] int32 on (a plan's; row_start None: at most rows / B from b * (rows / B), n_new None: rows / B), and the
+    last of them stands at its last position.  causal: a row sees the positions up to its own, with a window only the last `window`
     of these.  Rows of no sequence stay as they are in out and lse.
     workspace: chunk_workspace_bytes(cache, rows, Hq) bytes, allocated for the call if not given."""
     st = _current(cache.device, stream)

@@ -159,7 +159,8 @@ __device__ __forceinline__ Seq seq_of(const C& a, int b) {
     };
     Seq s;
     s.row0 = a.row_start ? get(a.row_start) : b * a.each;
-    const int n = a.n_new ? get(a.n_new) : a.each;
+    int n = a.n_new ? get(a.n_new) : a.each;
+    if (!a.row_start) n = min(n, a.each);      // the next sequence's rows begin there
     s.len = get(a.len);
     if ((unsigned)s.len > (unsigned)a.cap) s.len = -1;
     s.n = s.row0 < 0 || s.row0 >= a.rows ? 0 : max(0, min(n, a.rows - s.row0));
