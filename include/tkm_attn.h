@@ -286,12 +286,12 @@ TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int ro
 /* Attention of each sequence's new rows over its len[b] cached positions, their own among them: row i
  * of n_new[b] stands at position p = len[b] - n_new[b] + i and sees the positions j < len[b], with
  * causal = 1 those of j <= p, and with window > 0 (causal only) of these j > p - window.
- * q: `rows` rows of Hq * D values, q_stride elements apart (a multiple of 8); o [rows][Hq * D]; lse
- * [rows][Hq] or NULL.  Sequence b has the rows row_start[b] .. row_start[b] + n_new[b] - 1; row_start
- * NULL: from b * (rows / B) on, of which n_new[b] (clamped to rows / B) are its rows; n_new NULL (only
- * then): all.  A sequence that begins outside [0, rows) has no rows, and rows behind them are passed
- * over; no two sequences may have a row, and o must not overlap q.  Rows of no sequence stay as they are
- * in o and lse.
+ * q: `rows` rows (1 at least: a step without rows leaves the call out) of Hq * D values, q_stride
+ * elements apart (a multiple of 8); o [rows][Hq * D]; lse [rows][Hq] or NULL.  Sequence b has the rows
+ * row_start[b] .. row_start[b] + n_new[b] - 1; row_start NULL: from b * (rows / B) on, of which n_new[b]
+ * (clamped to rows / B) are its rows; n_new NULL (only then): all.  A sequence that begins outside
+ * [0, rows) has no rows, and rows behind them are passed over; no two sequences may have a row, and o
+ * must not overlap q.  Rows of no sequence stay as they are in o and lse.
  * A row that sees nothing gets O = 0, LSE = -inf.  What a row does not see has no part in it, whatever
  * it holds; what it sees of NaN and infinities acts as in tkm_attn_decode, and so do lengths and pages
  * outside their bounds.  Infinities and NaN among the values cost a second walk.  Values of more than

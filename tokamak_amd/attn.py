@@ -668,7 +668,7 @@ def gqa_chunk(q, cache, Hq, row_start=None, n_new=None, scale=None, causal=True,
     among them (append first).  q: [rows, >= Hq*D] with the Q heads first.  Sequence b has n_new[b] int32 rows from
     row_start[b] int32 on (a plan's; row_start None: at most rows / B from b * (rows / B), n_new None: rows / B), and the
     last of them stands at its last position.  causal: a row sees the positions up to its own, with a window only the last `window`
-    of these.  Rows of no sequence stay as they are in out and lse.
+    of these.  Rows of no sequence stay as they are in out and lse; without rows nothing is launched.
     workspace: chunk_workspace_bytes(cache, rows, Hq) bytes, allocated for the call if not given."""
     st = _current(cache.device, stream)
     if st is None:
@@ -698,6 +698,8 @@ def _gqa_chunk(q, cache, Hq, row_start, n_new, scale, causal, window, out, lse, 
         lse = torch.empty((rows, max(0, Hq)), dtype=torch.float32, device=dev)
     else:
         _check_tensor("lse", lse, rows * Hq, dev, torch.float32)
+    if rows == 0:
+        return out, lse
     if workspace is None:
         wbytes = chunk_workspace_bytes(cache, rows, Hq)
         if wbytes:
