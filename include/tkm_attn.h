@@ -231,8 +231,10 @@ TKM_ATTN_API int tkm_attn_rope_from_freqs(const double *freqs, int rot, int layo
 /* Rotates the Q and K heads of `rows` rows of (Hq + 2*Hkv) * D values, strides in elements (multiples
  * of 8); Hkv 0: rows of Q heads.  V is copied.  out == in (and the strides equal): in place, V is left
  * alone.  Row r is at position pos[r], or r % S where pos is NULL; a row of a negative position is
- * left as it is in out.  inverse = 1 turns the other way, which is the gradient: din from dout.
- * 0 rows launch nothing. */
+ * left as it is in out.  inverse = 1 turns the other way, which is the gradient: din from dout; with
+ * TKM_ROPE_CLEAR added to it, rows of negative positions become 0 in out, all heads of them, as a new
+ * tensor needs it.  0 rows launch nothing. */
+enum { TKM_ROPE_CLEAR = 256 };
 TKM_ATTN_API int tkm_attn_rope_rows(const tkm_attn_rope *rope, const void *in, long long in_stride, void *out,
                                     long long out_stride, const int32_t *pos, int S, int rows, int Hq, int Hkv, int D,
                                     int dtype, int inverse, void *stream);

@@ -2,6 +2,8 @@
 import pytest
 
 from step_cases import plan_ref
+from test_step_cpu import EINVAL, OK, call_rope
+from tokamak_amd import attn
 
 
 @pytest.mark.parametrize("rows,want,n_new", [(10, [8, 5, 2], [8, 0, 0]), (10, [8, 2, 5], [8, 2, 0]), (10, [30, 1, 1], [0, 0, 0]),
@@ -10,3 +12,14 @@ def test_rows_that_do_not_fit_hold_up_those_behind(rows, want, n_new):
     """What the helper of the GPU tests gives is what include/tkm_attn.h says."""
     p = plan_ref([[-1] * 4 for _ in range(3)], [2, 1, 0], 3, [0, 0, 0], want, [0, 0, 0], 32, 3, rows)
     assert p["n_new"] == n_new and p["row_start"] == [0, n_new[0], n_new[0] + n_new[1], sum(n_new)]
+
+
+@pytest.mark.parametrize("inverse", [-1, 2, 3, 255, 258, 512, 1 | 512])
+def test_rope_knows_no_other_flags(inverse):
+    assert call_rope(inverse=inverse) == EINVAL
+    assert b"inverse" in attn.lib().tkm_attn_last_error()
+
+
+@pytest.mark.parametrize("inverse", [256, 257])
+def test_rope_takes_the_flag(inverse):
+    assert call_rope(inverse=inverse, rows=0, x=None, y=None) == OK

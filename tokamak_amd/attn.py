@@ -438,6 +438,9 @@ def _kv_evict(cache, budget, sink, recent, dst, kept, st):
     return kept
 
 
+ROPE_CLEAR = 256      # TKM_ROPE_CLEAR
+
+
 class Rope:
     """Rotary positions (tkm_attn_rope, include/tkm_attn.h): the first `rot` dims of a head turn, pair i by freqs[i]
     radians a position.
@@ -493,12 +496,13 @@ class Rope:
 def rope_fwd(x, rope, Hq, Hkv, D, pos=None, S=None, out=None, stream=None):
     """Rotates the Q and K heads of packed rows x [..., (Hq+2Hkv)*D] (rows any multiple of 8 elements apart in a 2-D
     x) to the positions pos [rows] int32, or, if these are None, to r % S of the row r; V is copied.  A row of a
-    negative position stays as it is in out.  out: a new tensor, or a given one; x itself: in place."""
+    negative position stays as it is in a given out (x itself: in place), and is 0 in a new one."""
     return _rope_on(x, rope, Hq, Hkv, D, pos, S, out, 0, stream)
 
 
 def rope_bwd(dout, rope, Hq, Hkv, D, pos=None, S=None, dx=None, stream=None):
-    """The gradient of rope_fwd's x from that of its output: the rotation the other way."""
+    """The gradient of rope_fwd's x from that of its output: the rotation the other way.  Rows of negative positions as
+    there."""
     return _rope_on(dout, rope, Hq, Hkv, D, pos, S, dx, 1, stream)
 
 
@@ -539,6 +543,7 @@ def _rope(x, rope, Hq, Hkv, D, pos, S, out, inverse, st):
         _check_dtype("pos", pos, rows, dev, "int32")
     if out is None:
         out, ostride = x.new_empty(x.shape), width
+        inverse |= ROPE_CLEAR
     else:
         n, ostride = _rows_of("out", out, width, dev, x.dtype)
         if n != rows:
@@ -627,8 +632,9 @@ def _kv_plan(cache, pages, want, rows, start, plan, st):
 
 def kv_append_rows(qkv, cache, Hq, plan, rope=None, q=None, stream=None):
     """Stores the K and V heads of a plan's packed rows qkv [rows, (Hq+2Hkv)*D] in their slots of the cache, K rotated
-    to its position if there is a rope, and returns the Q heads [rows, >= Hq*D], rotated too: a new tensor, or the
-    given q (qkv itself: in place; without a rope and q they stay where they are).  kv_len is the plan's business."""
+    to its position if there is a rope, and returns the Q heads [rows, >= Hq*D], rotated too: a new tensor, whose rows
+    of no sequence hold anything, or the given q (qkv itself: in place; without a rope and q they stay where they are).
+    kv_len is the plan's business."""
     st = _current(cache.device, stream)
     if st is None:
         with _On(cache.device, stream) as st:
@@ -668,7 +674,8 @@ def gqa_chunk(q, cache, Hq, row_start=None, n_new=None, scale=None, causal=True,
     among them (append first).  q: [rows, >= Hq*D] with the Q heads first.  Sequence b has n_new[b] int32 rows from
     row_start[b] int32 on (a plan's; row_start None: at most rows / B from b * (rows / B), n_new None: rows / B), and the
     last of them stands at its last position.  causal: a row sees the positions up to its own, with a window only the last `window`
-    of these.  Rows of no sequence stay as they are in out and lse; without rows nothing is launched.
+    of these.  Rows of no sequence stay as they are in out and lse (in new ones they hold anything); without rows
+    nothing is launched.
     workspace: chunk_workspace_bytes(cache, rows, Hq) bytes, allocated for the call if not given."""
     st = _current(cache.device, stream)
     if st is None:

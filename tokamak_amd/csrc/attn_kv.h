@@ -53,7 +53,7 @@ struct RopeArgs {
     void* out;
     long long out_stride;
     const int32_t* pos;     // NULL: r % S
-    int S, rows, Hq, Hkv, D, dtype, inverse;
+    int S, rows, Hq, Hkv, D, dtype, inverse, clear;     // clear: rows of negative positions become 0
     void* stream;
 };
 

@@ -116,15 +116,20 @@ struct RopeK {
     long long in_stride, out_stride;
     int S, rows, heads, all, D, T;     // rotated heads, heads of a row
     float sign;
+    int clear;
 };
 
 template <int DT, int LAYOUT, int V>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeK a) {
     __shared__ float2 cs[kThreads / 64][64];
     const Row w = begin_row(cs, a.T, a.rows, a.pos, a.S, a.rope, a.sign);
-    if (w.pos < 0) return;
     const uint16_t* in = a.in + w.r * a.in_stride;
     uint16_t* out = a.out + w.r * a.out_stride;
+    if (w.pos < 0) {
+        if (a.clear && w.r < a.rows)
+            for (int i = w.t; i < a.all * (a.D / 8); i += w.T) *(u32x4*)(out + i * 8) = u32x4{0u, 0u, 0u, 0u};
+        return;
+    }
     const int chunks = a.D / 8, rotate = a.heads * chunks, all = in == out ? rotate : a.all * chunks;
     for (int i = w.t; i < all; i += w.T) {
         Chunk x;
@@ -269,7 +274,7 @@ bool rows_fit(const tkm_attn_kv* kv, int rows) {
 
 int launch_rope(const RopeArgs& a) {
     RopeK k{a.rope, (const uint16_t*)a.in, (uint16_t*)a.out, a.pos, a.in_stride, a.out_stride, a.S, a.rows, a.Hq + a.Hkv,
-            a.Hq + 2 * a.Hkv, a.D, threads_a_row(a.rows, kFewTurned), a.inverse ? -1.0f : 1.0f};
+            a.Hq + 2 * a.Hkv, a.D, threads_a_row(a.rows, kFewTurned), a.inverse ? -1.0f : 1.0f, a.clear};
     note_kernels(kRope);
     pick(a.dtype, a.rope, k, [&](auto DT, auto L, auto V) {
         hipLaunchKernelGGL((rope_kernel<decltype(DT)::value, decltype(L)::value, decltype(V)::value>), dim3(row_blocks(a.rows, kFewTurned)),

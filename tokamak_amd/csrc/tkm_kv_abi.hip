@@ -93,7 +93,8 @@ TKM_ATTN_API int tkm_attn_rope_rows(const tkm_attn_rope* rope, const void* in, l
         return fail(TKM_ATTN_EUNSUPPORTED, "dtype %d (supported: TKM_ATTN_F16, TKM_ATTN_BF16)", dtype);
     const int rc = check_rope(rope, D);
     if (rc) return rc;
-    if (inverse != 0 && inverse != 1) return fail(TKM_ATTN_EINVAL, "inverse must be 0 or 1, got %d", inverse);
+    if ((inverse & ~TKM_ROPE_CLEAR) != 0 && (inverse & ~TKM_ROPE_CLEAR) != 1)
+        return fail(TKM_ATTN_EINVAL, "inverse must be 0 or 1 (and TKM_ROPE_CLEAR), got %d", inverse);
     if (!pos && S < 1) return fail(TKM_ATTN_EINVAL, "without positions S=%d must be positive", S);
     const double width = ((double)Hq + 2.0 * Hkv) * D;
     if (width > 1073741824.0) return fail(TKM_ATTN_EUNSUPPORTED, "rows are too wide");
@@ -105,7 +106,7 @@ TKM_ATTN_API int tkm_attn_rope_rows(const tkm_attn_rope* rope, const void* in, l
     if (!aligned(in, 16) || !aligned(out, 16) || !aligned(pos, 4))
         return fail(TKM_ATTN_EALIGN, "in and out must be 16-byte aligned, pos 4-byte");
     if (!tkm::rows_fit(nullptr, rows)) return fail(TKM_ATTN_EUNSUPPORTED, "grid too large");
-    const tkm::RopeArgs a{*rope, in, in_stride, out, out_stride, pos, S, rows, Hq, Hkv, D, dtype, inverse, stream};
+    const tkm::RopeArgs a{*rope, in, in_stride, out, out_stride, pos, S, rows, Hq, Hkv, D, dtype, inverse & 1, inverse & TKM_ROPE_CLEAR, stream};
     if (tkm::launch_rope(a)) return fail(TKM_ATTN_ELAUNCH, "rope: kernel launch failed");
     return TKM_ATTN_OK;
 }
