@@ -2,9 +2,10 @@
 //
 //   (x0, x1) -> factor (x0 cos a - x1 sin a, x0 sin a + x1 cos a),  a = pos * turns_i * 2^-64 of a circle
 //
-// An angle is the low 64 bits of pos * turns_i, of which the upper 32 are kept (two 32-bit products): off by 2^-33
-// of a circle whatever the position is.  A row's rot/2 sines and cosines are formed once, in fp32, and shared by its
-// heads through LDS; products and sums are fp32, rounded once on the way out.
+// An angle is the low 64 bits of pos * turns_i, of which the upper 32 are kept (two 32-bit products) and rounded to fp32:
+// cut by less than 2^-32 of a circle and rounded by 2^-26 at most, whatever the position is.  A row's rot/2 sines and
+// cosines are formed once, in fp32, and shared by its heads through LDS; products and sums are fp32, rounded once on the
+// way out.
 //
 // Both kernels move data and are bound by HBM, or by the launch where rows are few.  A thread has a chunk of 8 dims, 16
 // bytes, of one head at a time, and forms its side of the pairs; a head's chunks are one wave's, at one time, which

@@ -3,8 +3,9 @@
  *
  * A pair's frequency is kept as the part of a circle that it turns by a position, in units of 2^-64:
  * pos * turns then wraps around just as the angle does, so that the kernels form the angle of any
- * position by integer products, exactly.  In long double (64 bits of mantissa): a frequency of 1 radian
- * is off by 2^-66 of a circle, at position 2^31 by 2^-35.
+ * position by integer products, exactly.  In long double (64 bits of mantissa): a frequency of at most 1
+ * radian, 0.16 of a circle, is formed in up to 16 roundings of 2^-64 of itself and cut to whole units, so that
+ * it is off by less than 2^-62 of a circle (plain ones by less than 2^-64), at position 2^31 by 2^-31 (2^-33).
  */
 #include <math.h>
 #include <string.h>
