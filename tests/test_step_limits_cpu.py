@@ -23,3 +23,13 @@ def test_rope_knows_no_other_flags(inverse):
 @pytest.mark.parametrize("inverse", [256, 257])
 def test_rope_takes_the_flag(inverse):
     assert call_rope(inverse=inverse, rows=0, x=None, y=None) == OK
+
+
+@pytest.mark.parametrize("kw", [{}, {"scaling": "yarn", "scale": 4.0}, {"freqs": [1.0] * 32}])
+def test_rope_factors_that_vanish_in_fp32(kw):
+    """They would make every rotated dim 0; 0 itself stands for the scaling's own."""
+    for factor in (1e-60, 7e-46):          # half of the least fp32, and below: rounded to 0
+        with pytest.raises(attn.AttnError, match="factor"):
+            attn.Rope(64, factor=factor, **kw)
+    assert attn.Rope(64, factor=1e-45, **kw).factor > 0.0
+    assert attn.Rope(64, factor=0.0, **kw).factor == attn.Rope(64, **kw).factor

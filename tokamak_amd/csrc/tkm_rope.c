@@ -20,8 +20,8 @@ static int check_shape(int rot, int layout, double factor) {
         return tkm_set_error(TKM_ATTN_EINVAL, "rot=%d must be even, 2 to 128", rot);
     if (layout != TKM_ROPE_HALVES && layout != TKM_ROPE_PAIRS)
         return tkm_set_error(TKM_ATTN_EINVAL, "layout %d (TKM_ROPE_HALVES, TKM_ROPE_PAIRS)", layout);
-    if (!(factor >= 0.0) || !isfinite((float)factor))
-        return tkm_set_error(TKM_ATTN_EINVAL, "factor must be finite and not negative");
+    if (!(factor >= 0.0) || !isfinite((float)factor) || (factor != 0.0 && (float)factor == 0.0f))
+        return tkm_set_error(TKM_ATTN_EINVAL, "factor must be 0 or positive, and neither infinite nor 0 in fp32");
     return TKM_ATTN_OK;
 }
 
