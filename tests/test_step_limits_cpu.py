@@ -1,5 +1,6 @@
 """Limits of a serving step's calls without a GPU, with results written out by hand."""
 import pytest
+import torch
 
 from step_cases import plan_ref
 from test_step_cpu import EINVAL, OK, call_rope
@@ -33,3 +34,16 @@ def test_rope_factors_that_vanish_in_fp32(kw):
             attn.Rope(64, factor=factor, **kw)
     assert attn.Rope(64, factor=1e-45, **kw).factor > 0.0
     assert attn.Rope(64, factor=0.0, **kw).factor == attn.Rope(64, **kw).factor
+
+
+@pytest.mark.parametrize("cls,name", [(attn.KvPages, "n_free"), (attn.KvPages, "held"), (attn.KvPlan, "slot"), (attn.KvPlan, "row_start")])
+def test_tensors_of_handles_are_written_not_replaced(cls, name):
+    """The C structs hold the first tensor's address, whatever the attribute says.  (Handles made without their
+    constructors, which take device tensors alone.)"""
+    h, t = cls.__new__(cls), torch.tensor([3, 4])
+    setattr(h, name, t)
+    setattr(h, name, getattr(h, name).add_(1))       # what h.name += 1 ends in
+    assert getattr(h, name) is t and t.tolist() == [4, 5]
+    with pytest.raises(AttributeError, match="cannot be replaced"):
+        setattr(h, name, torch.tensor([4, 5]))
+    assert getattr(h, name) is t

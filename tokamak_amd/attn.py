@@ -255,7 +255,17 @@ def gqa_bwd(qkv, o, dout, lse, B, S, Hq, Hkv, D, causal=True, kv_len=None, scale
     return dqkv
 
 
-class KvCache:
+class _Handle:
+    """Of tensors whose addresses a C struct holds: an attribute that has been set stays, for a tensor in its place would
+    leave the struct with the address of memory that may be freed."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__ and value is not self.__dict__[name]:     # c.kv_len += 1 ends in c.kv_len = c.kv_len
+            raise AttributeError(f"{name} cannot be replaced: write into the tensor")
+        super().__setattr__(name, value)
+
+
+class KvCache(_Handle):
     """A paged key-value cache over the caller's tensors (tkm_attn_kv, include/tkm_attn.h):
 
     k       [num_pages, Hkv, page/32, D/32, 32, 32]  float16 or bfloat16, blocks of 32 tokens x 32 dims
@@ -288,11 +298,6 @@ class KvCache:
         self._c = _Kv(_ptr(k), _ptr(v), _ptr(table), _ptr(kv_len), _ptr(weight), B, Hkv, D, page, max_pages, num_pages, dt)
         self._ref = ctypes.byref(self._c)
         self._ws = {}
-
-    def __setattr__(self, name, value):
-        if name in self.__dict__ and value is not self.__dict__[name]:     # c.kv_len += 1 ends in c.kv_len = c.kv_len
-            raise AttributeError(f"{name} cannot be replaced: write into the tensor")
-        super().__setattr__(name, value)
 
     @classmethod
     def empty(cls, B, max_pages, num_pages, Hkv, D, page=64, dtype=None, device="cuda", weights=False):
@@ -553,9 +558,10 @@ def _rope(x, rope, Hq, Hkv, D, pos, S, out, inverse, st):
     return out
 
 
-class KvPages:
+class KvPages(_Handle):
     """The pages of a pool that no sequence has, and how many each sequence has (tkm_attn_pages): free [num_pages]
-    int32, of which the first n_free [1] int32 are free, and held [B] int32.  The tensors stay the caller's."""
+    int32, of which the first n_free [1] int32 are free, and held [B] int32.  The tensors stay the caller's, and are
+    attributes here: write into them, do not replace them."""
 
     def __init__(self, free, n_free, held):
         dev = held.device
@@ -575,9 +581,9 @@ class KvPages:
                    torch.zeros(cache.B, dtype=torch.int32, device=dev))
 
 
-class KvPlan:
+class KvPlan(_Handle):
     """What a step does (tkm_attn_plan), written by kv_plan: n_new [B], row_start [B + 1], and per packed row seq, pos
-    [rows], all int32, and slot [rows] int64."""
+    [rows], all int32, and slot [rows] int64; write into them, do not replace them."""
 
     def __init__(self, n_new, row_start, seq, pos, slot):
         dev, B, rows = n_new.device, n_new.numel(), slot.numel()
