@@ -575,8 +575,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
             }
             wait_dma();
             __syncthreads();
-            auto step = [&](int t, auto Buf) __attribute__((always_inline)) {
-                const int buf = Buf;
+            for (int t = ta; t < te; ++t) {
+                const int buf = (t - ta) & 1;
                 int me = threadIdx.x;
                 if constexpr (ODD) asm volatile("" : "+v"(me));
                 if (ODD || t < it.alike || t >= it.alike_end) odd |= search(t, buf, me);
@@ -590,14 +590,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
                 }
                 wait_dma();
                 __syncthreads();
-            };
-            if constexpr (D == 64 || ODD) {       // one body: two would take more registers than three waves a SIMD leave
-                for (int t = ta; t < te; ++t) step(t, (t - ta) & 1);
-            } else {                              // 3% faster than one at 128 rows an item
-                for (int t = ta; t < te; t += 2) {
-                    step(t, std::integral_constant<int, 0>{});
-                    if (t + 1 < te) step(t + 1, std::integral_constant<int, 1>{});
-                }
             }
             return odd;
         };
