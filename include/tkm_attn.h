@@ -282,7 +282,9 @@ TKM_ATTN_API int tkm_attn_kv_append_rows(const tkm_attn_kv *kv, const tkm_attn_r
                                          int rows, int Hq, void *stream);
 
 /* Bytes of device workspace tkm_attn_chunk needs; 0 if none (short tables, few rows), also if it refuses
- * the arguments.  It holds nothing from call to call; calls that may overlap need one each. */
+ * the arguments.  It holds nothing from call to call; calls that may overlap need one each.
+ * Like the call's form, it goes by what the tables could hold, not by what sequences do: where they are
+ * short, tables of up to 2048 tokens (640 for few rows) spare them two launches, about 20 us. */
 TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int rows, int Hq);
 
 /* Attention of each sequence's new rows over its len[b] cached positions, their own among them: row i
@@ -296,10 +298,12 @@ TKM_ATTN_API size_t tkm_attn_chunk_workspace_bytes(const tkm_attn_kv *kv, int ro
  * must not overlap q.  Rows of no sequence stay as they are in o and lse.
  * A row that sees nothing gets O = 0, LSE = -inf.  What a row does not see has no part in it, whatever
  * it holds; what it sees of NaN and infinities acts as in tkm_attn_decode, and so do lengths and pages
- * outside their bounds.  Infinities and NaN among the values cost a second walk.  Values of more than
- * 2^100 may overflow in the sums, which hold weights of up to 2^16.
- * Scores, softmax and sums are fp32; the weights are multiplied with the values as 16-bit parts of together 22 bits (fp16)
- * or 24 (bf16), as in tkm_attn_decode.  Results do not depend on timing. */
+ * outside their bounds.  Infinities and NaN among the values cost a second walk.  No weights are gathered:
+ * positions that only these rows attend to keep the 0 that tkm_attn_kv_append_rows gave them, and
+ * tkm_attn_kv_evict drops them before all that tkm_attn_decode has added to, but for its sink and recent.
+ * Scores, softmax and sums are fp32; the weights are multiplied with the values as 16-bit parts of together
+ * 22 bits (fp16) or 24 (bf16), as in tkm_attn_decode.  The sums hold weights of up to 2^16: values of more
+ * than 2^100 may overflow in them.  Results do not depend on timing. */
 TKM_ATTN_API int tkm_attn_chunk(const tkm_attn_kv *kv, const void *q, long long q_stride, const int32_t *row_start,
                                 const int32_t *n_new, int rows, void *o, float *lse, int Hq, float scale, int causal,
                                 int window, void *workspace, size_t workspace_bytes, void *stream);

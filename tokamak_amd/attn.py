@@ -681,7 +681,7 @@ def gqa_chunk(q, cache, Hq, row_start=None, n_new=None, scale=None, causal=True,
     row_start[b] int32 on (a plan's; row_start None: at most rows / B from b * (rows / B), n_new None: rows / B), and the
     last of them stands at its last position.  causal: a row sees the positions up to its own, with a window only the last `window`
     of these.  Rows of no sequence stay as they are in out and lse (in new ones they hold anything); without rows
-    nothing is launched.
+    nothing is launched.  No weights are gathered: eviction by weight needs gqa_decode's add_weights.
     workspace: chunk_workspace_bytes(cache, rows, Hq) bytes, allocated for the call if not given."""
     st = _current(cache.device, stream)
     if st is None:

@@ -17,18 +17,22 @@
 // formed once more), and the 8 keep weights of down to 2^-22 of the row's largest in fp16's normal range.  P goes to the
 // second product in parts that hold what decoding (attn_decode.hip) keeps of it, two in fp16 (22 bits) and three in bf16
 // (24), so that a row has the same precision in either.  One part in fp16 and two in bf16 lost 2^-11 and 2^-16 of a P, and
-// took 929 us for 1226 (prompts in fp16, limited by the products' power), 309 for 365 (a mixed step in bf16).
+// took, on one card, 957 us for 1310 (prompts in fp16, limited by the products' power), and in bf16 321 for 392 (a mixed
+// step), 117 for 131 (13 rows over 131000 tokens), 61.5 for 71 (windows, 64 dims).
 //
 // Splitting: all items' tiles are numbered in one line, kv head after kv head, and every workgroup takes an equal
 // share, whatever the lengths are, which are read on the device: a first launch of one workgroup lists the items of a
 // kv head, the place where each share begins, and the items that no one workgroup has whole.  These leave pieces in
 // the workspace, which a third launch joins in the order of the tokens: results do not depend on timing.  Where items
 // are short, or fill the card, a workgroup has one, and there is one launch.  (Shares weighted by what a tile has of
-// rows were slower: on a full card a tile takes 2 us, be it one row's, from HBM, or 128 rows', whose keys are in L2.)
+// rows were slower: on a full card a tile took 2 us, with fewer parts of P, be it one row's, from HBM, or 128 rows', whose
+// keys are in L2.)
 //
-// What bounds it: for few rows HBM (13 tokens, 32 heads of 128 on 8, about 131000: 101 us for 537 MB, 5.3 TB/s; listing and
-// joining 15 more); for prompts of 128 dims products and exponentials one after the other (46 and 36% of the clocks at 1.86
-// GHz; 707 GFLOP seen, 854 done in tiles, in 940 us); at 64 dims the issue of exponentials and sums, three waves a SIMD, and a part's beginning and end.
+// What bounds it: for few rows HBM and, between two tiles, the products of the one or two waves that have rows (13 tokens,
+// 32 heads of 128 on 8, about 131000: 116 us for 537 MB, 4.6 TB/s; listing and joining 15 more); for prompts of 128 dims
+// products and vector instructions one after the other (52 and 39% of the clocks at 1.84 GHz; 849 GFLOP, 1281 with the second
+// product's parts, in 1270 to 1310 us); at 64 dims the issue of exponentials, sums and parts, three waves a SIMD, and a
+// part's beginning and end.
 //
 // 0 times an infinity or NaN is NaN, also where P is 0 because its row does not see the token, and an infinity times a part
 // of P that is 0 or negative is NaN where the whole of P makes it infinite.  So a tile that an item's rows do not see alike
@@ -51,7 +55,7 @@ namespace {
 constexpr int BM = 128;           // rows of an item
 constexpr int BN = 64;            // tokens of a tile
 constexpr int kWaves = 4;
-// Three or two workgroups on each compute unit (5 prompts in windows of 1024, 12 heads of 64: 63 and 71 us).
+// Three or two workgroups on each compute unit (5 prompts in windows of 1024, 12 heads of 64: 71 and 89 us).
 constexpr int workers_at(int D) { return D == 64 ? 768 : 512; }
 constexpr float kLift = 8.0f;
 constexpr float kSumMax = 65504.0f;
@@ -730,12 +734,14 @@ long long items_each(const tkm_attn_kv& kv, int rows, int Hq) { return ((long lo
 long long items_most(const tkm_attn_kv& kv, int rows, int Hq) { return items_each(kv, rows, Hq) + std::min<long long>(kv.B, rows); }
 
 // A workgroup an item, in one launch, of a grid laid out for all rows being one sequence's:
-//   where no item has more than 10 tiles, which take a lone workgroup about 1.4 us each (kernels, one launch or three: 4
-//     times 5 rows over up to 300 tokens 12 and 16 us, 500 15 and 16, 900 24 and 16);
+//   where no item has more than 10 tiles, which take a lone workgroup about 1.1 us each (kernels, one launch or three: 4
+//     times 5 rows over up to 300 tokens 12 and 16 us, 500 14 and 16, 900 21 and 16);
 //   where full items are workgroups enough for the card and the longest, by the table or the window, has a 16th as
-//     many tiles, and at most 32 (32 heads of 128, 4 prompts of up to 500 tokens 33 and 52 us, 1000 78 and 99, 1900 194
-//     and 216; 12 heads of 64, 5 prompts in windows of 256 36 and 53, 1024 68 and 76, 2048 110 and 109; but 64 rows
-//     over up to 990 57 and 45).
+//     many tiles, and at most 32 (32 heads of 128, fp16, 4 prompts of up to 500 tokens 35 and 56 us, 1000 80 and 99, 1900
+//     214 and 236; 12 heads of 64, bf16, 5 prompts in windows of 256 38 and 54, 1024 75 and 81, 2048 126 and 124; but 64 rows
+//     over 990, 33 and 29).
+// What sequences hold is known to the device alone: the same 4 prompts of 500 take the three launches, 55 us for 33 a call,
+// where the tables could hold 131072 tokens.
 constexpr long long kFewTiles = 10, kFewItems = 1024, kMoreTiles = 32, kMoreItems = 16384, kFill = 16;
 
 bool item_each(const tkm_attn_kv& kv, int rows, int Hq, int window) {

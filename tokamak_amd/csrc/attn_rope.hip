@@ -11,8 +11,8 @@
 // bytes, of one head at a time, and forms its side of the pairs; a head's chunks are one wave's, at one time, which
 // reads the other sides before it writes, so that rows may be rotated in place.  (With a pair's sides in one thread, stores
 // were as wide as the largest power of two in rot / 2: 16384 rows of 40 heads of 64 with 40 dims rotated took 41 us for
-// 27.)  A training batch of 8192 rows of 48 heads of 128: 45 us of operands from HBM, 4.4 TB/s; 7600 prompt rows of 28 heads
-// of 128 into the cache: 52 us, 4.4 TB/s.
+// 27.)  A training batch of 8192 rows of 48 heads of 128: 45 us of operands from HBM, 4.4 TB/s; 15011 prompt rows of 28 heads
+// of 128 into the cache: 51.5 us, 4.2 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "attn_common.h"
